@@ -187,7 +187,7 @@ def run(s):
 
 
 def _own_top(s):
-    leaf, weight = _layers().top_leaves(s["phi"], s["L"], s["k"], renormalize=s["renorm"])
+    leaf, weight = _layers().top_leaves(s["phi"], s["k"], num_leaves=s["L"], renormalize=s["renorm"])
     out = {"leaf": leaf, "weight": weight}
     if s["train"]:
         out["dphi"], = torch.autograd.grad(weight, s["phi"], s["dweight"])
