@@ -75,6 +75,20 @@ EXPORTS = {
     "bnpvi_kmeans_first_nested": (_i, [_p, _p, _p, _i, _i64, _p, _i, _p, _p, _p]),
     "bnpvi_path_distances": (_i, [_p, _p, _p, _i, _i64, _i, _p, _p, _i, _p, _p, _p]),
     "bnpvi_remap_columns": (_i, [_p, _p, _i, _p, _i, _i64, _i, _p, _p, _p]),
+    "bnpvi_top_leaves_max": (_i, []),
+    "bnpvi_top_leaves": (_i, [_p, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, _p]),
+    "bnpvi_top_leaves_backward": (_i, [_p, _p, _p, _p, _p, _i64, _i, _i, _i, _p, _i64, _i, _p]),
+    "bnpvi_leaf_sort_max_leaves": (_i, []),
+    "bnpvi_leaf_sort_workspace": (_i64, [_i64, _i]),
+    "bnpvi_leaf_sort": (_i, [_p, _p, _i64, _i, _p, _p, _p, _p, _i64, _p]),
+    "bnpvi_rows_to_leaves": (_i, [_p, _i, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _i64, _p]),
+    "bnpvi_rows_from_leaves": (_i, [_p, _i, _p, _i64, _p, _p, _p, _i, _i64, _i, _i, _p, _i64, _p]),
+    "bnpvi_rows_from_leaves_backward": (_i, [_p, _i, _p, _i64, _p, _i64, _p, _p, _p, _i, _i64, _i, _i, _p, _i64, _p, _p]),
+    "bnpvi_dense_workspace": (_i64, [_i, _i64, _i64, _i64, _i, _i]),
+    "bnpvi_dense": (_i, [_p, _i, _p, _i64, _p, _i64, _i64, _p, _i64, _i, _p, _i64, _p, _i, _i64, _i64, _i64, _p, _i64,
+                         _p, _i64, _p, _i64, _p]),
+    "bnpvi_dense_backward": (_i, [_p, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i, _i64, _i64, _i64, _p,
+                                  _i64, _p, _p, _p, _i64, _p, _i64, _p]),
 }
 
 for _name, (_res, _args) in EXPORTS.items():

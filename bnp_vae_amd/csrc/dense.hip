@@ -1,0 +1,551 @@
+// Entry points of the dense product (dense_kernels.h) and the passes around its matrix kernel: the row tiles of the
+// groups, dz = dy act'(z) with the bias gradient's partial sums, and the sums over partial results.
+#include "dense_kernels.h"
+
+namespace bnpvi {
+
+// ---- row tiles of the groups ---------------------------------------------------------------------------------------
+// map[t] = {group, first row, end row}; rows in front of the first and behind the last group make tiles of group -1,
+// unused entries are empty.  first[g] = first tile of group g (first[G] = their number).  One workgroup: a scan of the
+// groups' tile counts, then every tile finds its group by bisection.
+__device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+__global__ __launch_bounds__(1024) void row_tiles_kernel(const int32_t* __restrict__ offsets, int G, int64_t M, int tile, int64_t ntiles,
+                                                         int4* __restrict__ map, int32_t* __restrict__ first) {
+  extern __shared__ int32_t start[];        // [G + 1] | [16]
+  int32_t* red = start + G + 1;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int per = (G + 1023) / 1024, g0 = min(G, t * per), g1 = min(G, g0 + per);
+  int32_t sum = 0;
+  for (int g = g0; g < g1; ++g) {
+    const int64_t lo = clamp_row(offsets[g], 0, M), hi = clamp_row(offsets[g + 1], lo, M);
+    sum += (int32_t)((hi - lo + tile - 1) / tile);
+  }
+  int32_t inc = sum;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(inc, d);
+    if (lane >= d) inc += o;
+  }
+  if (lane == 63) red[w] = inc;
+  __syncthreads();
+  int32_t run = inc - sum;
+  for (int i = 0; i < w; ++i) run += red[i];
+  for (int g = g0; g < g1; ++g) {
+    const int64_t lo = clamp_row(offsets[g], 0, M), hi = clamp_row(offsets[g + 1], lo, M);
+    start[g] = run;
+    run += (int32_t)((hi - lo + tile - 1) / tile);
+  }
+  if (g1 == G && g0 < g1) start[G] = run;
+  __syncthreads();
+  if (first != nullptr)
+    for (int g = t; g <= G; g += 1024) first[g] = start[g];
+  const int32_t used = start[G];
+  const int64_t head = clamp_row(offsets[0], 0, M), tail = clamp_row(offsets[G], 0, M);
+  const int64_t nhead = (head + tile - 1) / tile;
+  for (int64_t i = t; i < ntiles; i += 1024) {
+    int4 m = {-1, 0, 0, 0};
+    if (i < used) {
+      int lo = 0, hi = G;                    // the last group that starts at or before tile i; empty groups share a start
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= i)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const int64_t r0 = clamp_row(offsets[lo], 0, M), r1 = clamp_row(offsets[lo + 1], r0, M);
+      const int64_t r = r0 + (i - start[lo]) * tile;
+      if (r >= r0 && r < r1) {               // always, where the offsets ascend
+        m.x = lo;
+        m.y = (int)r;
+        m.z = (int)(r + tile < r1 ? r + tile : r1);
+      }
+    } else {
+      const int64_t j = i - used;
+      const int64_t r0 = j < nhead ? j * tile : tail + (j - nhead) * tile, r1 = j < nhead ? head : M;
+      if (r0 < r1) {
+        m.y = (int)r0;
+        m.z = (int)(r0 + tile < r1 ? r0 + tile : r1);
+      }
+    }
+    map[i] = m;
+  }
+}
+
+// ---- dz, residual gradient, partial sums of the bias gradient --------------------------------------------------------
+// One workgroup: a row tile (of one group) x 256 columns.  dz = dy * d rounded once; the bias gradient adds the
+// unrounded products: per thread over its rows, then the eight row threads of a column in order.  dres (or nullptr):
+// dy, 0 in the rows of no group.
+constexpr int kDzRows = 128;
+
+template <typename T, int E>
+__global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64_t lddy, const typename Deriv<T>::type* __restrict__ d,
+                                                 int64_t ldd, const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz,
+                                                 int64_t lddz, T* __restrict__ dres, int64_t lddres, float* __restrict__ part) {
+  constexpr int CT = 32;                     // threads across
+  __shared__ float sums[8][CT * E + 1];
+  const int tx = threadIdx.x % CT, ty = threadIdx.x / CT;
+  int64_t r0 = (int64_t)blockIdx.x * kDzRows, r1 = min(M, r0 + kDzRows);
+  int g = 0;
+  if (map != nullptr) {
+    const int4 m = map[blockIdx.x];
+    g = m.x;
+    r0 = m.y;
+    r1 = m.z;
+  }
+  const int c = ((int)blockIdx.y * CT + tx) * E;
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  if (c < n) {
+    for (int64_t r = r0 + ty; r < r1; r += 8) {
+      float v[E], o[E];
+      if (g < 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+        if (dres != nullptr) store_vec<T, E>(dres + r * lddres + c, o);
+        continue;
+      }
+      load_vec<T, E>(dy + r * lddy + c, v);
+      if (dres != nullptr) store_vec<T, E>(dres + r * lddres + c, v);
+      if (d != nullptr) {
+        load_vec<typename Deriv<T>::type, E>(d + r * ldd + c, o);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= o[e];
+        if (dz != nullptr) store_vec<T, E>(dz + r * lddz + c, v);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += v[e];
+    }
+  }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < E; ++e) sums[ty][tx * E + e] = acc[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < CT * E; i += 256) {
+    const int col = (int)blockIdx.y * CT * E + i;
+    if (col < n) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += sums[k][i];
+      part[(int64_t)blockIdx.x * n + col] = s;
+    }
+  }
+}
+
+// db[g] = sum over the group's row tiles, 16 interleaved partial sums per column, added in order
+template <typename T>
+__global__ __launch_bounds__(1024) void db_kernel(const float* __restrict__ part, const int32_t* __restrict__ first, int64_t tiles, int n,
+                                                  T* __restrict__ db) {
+  __shared__ float sums[16][64];
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, g = blockIdx.y, col = blockIdx.x * 64 + tx;
+  const int64_t t0 = first != nullptr ? clamp_row(first[g], 0, tiles) : 0;
+  const int64_t t1 = first != nullptr ? clamp_row(first[g + 1], t0, tiles) : tiles;
+  float acc = 0.f;
+  if (col < n)
+    for (int64_t t = t0 + ty; t < t1; t += 16) acc += part[t * n + col];
+  sums[ty][tx] = acc;
+  __syncthreads();
+  if (ty == 0 && col < n) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) acc += sums[k][tx];
+    db[(int64_t)g * n + col] = (T)acc;
+  }
+}
+
+// ---- sums over the splits of the reduce axis, in order -------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict__ slab, int splits, int64_t elems, int64_t groups,
+                                                        T* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems * groups; i += (int64_t)gridDim.x * 256) {
+    const int64_t g = i / elems, e = i % elems;
+    const float* p = slab + g * splits * elems + e;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += p[k * elems];
+    out[i] = (T)s;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void split_epilogue_kernel(const float* __restrict__ slab, int splits, const GemmArgs a) {
+  typedef typename Deriv<T>::type DT;
+  const int64_t elems = a.rows * a.cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / a.cols, col = i % a.cols;
+    float z = 0.f;
+    for (int k = 0; k < splits; ++k) z += slab[k * elems + i];
+    if (a.bias != nullptr) z += (float)reinterpret_cast<const T*>(a.bias)[col];
+    float y, d;
+    activate(a.act, z, y, d);
+    if (a.res != nullptr) y += (float)reinterpret_cast<const T*>(a.res)[row * a.ldres + col];
+    if (a.dact != nullptr) reinterpret_cast<DT*>(a.dact)[row * a.lddact + col] = (DT)d;
+    reinterpret_cast<T*>(a.C)[row * a.ldc + col] = (T)y;
+  }
+}
+
+// ---- sizes of one call -----------------------------------------------------------------------------------------------
+struct GemmPlan {
+  int tile, splits;
+  int64_t row_tiles;
+  int col_tiles;
+  size_t slab;                 // bytes
+};
+
+static void tile_size(int tile, int& br, int& bc) {
+  br = tile == kTile128 || tile == kTileTall ? 128 : tile == kTile64 ? 64 : 32;
+  bc = tile == kTile128 || tile == kTileFlat ? 128 : tile == kTile64 ? 64 : 32;
+}
+
+// rows x cols of output, `K` summed; grouped: G groups along the rows (kFwd, kDx) or along the sum (kDw)
+static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64_t K, bool grouped, int G) {
+  GemmPlan p;
+  const int bk = 128 / dtype_bytes(dtype);
+  const int64_t z = grouped ? G : 1;
+  const int64_t per_group = grouped && kind != kDw ? ceil_div(rows, G) : rows;
+  if (cols <= 32 && per_group > 32)
+    p.tile = kTileTall;
+  else if (per_group <= 32)
+    p.tile = kTileFlat;
+  else if (cols <= 64 || per_group <= 64)
+    p.tile = kTile64;
+  else
+    p.tile = ceil_div(rows, 128) * ceil_div(cols, 128) * (kind == kDw ? z : 1) >= 200 || K >= 8192 ? kTile128 : kTile64;
+  int br, bc;
+  tile_size(p.tile, br, bc);
+  p.row_tiles = ceil_div(rows, br) + (grouped && kind != kDw ? G + 2 : 0);
+  p.col_tiles = (int)ceil_div(cols, bc);
+  p.splits = 1;
+  const int64_t blocks = p.row_tiles * p.col_tiles * (kind == kDw ? z : 1);
+  if (!(grouped && kind != kDw)) {
+    // split the sum while that fills idle CUs: at least four stages a part
+    const int64_t per = kind == kDw && grouped ? ceil_div(K, G) : K;
+    int64_t s = blocks < 512 ? 512 / (blocks < 1 ? 1 : blocks) : 1;
+    s = std::min(s, per / (4 * bk));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+  }
+  p.slab = p.splits > 1 ? (size_t)z * p.splits * rows * cols * 4 : 0;
+  if (!(kind == kDw) && grouped) p.slab = 0;
+  return p;
+}
+
+static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+struct DensePlan {
+  GemmPlan fwd, dx, dw;
+  bool grouped;
+  int64_t dz_tiles;
+  // byte offsets of the workspace's parts
+  size_t fwd_map, fwd_slab, fwd_bytes;
+  size_t dz_map, dz_first, dx_map, part, dz, slab, bwd_bytes;
+};
+
+static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G) {
+  DensePlan p;
+  const int e = dtype_bytes(dtype);
+  p.grouped = G > 0;
+  p.fwd = gemm_plan(kFwd, dtype, M, n, K, p.grouped, G);
+  p.dx = gemm_plan(kDx, dtype, M, K, n, p.grouped, G);
+  p.dw = gemm_plan(kDw, dtype, n, K, M, p.grouped, G);
+  p.dz_tiles = ceil_div(M, kDzRows) + (p.grouped ? G + 2 : 0);
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t o = at;
+    at += up256(bytes);
+    return o;
+  };
+  p.fwd_map = take(p.grouped ? p.fwd.row_tiles * sizeof(int4) : 0);
+  p.fwd_slab = take(p.fwd.slab);
+  p.fwd_bytes = at;
+  at = 0;
+  p.dz_map = take(p.grouped ? p.dz_tiles * sizeof(int4) : 0);
+  p.dz_first = take(p.grouped ? (size_t)(G + 1) * 4 : 0);
+  p.dx_map = take(p.grouped ? p.dx.row_tiles * sizeof(int4) : 0);
+  p.part = take((size_t)p.dz_tiles * n * 4);
+  p.dz = take((size_t)M * n * e);
+  p.slab = take(std::max(p.dx.slab, p.dw.slab));
+  p.bwd_bytes = at;
+  return p;
+}
+
+// elements an access may take so that every row of the operand starts on it and the contiguous extent divides
+static int access_elems(const void* p, int64_t ld, int64_t group, int64_t extent, int e) {
+  const uint64_t all = (uint64_t)(uintptr_t)p | (uint64_t)(ld * e) | (uint64_t)(group * e) | (uint64_t)(extent * e);
+  const int bytes = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+  return bytes / e;
+}
+
+static bool wide(const void* p, int64_t ld, int e) { return p == nullptr || ((uintptr_t)p % 16 == 0 && ld * e % 16 == 0); }
+
+static int run_gemm(int kind, int dtype, const GemmPlan& p, GemmArgs& a, int device, hipStream_t s) {
+  const int e = dtype_bytes(dtype);
+  a.rv = access_elems(a.R, a.ldr, 0, kind == kDw ? a.rows : a.K, e);
+  a.sv = access_elems(a.S, a.lds, a.s_group, kind == kFwd ? a.K : a.cols, e);
+  a.row_tiles = p.row_tiles;
+  a.col_tiles = p.col_tiles;
+  a.splits = p.splits;
+  const bool direct = a.rv * e == 16 && a.sv * e == 16;
+  return dtype == BNPVI_F32    ? launch_gemm_f32(kind, p.tile, direct, a, device, s)
+         : dtype == BNPVI_BF16 ? launch_gemm_bf16(kind, p.tile, direct, a, device, s)
+                               : launch_gemm_f16(kind, p.tile, direct, a, device, s);
+}
+
+static int row_tiles(const int32_t* offsets, int G, int64_t M, int tile, int64_t ntiles, void* map, void* first, int device,
+                     hipStream_t s) {
+  static LdsLimit limit;
+  const size_t lds = (size_t)(G + 1 + 16) * 4;
+  if (lds > 64 * 1024) BNPVI_HIP(limit.raise((const void*)row_tiles_kernel, device));
+  row_tiles_kernel<<<1, 1024, lds, s>>>(offsets, G, M, tile, ntiles, (int4*)map, (int32_t*)first);
+  BNPVI_LAUNCH_CHECK();
+  return BNPVI_OK;
+}
+
+static unsigned flat_grid(int64_t elems) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(elems, 256), 4096)); }
+
+template <typename T>
+static void launch_dz(const T* dy, int64_t lddy, const void* d, int64_t ldd, const int4* map, int64_t M, int n, int64_t tiles, T* dz,
+                      int64_t lddz, T* dres, int64_t lddres, float* part, hipStream_t s) {
+  typedef typename Deriv<T>::type DT;
+  const DT* dd = (const DT*)d;
+  const int e = (int)sizeof(T), de = (int)sizeof(DT);
+  const bool vec = n % 8 == 0 && wide(dy, lddy, e) && wide(dz, lddz, e) && wide(dres, lddres, e) && wide(d, ldd, de);
+  if (vec)
+    dz_kernel<T, 8><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 256)), 256, 0, s>>>(dy, lddy, dd, ldd, map, M, n, dz, lddz, dres,
+                                                                                       lddres, part);
+  else
+    dz_kernel<T, 1><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 32)), 256, 0, s>>>(dy, lddy, dd, ldd, map, M, n, dz, lddz, dres,
+                                                                                      lddres, part);
+}
+
+template <typename T>
+static void launch_db(const float* part, const int32_t* first, int64_t tiles, int n, int G, void* db, hipStream_t s) {
+  db_kernel<T><<<dim3((unsigned)ceil_div(n, 64), (unsigned)G), 1024, 0, s>>>(part, first, tiles, n, (T*)db);
+}
+
+template <typename T>
+static void launch_split_sum(const float* slab, int splits, int64_t elems, int64_t groups, void* out, hipStream_t s) {
+  split_sum_kernel<T><<<flat_grid(elems * groups), 256, 0, s>>>(slab, splits, elems, groups, (T*)out);
+}
+
+constexpr int64_t kMaxPitchBytes = int64_t(1) << 22;       // 256 rows of a tile stay below 2^31 bytes
+
+static int check_dense(const char* what, bnpvi_ctx* ctx, int dtype, int64_t M, int64_t K, int64_t n, int G, const int32_t* offsets) {
+  BNPVI_REQUIRE(ctx != nullptr, "%s: ctx is NULL", what);
+  BNPVI_REQUIRE(dtype_bytes(dtype) > 0, "%s: dtype %d unknown", what, dtype);
+  BNPVI_REQUIRE(M >= 0 && M <= INT32_MAX, "%s: M=%lld rows (0 .. 2^31 - 1)", what, (long long)M);
+  BNPVI_REQUIRE(K >= 1 && K <= (1 << 20) && n >= 1 && n <= (1 << 20), "%s: K=%lld, n=%lld (1 .. 2^20)", what, (long long)K, (long long)n);
+  BNPVI_REQUIRE(G >= 0 && G <= kSortMaxLeaves, "%s: G=%d groups (0 .. %d)", what, G, kSortMaxLeaves);
+  BNPVI_REQUIRE((G > 0) == (offsets != nullptr), "%s: G=%d groups need offsets, and only they do", what, G);
+  return BNPVI_OK;
+}
+
+static bool pitch_fits(int64_t ld, int64_t width, int dtype) {
+  return ld >= width && ld * dtype_bytes(dtype) <= kMaxPitchBytes;
+}
+
+}  // namespace bnpvi
+
+using namespace bnpvi;
+
+extern "C" {
+
+int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G, int backward) {
+  if (dtype_bytes(dtype) == 0 || M < 0 || M > INT32_MAX || K < 1 || K > (1 << 20) || n < 1 || n > (1 << 20) || G < 0 ||
+      G > kSortMaxLeaves)
+    return -1;
+  const DensePlan p = dense_plan(dtype, M, K, n, G);
+  return (int64_t)(backward ? p.bwd_bytes : p.fwd_bytes);
+}
+
+int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const void* bias,
+                int64_t bias_group, int activation, const void* residual, int64_t ldres, const int32_t* offsets, int G, int64_t M,
+                int64_t K, int64_t n, void* y, int64_t ldy, void* dact, int64_t lddact, void* work, int64_t work_bytes, void* stream) {
+  const int rc = check_dense("bnpvi_dense", ctx, dtype, M, K, n, G, offsets);
+  if (rc) return rc;
+  BNPVI_REQUIRE(activation >= BNPVI_ACT_NONE && activation <= BNPVI_ACT_GELU, "bnpvi_dense: activation %d unknown", activation);
+  BNPVI_REQUIRE(pitch_fits(ldx, K, dtype) && pitch_fits(ldw, K, dtype),
+                "bnpvi_dense: pitches x %lld, w %lld for K=%lld (at least K, at most 4 MiB)", (long long)ldx, (long long)ldw, (long long)K);
+  BNPVI_REQUIRE(ldy >= n && (!residual || ldres >= n) && (!dact || lddact >= n), "bnpvi_dense: pitch of y, residual or dact below n=%lld",
+                (long long)n);
+  if (M == 0) return BNPVI_OK;
+  BNPVI_REQUIRE(x && w && y, "bnpvi_dense: NULL device pointer");
+  const DensePlan p = dense_plan(dtype, M, K, n, G);
+  BNPVI_REQUIRE(work_bytes >= (int64_t)p.fwd_bytes && (p.fwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
+                "bnpvi_dense: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes, (long long)p.fwd_bytes);
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  const int e = dtype_bytes(dtype), de = dtype == BNPVI_BF16 ? 2 : 4;
+  char* wk = (char*)work;
+  GemmArgs a = {};
+  a.R = x;
+  a.ldr = ldx;
+  a.S = w;
+  a.lds = ldw;
+  a.s_group = G > 1 ? w_group : 0;
+  a.rows = M;
+  a.cols = n;
+  a.K = K;
+  a.G = G;
+  a.C = y;
+  a.ldc = ldy;
+  a.bias = bias;
+  a.bias_group = G > 1 ? bias_group : 0;
+  a.res = residual;
+  a.ldres = ldres;
+  a.dact = dact;
+  a.lddact = lddact;
+  a.act = activation;
+  a.cvec = wide(y, ldy, e) && wide(residual, ldres, e) && wide(dact, lddact, de) && (dact == nullptr || de == 4 || lddact % 8 == 0) &&
+           (e == 4 || ldy % 8 == 0);
+  if (G > 0) {
+    int br, bc;
+    tile_size(p.fwd.tile, br, bc);
+    const int r = row_tiles(offsets, G, M, br, p.fwd.row_tiles, wk + p.fwd_map, nullptr, ctx->device, s);
+    if (r) return r;
+    a.map = (const int4*)(wk + p.fwd_map);
+  }
+  if (p.fwd.slab) a.slab = (float*)(wk + p.fwd_slab);
+  const int r = run_gemm(kFwd, dtype, p.fwd, a, ctx->device, s);
+  if (r) return r;
+  if (p.fwd.slab) {
+    const unsigned g = flat_grid(M * n);
+    if (dtype == BNPVI_F32)
+      split_epilogue_kernel<float><<<g, 256, 0, s>>>(a.slab, p.fwd.splits, a);
+    else if (dtype == BNPVI_BF16)
+      split_epilogue_kernel<bf16_t><<<g, 256, 0, s>>>(a.slab, p.fwd.splits, a);
+    else
+      split_epilogue_kernel<f16_t><<<g, 256, 0, s>>>(a.slab, p.fwd.splits, a);
+    BNPVI_LAUNCH_CHECK();
+  }
+  return BNPVI_OK;
+}
+
+int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy, const void* dact, int64_t lddact, const void* x,
+                         int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const int32_t* offsets, int G, int64_t M, int64_t K,
+                         int64_t n, void* dx, int64_t lddx, void* dw, void* db, void* dres, int64_t lddres, void* work,
+                         int64_t work_bytes, void* stream) {
+  const int rc = check_dense("bnpvi_dense_backward", ctx, dtype, M, K, n, G, offsets);
+  if (rc) return rc;
+  BNPVI_REQUIRE(pitch_fits(lddy, n, dtype) && (!dact || lddact >= n) && (!dx || (pitch_fits(ldw, K, dtype) && lddx >= K)) &&
+                    (!dw || pitch_fits(ldx, K, dtype)) && (!dres || lddres >= n),
+                "bnpvi_dense_backward: a row pitch is below its width, or above 4 MiB");
+  const DensePlan p = dense_plan(dtype, M, K, n, G);
+  BNPVI_REQUIRE(work_bytes >= (int64_t)p.bwd_bytes && (p.bwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
+                "bnpvi_dense_backward: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes,
+                (long long)p.bwd_bytes);
+  BNPVI_REQUIRE(M == 0 || (dy && (!dx || w) && (!dw || x)), "bnpvi_dense_backward: NULL device pointer");
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  const int e = dtype_bytes(dtype);
+  const int groups = G > 0 ? G : 1;
+  char* wk = (char*)work;
+  int r = BNPVI_OK;
+  const int4* dz_map = nullptr;
+  int32_t* first = nullptr;
+  const bool need_dz = (dact != nullptr && (dx || dw)) || db || dres;
+  const bool none = M == 0;
+  if (need_dz && G > 0) {
+    first = (int32_t*)(wk + p.dz_first);
+    dz_map = (const int4*)(wk + p.dz_map);
+    r = row_tiles(offsets, G, M, kDzRows, p.dz_tiles, wk + p.dz_map, first, ctx->device, s);
+    if (r) return r;
+  }
+  const void* dz = dy;
+  int64_t lddz = lddy;
+  float* part = db ? (float*)(wk + p.part) : nullptr;
+  if (need_dz && !none) {
+    void* out = dact ? (void*)(wk + p.dz) : nullptr;
+    if (dtype == BNPVI_F32)
+      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, n, (float*)dres, lddres, part, s);
+    else if (dtype == BNPVI_BF16)
+      launch_dz<bf16_t>((const bf16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (bf16_t*)out, n, (bf16_t*)dres, lddres, part,
+                        s);
+    else
+      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, n, (f16_t*)dres, lddres, part, s);
+    BNPVI_LAUNCH_CHECK();
+    if (dact) {
+      dz = out;
+      lddz = n;
+    }
+  }
+  if (db) {
+    const int64_t tiles = none ? 0 : p.dz_tiles;
+    if (dtype == BNPVI_F32)
+      launch_db<float>(part, first, tiles, (int)n, groups, db, s);
+    else if (dtype == BNPVI_BF16)
+      launch_db<bf16_t>(part, first, tiles, (int)n, groups, db, s);
+    else
+      launch_db<f16_t>(part, first, tiles, (int)n, groups, db, s);
+    BNPVI_LAUNCH_CHECK();
+  }
+  if (dx && !none) {
+    GemmArgs a = {};
+    a.R = dz;
+    a.ldr = lddz;
+    a.S = w;
+    a.lds = ldw;
+    a.s_group = G > 1 ? w_group : 0;
+    a.rows = M;
+    a.cols = K;
+    a.K = n;
+    a.G = G;
+    a.C = dx;
+    a.ldc = lddx;
+    a.cvec = wide(dx, lddx, e);
+    if (G > 0) {
+      int br, bc;
+      tile_size(p.dx.tile, br, bc);
+      r = row_tiles(offsets, G, M, br, p.dx.row_tiles, wk + p.dx_map, nullptr, ctx->device, s);
+      if (r) return r;
+      a.map = (const int4*)(wk + p.dx_map);
+    }
+    if (p.dx.slab) a.slab = (float*)(wk + p.slab);
+    r = run_gemm(kDx, dtype, p.dx, a, ctx->device, s);
+    if (r) return r;
+    if (p.dx.slab) {
+      // no epilogue: a plain sum over the splits into rows of pitch lddx
+      GemmArgs b = a;
+      b.act = BNPVI_ACT_NONE;
+      const unsigned g = flat_grid(M * K);
+      if (dtype == BNPVI_F32)
+        split_epilogue_kernel<float><<<g, 256, 0, s>>>(a.slab, p.dx.splits, b);
+      else if (dtype == BNPVI_BF16)
+        split_epilogue_kernel<bf16_t><<<g, 256, 0, s>>>(a.slab, p.dx.splits, b);
+      else
+        split_epilogue_kernel<f16_t><<<g, 256, 0, s>>>(a.slab, p.dx.splits, b);
+      BNPVI_LAUNCH_CHECK();
+    }
+  }
+  if (dw) {
+    GemmArgs a = {};
+    a.R = dz;
+    a.ldr = lddz;
+    a.S = x;
+    a.lds = ldx;
+    a.rows = n;
+    a.cols = K;
+    a.K = M;
+    a.G = groups;
+    a.offsets = offsets;
+    a.C = dw;
+    a.ldc = K;
+    a.c_group = n * K;
+    a.cvec = wide(dw, K, e) && (groups == 1 || n * K * e % 16 == 0);
+    if (p.dw.slab) a.slab = (float*)(wk + p.slab);
+    r = run_gemm(kDw, dtype, p.dw, a, ctx->device, s);
+    if (r) return r;
+    if (p.dw.slab) {
+      if (dtype == BNPVI_F32)
+        launch_split_sum<float>(a.slab, p.dw.splits, n * K, groups, dw, s);
+      else if (dtype == BNPVI_BF16)
+        launch_split_sum<bf16_t>(a.slab, p.dw.splits, n * K, groups, dw, s);
+      else
+        launch_split_sum<f16_t>(a.slab, p.dw.splits, n * K, groups, dw, s);
+      BNPVI_LAUNCH_CHECK();
+    }
+  }
+  return BNPVI_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,649 @@
+// From responsibilities to rows in leaf order and back: the k likeliest leaves of every frame, the stable counting
+// sort of the (frame, choice) slots by leaf, the copy of frames' rows into that order and the weighted sum back, each
+// with its gradient.  All of it is bound by memory; no kernel here adds with atomics on floating-point values, so
+// every result has the same bits on every launch.
+#include "layers_common.h"
+
+namespace bnpvi {
+
+// ------------------------------------------------------------------------------------------------------------------
+// Top leaves.  A row is read once, 16 bytes a lane where it is aligned; LPR lanes share a row (a wave holds 64 / LPR
+// rows), each keeps its own K best in order, then K rounds of a maximum over the LPR lanes take the best heads off.
+// Ties: a lane visits its columns in ascending order and only a larger value moves an earlier one down; between
+// lanes the lowest column among the equal heads wins.  What is not a finite positive number is never taken.
+template <int K>
+struct Best {
+  float v[K];
+  int i[K];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      v[j] = 0.f;
+      i[j] = 0x7fffffff;
+    }
+  }
+  __device__ __forceinline__ void add(float x, int col) {
+    if (!(x > v[K - 1]) || !(x < __builtin_inff())) return;
+    v[K - 1] = x;
+    i[K - 1] = col;
+#pragma unroll
+    for (int j = K - 1; j > 0; --j) {
+      const bool up = v[j] > v[j - 1];
+      const float a = v[j - 1], b = v[j];
+      const int ia = i[j - 1], ib = i[j];
+      v[j - 1] = up ? b : a;
+      v[j] = up ? a : b;
+      i[j - 1] = up ? ib : ia;
+      i[j] = up ? ia : ib;
+    }
+  }
+  __device__ __forceinline__ void pop() {
+#pragma unroll
+    for (int j = 0; j + 1 < K; ++j) {
+      v[j] = v[j + 1];
+      i[j] = i[j + 1];
+    }
+    v[K - 1] = 0.f;
+    i[K - 1] = 0x7fffffff;
+  }
+};
+
+template <int K, int LPR, int VEC>
+__global__ __launch_bounds__(256) void top_leaves_kernel(const float* __restrict__ phi, int64_t ldphi, int64_t N, int L, int k,
+                                                         int renorm, int32_t* __restrict__ leaf, float* __restrict__ weight,
+                                                         float* __restrict__ total) {
+  constexpr int RPB = 256 / LPR;
+  const int sub = threadIdx.x % LPR, r = threadIdx.x / LPR;
+  for (int64_t n0 = (int64_t)blockIdx.x * RPB; n0 < N; n0 += (int64_t)gridDim.x * RPB) {
+    const int64_t n = n0 + r;
+    const bool live = n < N;
+    Best<K> best;
+    best.clear();
+    if (live) {
+      const float* row = phi + n * ldphi;
+      for (int c = sub * VEC; c < L; c += LPR * VEC) {
+        if (VEC == 4) {
+          const f32x4 q = *reinterpret_cast<const f32x4*>(row + c);    // c + 3 < ldphi: columns from L on are skipped
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < L) best.add(q[e], c + e);
+        } else {
+          best.add(row[c], c);
+        }
+      }
+    }
+    float myv = 0.f;
+    int myi = -1;
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      if (j < k) {
+        const float m = lanes_max<LPR>(best.v[0]);
+        const int at = lanes_min<LPR>(best.v[0] == m ? best.i[0] : 0x7fffffff);
+        if (best.i[0] == at) best.pop();      // columns are distinct: one lane of the row holds it (or all are empty)
+        if (sub == j) {                       // K <= 8 <= LPR: one lane a choice
+          myv = m;
+          myi = m > 0.f ? at : -1;
+        }
+        sum += (double)m;
+      }
+    }
+    if (live) {
+      if (sub < k) {
+        leaf[n * k + sub] = myi;
+        weight[n * k + sub] = renorm ? (sum > 0.0 ? (float)((double)myv / sum) : 0.f) : myv;
+      }
+      if (total != nullptr && sub == 0) total[n] = (float)sum;
+    }
+  }
+}
+
+template <int LPR, int VEC>
+__global__ __launch_bounds__(256) void top_leaves_bwd_kernel(const int32_t* __restrict__ leaf, const float* __restrict__ weight,
+                                                             const float* __restrict__ total, const float* __restrict__ dweight,
+                                                             int64_t N, int L, int k, int renorm, float* __restrict__ dphi,
+                                                             int64_t ld, int cols) {
+  constexpr int RPB = 256 / LPR;
+  const int sub = threadIdx.x % LPR, r = threadIdx.x / LPR;
+  for (int64_t n = (int64_t)blockIdx.x * RPB + r; n < N; n += (int64_t)gridDim.x * RPB) {
+    int at[kTopMax];
+    float g[kTopMax];
+    double dot = 0.0;
+#pragma unroll
+    for (int j = 0; j < kTopMax; ++j) {
+      at[j] = -1;
+      g[j] = 0.f;
+      if (j < k) {
+        at[j] = leaf[n * k + j];
+        g[j] = dweight[n * k + j];
+        if (renorm && at[j] >= 0) dot += (double)g[j] * (double)weight[n * k + j];
+      }
+    }
+    if (renorm) {
+      const float s = total[n];
+#pragma unroll
+      for (int j = 0; j < kTopMax; ++j) g[j] = s > 0.f ? (float)(((double)g[j] - dot) / (double)s) : 0.f;
+    }
+    float* row = dphi + n * ld;
+    for (int c = sub * VEC; c < cols; c += LPR * VEC) {
+      f32x4 q = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kTopMax; ++j) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (at[j] == c + e) q[e] = g[j];
+      }
+      if (VEC == 4)
+        *reinterpret_cast<f32x4*>(row + c) = q;
+      else
+        row[c] = q[0];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Stable counting sort of M slots by leaf, slots without a leaf behind the last one (bin L).  A workgroup owns a
+// contiguous chunk, each of its W waves a contiguous part of it.  Counting is order-free (integer LDS adds).  Placing
+// keeps the order: a wave takes 64 slots at a time, finds the lanes that hold the same leaf by one ballot per bit of
+// the leaf number, and the lowest of them advances that leaf's place in the wave's own LDS row -- no wave writes
+// another's row, so nothing is added atomically and the result is the stable order itself.
+__device__ __forceinline__ int bin_of(int32_t l, int L) { return (uint32_t)l < (uint32_t)L ? l : L; }
+
+__global__ __launch_bounds__(256) void leaf_count_kernel(const int32_t* __restrict__ leaf, int64_t M, int L, int64_t chunk,
+                                                         int32_t* __restrict__ hist) {
+  extern __shared__ int32_t cnt[];
+  const int B = L + 1;
+  for (int i = threadIdx.x; i < B; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  const int64_t lo = (int64_t)blockIdx.x * chunk, hi = min(M, lo + chunk);
+  for (int64_t s = lo + threadIdx.x; s < hi; s += blockDim.x) atomicAdd(&cnt[bin_of(leaf[s], L)], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i < B; i += blockDim.x) hist[(int64_t)blockIdx.x * B + i] = cnt[i];
+}
+
+// hist[b][bin] -> slots of that bin in the chunks before b; totals[bin] = slots of that bin.  64 bins a workgroup, 16
+// waves that share the chunks.
+__global__ __launch_bounds__(1024) void leaf_scan_kernel(int32_t* __restrict__ hist, int nb, int B, int32_t* __restrict__ totals) {
+  __shared__ int32_t part[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int bin = blockIdx.x * 64 + lane;
+  const int per = (nb + 15) / 16, b0 = min(nb, w * per), b1 = min(nb, b0 + per);
+  int32_t sum = 0;
+  if (bin < B)
+    for (int b = b0; b < b1; ++b) sum += hist[(int64_t)b * B + bin];
+  part[w][lane] = sum;
+  __syncthreads();
+  int32_t run = 0;
+  for (int i = 0; i < w; ++i) run += part[i][lane];
+  if (bin < B) {
+    if (w == 15) totals[bin] = run + sum;
+    for (int b = b0; b < b1; ++b) {
+      const int32_t h = hist[(int64_t)b * B + bin];
+      hist[(int64_t)b * B + bin] = run;
+      run += h;
+    }
+  }
+}
+
+// exclusive scan of src[0 .. B) into dst (LDS), whole workgroup; red: one int per wave
+__device__ void scan_bins(const int32_t* src, int32_t* dst, int B, int32_t* red) {
+  const int T = blockDim.x, t = threadIdx.x, lane = t & 63, w = t >> 6, W = T >> 6;
+  const int per = (B + T - 1) / T, i0 = min(B, t * per), i1 = min(B, i0 + per);
+  int32_t sum = 0;
+  for (int i = i0; i < i1; ++i) sum += src[i];
+  int32_t inc = sum;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(inc, d);
+    if (lane >= d) inc += o;
+  }
+  if (lane == 63) red[w] = inc;
+  __syncthreads();
+  int32_t run = inc - sum;
+  for (int i = 0; i < w && i < W; ++i) run += red[i];
+  for (int i = i0; i < i1; ++i) {
+    const int32_t v = src[i];               // src may be dst: each thread reads an entry before it writes it
+    dst[i] = run;
+    run += v;
+  }
+  __syncthreads();
+}
+
+// LDS: base[W][B] | red[W].  One workgroup (hist == nullptr) does the whole sort: counts, scan, places.
+__global__ __launch_bounds__(1024) void leaf_place_kernel(const int32_t* __restrict__ leaf, int64_t M, int L, int64_t chunk, int bits,
+                                                          const int32_t* __restrict__ hist, const int32_t* __restrict__ totals,
+                                                          int32_t* __restrict__ place, int32_t* __restrict__ order,
+                                                          int32_t* __restrict__ offsets) {
+  extern __shared__ int32_t lds[];
+  const int B = L + 1, W = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int32_t* mine = lds + (size_t)w * B;
+  int32_t* start = lds + (size_t)W * B;              // [B] first place of each bin
+  int32_t* red = start + B;
+  const int64_t lo = (int64_t)blockIdx.x * chunk, hi = min(M, lo + chunk);
+  const int64_t per = ((hi - lo + W - 1) / W + 63) / 64 * 64;
+  const int64_t s0 = min(hi, lo + w * per), s1 = min(hi, s0 + per);
+  for (int i = threadIdx.x; i < W * B; i += blockDim.x) lds[i] = 0;
+  __syncthreads();
+  for (int64_t s = s0 + lane; s < s1; s += 64) atomicAdd(&mine[bin_of(leaf[s], L)], 1);
+  __syncthreads();
+  if (hist != nullptr) {
+    scan_bins(totals, start, B, red);
+  } else {
+    for (int i = threadIdx.x; i < B; i += blockDim.x) {
+      int32_t sum = 0;
+      for (int v = 0; v < W; ++v) sum += lds[(size_t)v * B + i];
+      start[i] = sum;
+    }
+    __syncthreads();
+    scan_bins(start, start, B, red);
+  }
+  for (int i = threadIdx.x; i < B; i += blockDim.x) {
+    if (blockIdx.x == 0) offsets[i] = start[i];      // offsets[L] = slots with a leaf = first place without one
+    int32_t run = start[i] + (hist != nullptr ? hist[(int64_t)blockIdx.x * B + i] : 0);
+    for (int v = 0; v < W; ++v) {
+      const int32_t c = lds[(size_t)v * B + i];
+      lds[(size_t)v * B + i] = run;
+      run += c;
+    }
+  }
+  __syncthreads();
+  for (int64_t s = s0; s < s1; s += 64) {
+    const int64_t at = s + lane;
+    const bool live = at < s1;
+    const int bin = live ? bin_of(leaf[at], L) : 0;
+    uint64_t peers = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t one = __ballot((bin >> b) & 1);
+      peers &= ((bin >> b) & 1) ? one : ~one;
+    }
+    if (live) {
+      const int rank = __popcll(peers & ((1ull << lane) - 1));
+      const int32_t from = *(volatile int32_t*)&mine[bin];
+      const int32_t p = from + rank;
+      if (rank == 0) *(volatile int32_t*)&mine[bin] = from + (int32_t)__popcll(peers);
+      place[at] = p;
+      order[p] = (int32_t)at;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Rows into leaf order.  A frame's row is read once and written to its k places; rows of slots without a leaf, which
+// lie from offsets[L] on, are zeroed.  TX lanes share a row, `V` bytes a lane.
+template <typename V>
+__global__ __launch_bounds__(256) void rows_to_leaves_kernel(const char* __restrict__ x, int64_t ldx, int64_t N, int k, int nvec, int tx,
+                                                             const int32_t* __restrict__ place, const int32_t* __restrict__ kept_at,
+                                                             char* __restrict__ xs, int64_t ldxs) {
+  const int sub = threadIdx.x % tx, r = threadIdx.x / tx, rpb = 256 / tx;
+  const int32_t kept = *kept_at;
+  const int64_t M = N * k;
+  for (int64_t n = (int64_t)blockIdx.x * rpb + r; n < N; n += (int64_t)gridDim.x * rpb) {
+    const int32_t* pl = place + n * k;
+    for (int c = sub; c < nvec; c += tx) {
+      const V v = *reinterpret_cast<const V*>(x + n * ldx + (int64_t)c * sizeof(V));
+      for (int j = 0; j < k; ++j) {
+        const int32_t p = pl[j];
+        if ((uint32_t)p < (uint64_t)M) *reinterpret_cast<V*>(xs + (int64_t)p * ldxs + (int64_t)c * sizeof(V)) = p < kept ? v : V{};
+      }
+    }
+  }
+}
+
+// y[n] = sum_j w[n][j] ys[place[n][j]] over the slots with a leaf (w = 1 where `weight` is null: the gradient of the
+// copy above); fp32 sums in the order of j, one rounding.
+template <typename T, int E>
+__global__ __launch_bounds__(256) void rows_from_leaves_kernel(const T* __restrict__ ys, int64_t ldys, const int32_t* __restrict__ place,
+                                                               const float* __restrict__ weight, const int32_t* __restrict__ kept_at,
+                                                               int64_t N, int k, int D, int tx, T* __restrict__ y, int64_t ldy) {
+  const int sub = threadIdx.x % tx, r = threadIdx.x / tx, rpb = 256 / tx;
+  const int32_t kept = *kept_at;
+  for (int64_t n = (int64_t)blockIdx.x * rpb + r; n < N; n += (int64_t)gridDim.x * rpb) {
+    for (int c = sub * E; c < D; c += tx * E) {
+      float acc[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      for (int j = 0; j < k; ++j) {
+        const int32_t p = place[n * k + j];
+        if ((uint32_t)p >= (uint32_t)kept) continue;
+        const float w = weight != nullptr ? weight[n * k + j] : 1.f;
+        float v[E];
+        load_vec<T, E>(ys + (int64_t)p * ldys + c, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+      }
+      store_vec<T, E>(y + n * ldy + c, acc);
+    }
+  }
+}
+
+// dys[place[n][j]] = w[n][j] dy[n], dweight[n][j] = <dy[n], ys[place[n][j]]>; zeros for slots without a leaf.  The tx
+// lanes of a row add their parts of the inner product in a fixed order.
+template <typename T, int E>
+__global__ __launch_bounds__(256) void rows_from_leaves_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ ys,
+                                                                   int64_t ldys, const int32_t* __restrict__ place,
+                                                                   const float* __restrict__ weight, const int32_t* __restrict__ kept_at,
+                                                                   int64_t N, int k, int D, int tx, T* __restrict__ dys, int64_t lddys,
+                                                                   float* __restrict__ dweight) {
+  const int sub = threadIdx.x % tx, r = threadIdx.x / tx, rpb = 256 / tx;
+  const int32_t kept = *kept_at;
+  const int64_t M = N * k;
+  const int64_t steps = (N + (int64_t)gridDim.x * rpb - 1) / ((int64_t)gridDim.x * rpb);
+  for (int64_t it = 0; it < steps; ++it) {          // the same number of turns for every lane: the sums below use all of a row's
+    const int64_t n = (it * gridDim.x + blockIdx.x) * rpb + r;
+    for (int j = 0; j < k; ++j) {
+      float dot = 0.f;
+      if (n < N) {
+        const int32_t p = place[n * k + j];
+        const bool in = (uint32_t)p < (uint32_t)kept;
+        const float w = in ? weight[n * k + j] : 0.f;
+        if ((uint32_t)p < (uint64_t)M) {
+          for (int c = sub * E; c < D; c += tx * E) {
+            float g[E], o[E];
+            load_vec<T, E>(dy + n * lddy + c, g);
+            if (in) {
+              float v[E];
+              load_vec<T, E>(ys + (int64_t)p * ldys + c, v);
+#pragma unroll
+              for (int e = 0; e < E; ++e) dot = fmaf(g[e], v[e], dot);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = in ? w * g[e] : 0.f;
+            if (dys != nullptr) store_vec<T, E>(dys + (int64_t)p * lddys + c, o);
+          }
+        }
+      }
+      for (int d = 1; d < tx; d <<= 1) dot += __shfl_xor(dot, d);
+      if (n < N && sub == 0 && dweight != nullptr) dweight[n * k + j] = dot;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+static int grid_for(const bnpvi_ctx* ctx, int64_t blocks) {
+  const int64_t most = (int64_t)ctx->num_cu * 32;         // 8 resident workgroups of 256 per CU, four turns
+  return (int)(blocks < 1 ? 1 : blocks < most ? blocks : most);
+}
+
+template <int LPR, int VEC>
+static void launch_top(const bnpvi_ctx* ctx, const float* phi, int64_t ld, int64_t N, int L, int k, int renorm, int32_t* leaf,
+                       float* weight, float* total, hipStream_t s) {
+  const int g = grid_for(ctx, ceil_div(N, 256 / LPR));
+  if (k == 1)
+    top_leaves_kernel<1, LPR, VEC><<<g, 256, 0, s>>>(phi, ld, N, L, k, renorm, leaf, weight, total);
+  else if (k == 2)
+    top_leaves_kernel<2, LPR, VEC><<<g, 256, 0, s>>>(phi, ld, N, L, k, renorm, leaf, weight, total);
+  else if (k <= 4)
+    top_leaves_kernel<4, LPR, VEC><<<g, 256, 0, s>>>(phi, ld, N, L, k, renorm, leaf, weight, total);
+  else
+    top_leaves_kernel<8, LPR, VEC><<<g, 256, 0, s>>>(phi, ld, N, L, k, renorm, leaf, weight, total);
+}
+
+// the widest access (16, 8, 4 or 2 bytes) at which every row of both arrays starts and a row's bytes divide
+static int access_bytes(uint64_t a, uint64_t b, int64_t lda_bytes, int64_t ldb_bytes, int64_t row_bytes) {
+  const uint64_t all = a | b | (uint64_t)lda_bytes | (uint64_t)ldb_bytes | (uint64_t)row_bytes;
+  return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+}
+
+// lanes that share a row of `n` accesses: a power of two up to a wave
+static int lanes_for(int64_t n) {
+  int tx = 1;
+  while (tx < 64 && tx < n) tx <<= 1;
+  return tx;
+}
+
+template <typename T>
+static void launch_from(const bnpvi_ctx* ctx, const T* ys, int64_t ldys, const int32_t* place, const float* weight,
+                        const int32_t* kept, int64_t N, int k, int D, T* y, int64_t ldy, hipStream_t s) {
+  const int v = access_bytes((uintptr_t)ys, (uintptr_t)y, ldys * sizeof(T), ldy * sizeof(T), (int64_t)D * sizeof(T)) / (int)sizeof(T);
+  constexpr int E = 16 / (int)sizeof(T);
+  const int tx = lanes_for(v == E ? D / E : v >= 2 ? D / 2 : D);
+  const int g = grid_for(ctx, ceil_div(N, 256 / tx));
+  if (v == E)
+    rows_from_leaves_kernel<T, E><<<g, 256, 0, s>>>(ys, ldys, place, weight, kept, N, k, D, tx, y, ldy);
+  else if (v >= 2)
+    rows_from_leaves_kernel<T, 2><<<g, 256, 0, s>>>(ys, ldys, place, weight, kept, N, k, D, tx, y, ldy);
+  else
+    rows_from_leaves_kernel<T, 1><<<g, 256, 0, s>>>(ys, ldys, place, weight, kept, N, k, D, tx, y, ldy);
+}
+
+template <typename T>
+static void launch_from_bwd(const bnpvi_ctx* ctx, const T* dy, int64_t lddy, const T* ys, int64_t ldys, const int32_t* place,
+                            const float* weight, const int32_t* kept, int64_t N, int k, int D, T* dys, int64_t lddys, float* dweight,
+                            hipStream_t s) {
+  const int v = std::min(access_bytes((uintptr_t)dy, (uintptr_t)ys, lddy * sizeof(T), ldys * sizeof(T), (int64_t)D * sizeof(T)),
+                         access_bytes((uintptr_t)dys, 0, lddys * sizeof(T), 0, 0)) / (int)sizeof(T);
+  constexpr int E = 16 / (int)sizeof(T);
+  const int tx = lanes_for(v == E ? D / E : v >= 2 ? D / 2 : D);
+  const int g = grid_for(ctx, ceil_div(N, 256 / tx));
+  if (v == E)
+    rows_from_leaves_bwd_kernel<T, E><<<g, 256, 0, s>>>(dy, lddy, ys, ldys, place, weight, kept, N, k, D, tx, dys, lddys, dweight);
+  else if (v >= 2)
+    rows_from_leaves_bwd_kernel<T, 2><<<g, 256, 0, s>>>(dy, lddy, ys, ldys, place, weight, kept, N, k, D, tx, dys, lddys, dweight);
+  else
+    rows_from_leaves_bwd_kernel<T, 1><<<g, 256, 0, s>>>(dy, lddy, ys, ldys, place, weight, kept, N, k, D, tx, dys, lddys, dweight);
+}
+
+}  // namespace bnpvi
+
+using namespace bnpvi;
+
+extern "C" {
+
+int bnpvi_top_leaves_max(void) { return kTopMax; }
+
+int bnpvi_top_leaves(bnpvi_ctx* ctx, const float* phi, int64_t ldphi, int64_t N, int L, int k, int renormalize, int32_t* leaf,
+                     float* weight, float* total, void* stream) {
+  BNPVI_REQUIRE(ctx != nullptr, "bnpvi_top_leaves: ctx is NULL");
+  BNPVI_REQUIRE(N >= 0 && N < (int64_t(1) << 33), "bnpvi_top_leaves: N=%lld", (long long)N);
+  BNPVI_REQUIRE(L >= 1 && ldphi >= L, "bnpvi_top_leaves: L=%d, ldphi=%lld (a row holds at least L columns)", L, (long long)ldphi);
+  BNPVI_REQUIRE(k >= 1 && k <= kTopMax && k <= L, "bnpvi_top_leaves: k=%d (1 .. min(%d, L=%d))", k, kTopMax, L);
+  if (N == 0) return BNPVI_OK;
+  BNPVI_REQUIRE(phi && leaf && weight, "bnpvi_top_leaves: NULL device pointer");
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  // 16-byte loads read up to column roundup(L, 4) - 1 of a row, so the pitch has to cover it
+  const bool vec = ldphi % 4 == 0 && ((uintptr_t)phi & 15) == 0;
+  if (vec) {
+    if (L <= 32)
+      launch_top<8, 4>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
+    else if (L <= 128)
+      launch_top<16, 4>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
+    else
+      launch_top<64, 4>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
+  } else {
+    if (L <= 32)
+      launch_top<16, 1>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
+    else
+      launch_top<64, 1>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
+  }
+  BNPVI_LAUNCH_CHECK();
+  return BNPVI_OK;
+}
+
+int bnpvi_top_leaves_backward(bnpvi_ctx* ctx, const int32_t* leaf, const float* weight, const float* total, const float* dweight,
+                              int64_t N, int L, int k, int renormalize, float* dphi, int64_t lddphi, int cols, void* stream) {
+  BNPVI_REQUIRE(ctx != nullptr, "bnpvi_top_leaves_backward: ctx is NULL");
+  BNPVI_REQUIRE(N >= 0 && N < (int64_t(1) << 33), "bnpvi_top_leaves_backward: N=%lld", (long long)N);
+  BNPVI_REQUIRE(k >= 1 && k <= kTopMax && k <= L, "bnpvi_top_leaves_backward: k=%d (1 .. min(%d, L=%d))", k, kTopMax, L);
+  BNPVI_REQUIRE(cols >= L && lddphi >= cols, "bnpvi_top_leaves_backward: L=%d, cols=%d, lddphi=%lld", L, cols, (long long)lddphi);
+  if (N == 0) return BNPVI_OK;
+  BNPVI_REQUIRE(leaf && dweight && dphi && (!renormalize || (weight && total)), "bnpvi_top_leaves_backward: NULL device pointer");
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  const bool vec = lddphi % 4 == 0 && cols % 4 == 0 && ((uintptr_t)dphi & 15) == 0;
+  if (vec) {
+    if (cols <= 32)
+      top_leaves_bwd_kernel<8, 4><<<grid_for(ctx, ceil_div(N, 32)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
+                                                                                  dphi, lddphi, cols);
+    else if (cols <= 128)
+      top_leaves_bwd_kernel<16, 4><<<grid_for(ctx, ceil_div(N, 16)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
+                                                                                   dphi, lddphi, cols);
+    else
+      top_leaves_bwd_kernel<64, 4><<<grid_for(ctx, ceil_div(N, 4)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
+                                                                                  dphi, lddphi, cols);
+  } else {
+    top_leaves_bwd_kernel<64, 1><<<grid_for(ctx, ceil_div(N, 4)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
+                                                                                dphi, lddphi, cols);
+  }
+  BNPVI_LAUNCH_CHECK();
+  return BNPVI_OK;
+}
+
+// ---- sort: sizes of one call ---------------------------------------------------------------------------------------
+struct SortPlan {
+  int waves, bits, nb;
+  int64_t chunk;
+  size_t lds;
+};
+
+static SortPlan sort_plan(int64_t M, int L) {
+  SortPlan p;
+  const int B = L + 1;
+  p.bits = 1;
+  while ((int64_t(1) << p.bits) < B) ++p.bits;
+  // the counters of all waves and one row of bin starts share the LDS
+  p.waves = (size_t)5 * B * 4 + 64 <= (size_t)kMaxLdsBytes ? 4 : 1;
+  if (M <= 8192 && (size_t)17 * B * 4 + 128 <= (size_t)kMaxLdsBytes) {
+    p.nb = 1;                                // a minibatch: one workgroup, one launch
+    p.waves = M <= 1024 ? 4 : 16;
+    p.chunk = M < 1 ? 1 : M;
+  } else {
+    // a chunk at least as long as its row of counters (they are written and read once each), at most 1024 chunks
+    int64_t c = B > 2048 ? B : 2048;
+    if (ceil_div(M, c) > 1024) c = ceil_div(M, 1024);
+    p.chunk = (c + 255) / 256 * 256;
+    p.nb = (int)ceil_div(M, p.chunk);
+    if (p.nb < 1) p.nb = 1;
+  }
+  p.lds = ((size_t)(p.waves + 1) * B + p.waves) * 4;
+  return p;
+}
+
+int bnpvi_leaf_sort_max_leaves(void) { return kSortMaxLeaves; }
+
+int64_t bnpvi_leaf_sort_workspace(int64_t M, int L) {
+  if (M < 0 || M > INT32_MAX || L < 1 || L > kSortMaxLeaves) return -1;
+  const SortPlan p = sort_plan(M, L);
+  return p.nb == 1 && M <= 8192 ? 0 : (int64_t)(p.nb + 1) * (L + 1) * 4;
+}
+
+int bnpvi_leaf_sort(bnpvi_ctx* ctx, const int32_t* leaf, int64_t M, int L, int32_t* place, int32_t* order, int32_t* offsets,
+                    void* work, int64_t work_bytes, void* stream) {
+  BNPVI_REQUIRE(ctx != nullptr, "bnpvi_leaf_sort: ctx is NULL");
+  BNPVI_REQUIRE(M >= 0 && M <= INT32_MAX, "bnpvi_leaf_sort: M=%lld slots (0 .. 2^31 - 1)", (long long)M);
+  BNPVI_REQUIRE(L >= 1 && L <= kSortMaxLeaves, "bnpvi_leaf_sort: L=%d (1 .. %d)", L, kSortMaxLeaves);
+  BNPVI_REQUIRE(offsets && (M == 0 || (leaf && place && order)), "bnpvi_leaf_sort: NULL device pointer");
+  const int64_t need = bnpvi_leaf_sort_workspace(M, L);
+  BNPVI_REQUIRE(work_bytes >= need && (need == 0 || work != nullptr), "bnpvi_leaf_sort: workspace of %lld bytes, %lld needed",
+                (long long)work_bytes, (long long)need);
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  const SortPlan p = sort_plan(M, L);
+  const int B = L + 1;
+  static LdsLimit place_limit, count_limit;
+  BNPVI_HIP(place_limit.raise((const void*)leaf_place_kernel, ctx->device));
+  if (need == 0) {
+    leaf_place_kernel<<<1, p.waves * 64, p.lds, s>>>(leaf, M, L, p.chunk, p.bits, nullptr, nullptr, place, order, offsets);
+  } else {
+    BNPVI_HIP(count_limit.raise((const void*)leaf_count_kernel, ctx->device));
+    int32_t* hist = (int32_t*)work;
+    int32_t* totals = hist + (size_t)p.nb * B;
+    leaf_count_kernel<<<p.nb, 256, (size_t)B * 4, s>>>(leaf, M, L, p.chunk, hist);
+    leaf_scan_kernel<<<(B + 63) / 64, 1024, 0, s>>>(hist, p.nb, B, totals);
+    leaf_place_kernel<<<p.nb, p.waves * 64, p.lds, s>>>(leaf, M, L, p.chunk, p.bits, hist, totals, place, order, offsets);
+  }
+  BNPVI_LAUNCH_CHECK();
+  return BNPVI_OK;
+}
+
+static int check_rows(const char* what, bnpvi_ctx* ctx, int dtype, int64_t N, int k, int D, int L) {
+  BNPVI_REQUIRE(ctx != nullptr, "%s: ctx is NULL", what);
+  BNPVI_REQUIRE(dtype_bytes(dtype) > 0, "%s: dtype %d unknown", what, dtype);
+  BNPVI_REQUIRE(k >= 1 && N >= 0 && N <= INT32_MAX / k, "%s: N=%lld, k=%d (N k below 2^31)", what, (long long)N, k);
+  BNPVI_REQUIRE(D >= 1, "%s: D=%d", what, D);
+  BNPVI_REQUIRE(L >= 1, "%s: L=%d", what, L);
+  return BNPVI_OK;
+}
+
+int bnpvi_rows_to_leaves(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, int64_t N, int k, int D, const int32_t* place,
+                         const int32_t* offsets, int L, void* xs, int64_t ldxs, void* stream) {
+  const int rc = check_rows("bnpvi_rows_to_leaves", ctx, dtype, N, k, D, L);
+  if (rc) return rc;
+  BNPVI_REQUIRE(ldx >= D && ldxs >= D, "bnpvi_rows_to_leaves: row pitch %lld / %lld below D=%d", (long long)ldx, (long long)ldxs, D);
+  if (N == 0) return BNPVI_OK;
+  BNPVI_REQUIRE(x && place && offsets && xs, "bnpvi_rows_to_leaves: NULL device pointer");
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  const int e = dtype_bytes(dtype);
+  const int64_t row = (int64_t)D * e, lx = ldx * e, ls = ldxs * e;
+  const int v = access_bytes((uintptr_t)x, (uintptr_t)xs, lx, ls, row);
+  const int nvec = (int)(row / v), tx = lanes_for(nvec);
+  const int g = grid_for(ctx, ceil_div(N, 256 / tx));
+  const int32_t* kept = offsets + L;
+  if (v == 16)
+    rows_to_leaves_kernel<u32x4><<<g, 256, 0, s>>>((const char*)x, lx, N, k, nvec, tx, place, kept, (char*)xs, ls);
+  else if (v == 8)
+    rows_to_leaves_kernel<u32x2><<<g, 256, 0, s>>>((const char*)x, lx, N, k, nvec, tx, place, kept, (char*)xs, ls);
+  else if (v == 4)
+    rows_to_leaves_kernel<uint32_t><<<g, 256, 0, s>>>((const char*)x, lx, N, k, nvec, tx, place, kept, (char*)xs, ls);
+  else
+    rows_to_leaves_kernel<uint16_t><<<g, 256, 0, s>>>((const char*)x, lx, N, k, nvec, tx, place, kept, (char*)xs, ls);
+  BNPVI_LAUNCH_CHECK();
+  return BNPVI_OK;
+}
+
+int bnpvi_rows_from_leaves(bnpvi_ctx* ctx, int dtype, const void* ys, int64_t ldys, const int32_t* place, const float* weight,
+                           const int32_t* offsets, int L, int64_t N, int k, int D, void* y, int64_t ldy, void* stream) {
+  const int rc = check_rows("bnpvi_rows_from_leaves", ctx, dtype, N, k, D, L);
+  if (rc) return rc;
+  BNPVI_REQUIRE(ldys >= D && ldy >= D, "bnpvi_rows_from_leaves: row pitch %lld / %lld below D=%d", (long long)ldys, (long long)ldy, D);
+  if (N == 0) return BNPVI_OK;
+  BNPVI_REQUIRE(ys && place && offsets && y, "bnpvi_rows_from_leaves: NULL device pointer");
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  const int32_t* kept = offsets + L;
+  if (dtype == BNPVI_F32)
+    launch_from<float>(ctx, (const float*)ys, ldys, place, weight, kept, N, k, D, (float*)y, ldy, s);
+  else if (dtype == BNPVI_BF16)
+    launch_from<bf16_t>(ctx, (const bf16_t*)ys, ldys, place, weight, kept, N, k, D, (bf16_t*)y, ldy, s);
+  else
+    launch_from<f16_t>(ctx, (const f16_t*)ys, ldys, place, weight, kept, N, k, D, (f16_t*)y, ldy, s);
+  BNPVI_LAUNCH_CHECK();
+  return BNPVI_OK;
+}
+
+int bnpvi_rows_from_leaves_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy, const void* ys, int64_t ldys,
+                                    const int32_t* place, const float* weight, const int32_t* offsets, int L, int64_t N, int k, int D,
+                                    void* dys, int64_t lddys, float* dweight, void* stream) {
+  const int rc = check_rows("bnpvi_rows_from_leaves_backward", ctx, dtype, N, k, D, L);
+  if (rc) return rc;
+  BNPVI_REQUIRE(lddy >= D && ldys >= D && (dys == nullptr || lddys >= D),
+                "bnpvi_rows_from_leaves_backward: row pitch %lld / %lld / %lld below D=%d", (long long)lddy, (long long)ldys,
+                (long long)lddys, D);
+  if (N == 0) return BNPVI_OK;
+  BNPVI_REQUIRE(dy && ys && place && weight && offsets, "bnpvi_rows_from_leaves_backward: NULL device pointer");
+  if (dys == nullptr && dweight == nullptr) return BNPVI_OK;
+  if (dys == nullptr) lddys = 0;
+  OnDevice on(ctx->device);
+  BNPVI_HIP(on.status());
+  hipStream_t s = (hipStream_t)stream;
+  const int32_t* kept = offsets + L;
+  if (dtype == BNPVI_F32)
+    launch_from_bwd<float>(ctx, (const float*)dy, lddy, (const float*)ys, ldys, place, weight, kept, N, k, D, (float*)dys, lddys,
+                           dweight, s);
+  else if (dtype == BNPVI_BF16)
+    launch_from_bwd<bf16_t>(ctx, (const bf16_t*)dy, lddy, (const bf16_t*)ys, ldys, place, weight, kept, N, k, D, (bf16_t*)dys, lddys,
+                            dweight, s);
+  else
+    launch_from_bwd<f16_t>(ctx, (const f16_t*)dy, lddy, (const f16_t*)ys, ldys, place, weight, kept, N, k, D, (f16_t*)dys, lddys,
+                           dweight, s);
+  BNPVI_LAUNCH_CHECK();
+  return BNPVI_OK;
+}
+
+}  // extern "C"

@@ -292,6 +292,92 @@ int bnpvi_gamma_remap(bnpvi_ctx* ctx, const double* in_dev, int K_old, double* o
                       int K_new, int V, const int32_t* src_host, double gamma_hyper,
                       void* stream);
 
+/* ======================================================================================================
+ * Layers that follow the tree: what a model does with the responsibilities.  The few leaves that matter for
+ * a frame, the frames' rows in leaf order and back, and the dense product with its epilogue -- one weight for
+ * all rows (src/layers.py:76-114 is the reference's dense layer) or one per leaf on the sorted rows.
+ *
+ * Common to all of them: element types below; row pitches (ld*) in ELEMENTS; no allocation and no
+ * synchronisation (workspaces are the caller's, their sizes come from the *_workspace functions, calls that
+ * overlap need one each); the caller's current device is left as it was; everything can be captured into a
+ * HIP graph; sums are kept in 32 bits or more and added in an order that the sizes fix, so a call gives the
+ * same bits every time.  Entries of `leaf` outside [0, L) mean "no leaf".  Entries of device arrays are not
+ * trusted: places and offsets outside their range are skipped, never followed. */
+enum { BNPVI_F32 = 0, BNPVI_BF16 = 1, BNPVI_F16 = 2 };
+enum {
+  BNPVI_ACT_NONE = 0,
+  BNPVI_ACT_RELU = 1,
+  BNPVI_ACT_SOFTSIGN = 2, /* z / (1 + |z|): the reference's encoder heads, src/model.py:70-83 */
+  BNPVI_ACT_TANH = 3,
+  BNPVI_ACT_SILU = 4,     /* z / (1 + exp(-z)) */
+  BNPVI_ACT_GELU = 5      /* z Phi(z), Phi the normal distribution function */
+};
+
+/* ---- the k likeliest leaves of every frame ------------------------------------------------------------
+ * phi: float [N][ldphi], its first L columns are looked at (rows readable up to column roundup(L, 4) - 1 where
+ * ldphi is a multiple of 4 and phi of 16 bytes).  leaf int32 [N][k], weight float [N][k]: the k largest of the
+ * finite positive entries, largest first, ties to the lowest leaf; where a row has fewer, leaf -1 and weight 0.
+ * renormalize != 0: the weights are divided by their sum (in fp64, one rounding).  total float [N] or NULL: the
+ * sum, which the backward call needs under renormalize.  1 <= k <= min(L, bnpvi_top_leaves_max()).
+ * backward: dphi [N][lddphi] (columns 0 .. cols, cols >= L, all written) = dweight at the chosen leaves -- under
+ * renormalize (dweight - sum_j dweight_j weight_j) / total -- and 0 elsewhere. */
+int bnpvi_top_leaves_max(void);
+int bnpvi_top_leaves(bnpvi_ctx* ctx, const float* phi_dev, int64_t ldphi, int64_t N, int L, int k, int renormalize,
+                     int32_t* leaf_dev, float* weight_dev, float* total_dev, void* stream);
+int bnpvi_top_leaves_backward(bnpvi_ctx* ctx, const int32_t* leaf_dev, const float* weight_dev, const float* total_dev,
+                              const float* dweight_dev, int64_t N, int L, int k, int renormalize, float* dphi_dev,
+                              int64_t lddphi, int cols, void* stream);
+
+/* ---- slots sorted by leaf -----------------------------------------------------------------------------
+ * leaf int32 [M] (M = frames x choices, slot = frame * k + choice; M < 2^31), 1 <= L <=
+ * bnpvi_leaf_sort_max_leaves().  A stable sort: order[p] = the slot at place p, place[slot] = p,
+ * offsets[l] (int32 [L + 1]) = first place of leaf l; places from offsets[L] on hold the slots without a leaf, in
+ * their own order. */
+int bnpvi_leaf_sort_max_leaves(void);
+int64_t bnpvi_leaf_sort_workspace(int64_t M, int L);      /* bytes; -1 where M or L is out of range */
+int bnpvi_leaf_sort(bnpvi_ctx* ctx, const int32_t* leaf_dev, int64_t M, int L, int32_t* place_dev, int32_t* order_dev,
+                    int32_t* offsets_dev, void* work_dev, int64_t work_bytes, void* stream);
+
+/* ---- rows into leaf order and back ---------------------------------------------------------------------
+ * place int32 [N][k] and offsets int32 [L + 1] from bnpvi_leaf_sort, M = N k.
+ * to_leaves    xs[place[n][j]] = x[n] for every slot with a leaf; the rows of xs from offsets[L] on are zeroed.
+ * from_leaves  y[n] = sum_j weight[n][j] ys[place[n][j]] over the slots with a leaf (weight NULL: 1); it is also the
+ *              gradient of to_leaves.  A frame without a leaf gets 0.
+ * backward     of from_leaves: dys[place[n][j]] = weight[n][j] dy[n] (0 from row offsets[L] on), dweight[n][j] =
+ *              <dy[n], ys[place[n][j]]> (0 without a leaf); dys or dweight may be NULL. */
+int bnpvi_rows_to_leaves(bnpvi_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, int64_t N, int k, int D,
+                         const int32_t* place_dev, const int32_t* offsets_dev, int L, void* xs_dev, int64_t ldxs, void* stream);
+int bnpvi_rows_from_leaves(bnpvi_ctx* ctx, int dtype, const void* ys_dev, int64_t ldys, const int32_t* place_dev,
+                           const float* weight_dev, const int32_t* offsets_dev, int L, int64_t N, int k, int D, void* y_dev,
+                           int64_t ldy, void* stream);
+int bnpvi_rows_from_leaves_backward(bnpvi_ctx* ctx, int dtype, const void* dy_dev, int64_t lddy, const void* ys_dev, int64_t ldys,
+                                    const int32_t* place_dev, const float* weight_dev, const int32_t* offsets_dev, int L, int64_t N,
+                                    int k, int D, void* dys_dev, int64_t lddys, float* dweight_dev, void* stream);
+
+/* ---- dense product with its epilogue ------------------------------------------------------------------
+ *     z = x W^T + b,   y = residual + act(z)
+ * x [M][ldx] (K wide), W [n][ldw], bias [n] or NULL, residual [M][ldres] or NULL (n wide), y [M][ldy].
+ * G = 0, offsets NULL: one weight for all rows.  G >= 1 and offsets int32 [G + 1], ascending: rows offsets[g] ..
+ * offsets[g + 1] - 1 use W + g w_group and bias + g bias_group (elements); rows of no group get y = 0, and what their
+ * x, residual and dy hold is not looked at.  dact NULL, or [M][lddact]: act'(z) for the backward call, in fp16 where
+ * dtype is BNPVI_BF16 and in fp32 otherwise.  fp32 accumulation; fp32 inputs are multiplied in fp32.
+ * backward, with dz = dy dact (dact NULL: dz = dy, the case of BNPVI_ACT_NONE), rounded to dtype once:
+ *     dx = dz W [M][lddx],  dw[g] = dz_g^T x_g [groups][n][K],  db[g] = sum of dz_g (unrounded) [groups][n],
+ *     dres = dy with zeros in the rows of no group [M][lddres]
+ * each NULL where it is not wanted; a group without rows gets zeros, and so does dx in the rows of no group.
+ * 1 <= K, n <= 2^20, M < 2^31, G <= bnpvi_leaf_sort_max_leaves(), pitches of what is multiplied at most 4 MiB.
+ * Workspace: bnpvi_dense_workspace(dtype, M, K, n, G, backward) bytes, aligned to 256. */
+int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G, int backward);
+int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int64_t w_group,
+                const void* bias_dev, int64_t bias_group, int activation, const void* residual_dev, int64_t ldres,
+                const int32_t* offsets_dev, int G, int64_t M, int64_t K, int64_t n, void* y_dev, int64_t ldy, void* dact_dev,
+                int64_t lddact, void* work_dev, int64_t work_bytes, void* stream);
+int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy_dev, int64_t lddy, const void* dact_dev, int64_t lddact,
+                         const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int64_t w_group,
+                         const int32_t* offsets_dev, int G, int64_t M, int64_t K, int64_t n, void* dx_dev, int64_t lddx,
+                         void* dw_dev, void* db_dev, void* dres_dev, int64_t lddres, void* work_dev, int64_t work_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,579 @@
+"""Layers that follow the tree on the GPU, against plain restatements in 64 bits on the CPU.
+
+Tolerances.  u = half a step of the element type (bf16 2^-8, fp16 2^-11, fp32 2^-24).  A sum of m products in fp32 is
+off by at most (m + 16) 2^-23 of the sum of the products' magnitudes (two half steps an addition, whatever its order and
+whatever the matrix unit does with its last bit); activations are good to 16 half steps of fp32 beside 1 and have slopes
+of at most 1.13 and second derivatives of at most 2; a result is rounded once.  Every bound below is built of these."""
+import math
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}      # smallest steps
+ACTS = [None, "relu", "softsign", "tanh", "silu", "gelu"]
+
+
+@pytest.fixture(scope="module")
+def layers():
+    from bnp_vae_amd import layers as module
+    return module
+
+
+def gpu(t):
+    return t.to("cuda")
+
+
+def rand(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def within(got, want, bound, what=""):
+    got, want = got.detach().cpu().double(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    off = (got - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), "%s: %d of %d values off, worst %g where %g is allowed (value %g)" % (
+        what, int(bad.sum()), bad.numel(), float((off - bound)[bad].max() if bad.any() else 0),
+        float(torch.as_tensor(bound).expand(want.shape)[bad][0]), float(want[bad][0]))
+
+
+# ------------------------------------------------------------------------------------------------ top leaves
+def top_reference(phi, L, k, renorm):
+    p = phi[:, :L].double().numpy()
+    N = p.shape[0]
+    leaf = np.full((N, k), -1, np.int32)
+    w = np.zeros((N, k))
+    for r in range(N):
+        ok = np.nonzero((p[r] > 0) & np.isfinite(p[r]))[0]
+        best = ok[np.lexsort((ok, -p[r][ok]))][:k]
+        leaf[r, :len(best)] = best
+        w[r, :len(best)] = p[r][best]
+        if renorm and len(best):
+            w[r] /= w[r].sum()
+    return torch.from_numpy(leaf), torch.from_numpy(w)
+
+
+def phi_rows(N, cols, seed):
+    g = torch.Generator().manual_seed(seed)
+    phi = torch.softmax(torch.randn((N, cols), generator=g) * 20, 1)
+    if N > 8 and cols > 3:
+        phi[1] = 0.0                                  # no leaf at all
+        phi[2] = 0.125                                # all tied
+        phi[3, 1:] = -1.0                             # one positive entry
+        phi[4] = float("nan")
+        phi[5, 0] = float("inf")
+        phi[6, 2] = float("nan")
+        phi[7] = 2.0 ** -140                          # denormal responsibilities
+    return phi
+
+
+@pytest.mark.parametrize("N,L,cols,k,renorm", [
+    (1, 1, 1, 1, True), (1, 64, 64, 2, True), (9, 5, 32, 5, False), (33, 25, 32, 3, True), (257, 32, 32, 8, True),
+    (100, 33, 64, 2, False), (70, 64, 64, 1, True), (70, 61, 61, 4, True), (50, 128, 128, 8, True), (50, 129, 160, 7, False),
+    (20, 512, 512, 4, True), (9, 7776, 7776, 8, True), (9, 7775, 7777, 3, True), (0, 64, 64, 2, True), (5001, 64, 64, 2, True)])
+def test_top_leaves(layers, N, L, cols, k, renorm):
+    phi = phi_rows(N, cols, N + L)
+    leaf, weight = layers.top_leaves(gpu(phi), k, num_leaves=L, renormalize=renorm)
+    want_leaf, want_weight = top_reference(phi, L, k, renorm)
+    assert leaf.dtype == torch.int32 and torch.equal(leaf.cpu(), want_leaf)
+    within(weight, want_weight, 2 ** -23 * want_weight + 2.0 ** -149, "weight")      # one rounding of an fp64 quotient
+    # the gradient: with the values given to the formula in 64 bits
+    x = gpu(phi).requires_grad_(True)
+    leaf2, w = layers.top_leaves(x, k, num_leaves=L, renormalize=renorm)
+    assert not leaf2.requires_grad and torch.equal(leaf2.cpu(), want_leaf)
+    dw = rand((N, k), torch.float32, 5)
+    got, = torch.autograd.grad(w, x, gpu(dw))
+    want = torch.zeros((N, cols), dtype=torch.float64)
+    bound = torch.zeros((N, cols), dtype=torch.float64)
+    p64 = torch.where((phi > 0) & torch.isfinite(phi), phi, 0.0).double()
+    for r in range(N):
+        on = want_leaf[r] >= 0
+        cols_r = want_leaf[r][on].long()
+        d = dw[r][on].double()
+        if renorm and on.any():
+            s = p64[r][cols_r].sum()
+            dot = (d * want_weight[r][on]).sum()
+            # dot from weights rounded to fp32, the sum rounded to fp32 (absolute 2^-150 where it is denormal)
+            off = 2.0 ** -22 * (d.abs() + (d * want_weight[r][on]).abs().sum()) + (d - dot).abs() * (2.0 ** -149 / s)
+            want[r, cols_r], bound[r, cols_r] = (d - dot) / s, off / s
+        else:
+            want[r, cols_r] = d
+    finite = want.abs() < 3e38                       # 1 / 2^-138 passes fp32's range
+    within(torch.where(finite, got.cpu().double(), 0.0), torch.where(finite, want, 0.0),
+           torch.where(finite, bound + 2.0 ** -24 * want.abs(), 0.0), "dphi")
+
+
+def test_top_leaves_of_views(layers):
+    """Rows that start off 16 bytes, a pitch wider than the row, a transposed matrix."""
+    big = phi_rows(40, 70, 3)
+    for view in (lambda t: t[:, 1:66], lambda t: t[:, :64], lambda t: t[::2, 4:], lambda t: t.t()):
+        v = view(big)
+        leaf, weight = layers.top_leaves(view(gpu(big)), 3)
+        want_leaf, want_weight = top_reference(v, v.shape[1], 3, True)
+        assert torch.equal(leaf.cpu(), want_leaf)
+        within(weight, want_weight, 2 ** -23 * want_weight + 2.0 ** -149)
+
+
+def test_top_leaves_gradient_against_differences(layers):
+    """d/dphi of sum(c w) by central differences: step h on an entry of size p bends the quotient by O((h/S)^2)."""
+    phi = torch.rand((6, 12), generator=torch.Generator().manual_seed(1)) + 0.2
+    phi = phi * (1 + 0.05 * torch.arange(12))        # no two entries closer than the step can reverse matter below
+    c = rand((6, 3), torch.float32, 2)
+    x = gpu(phi).requires_grad_(True)
+    leaf, w = layers.top_leaves(x, 3)
+    got, = torch.autograd.grad(w, x, gpu(c))
+    h = 2.0 ** -9
+    def value(p):
+        p = p.double()
+        picked = torch.gather(p, 1, leaf.cpu().long())      # the choice itself is held
+        return (c.double() * picked / picked.sum(1, keepdim=True)).sum()
+    for r in range(6):
+        for j in range(12):
+            up, down = phi.clone().double(), phi.clone().double()
+            up[r, j] += h
+            down[r, j] -= h
+            slope = float(value(up) - value(down)) / (2 * h)
+            # third derivative of a quotient of sums of at least 0.6: at most 6 |c| / S^3
+            assert abs(slope - float(got[r, j])) <= 6 * float(c.abs().sum()) / 0.6 ** 3 * h * h / 6 + 1e-6
+
+
+# ------------------------------------------------------------------------------------------------ sort, dispatch, combine
+def sort_reference(leaf, L):
+    flat = leaf.reshape(-1).to(torch.int64)
+    key = torch.where((flat >= 0) & (flat < L), flat, L)
+    order = torch.sort(key, stable=True).indices
+    place = torch.empty_like(order)
+    place[order] = torch.arange(order.numel())
+    counts = torch.bincount(key, minlength=L + 1)
+    return place, order, torch.cumsum(counts, 0) - counts
+
+
+@pytest.mark.parametrize("M,L", [(0, 3), (1, 1), (63, 2), (64, 64), (65, 7), (1000, 25), (1024, 64), (1025, 64), (8192, 512),
+                                 (8193, 512), (50000, 64), (5000, 7776), (20000, 7776), (300001, 7776), (9000, 16384), (200, 16384),
+                                 (300007, 3), (2100001, 100)])
+@pytest.mark.parametrize("kind", ["spread", "one", "none"])
+def test_sort_by_leaf(layers, M, L, kind):
+    g = torch.Generator().manual_seed(M + L)
+    leaf = torch.randint(-1, L, (M,), generator=g, dtype=torch.int32)
+    if kind == "one":
+        leaf.fill_(L - 1)
+    elif kind == "none":
+        leaf.fill_(-1)
+    elif M > 10:
+        leaf[3], leaf[5], leaf[7] = L, 2 ** 31 - 1, -2 ** 31           # no leaf either
+    plan = layers.sort_by_leaf(gpu(leaf), L)
+    place, order, offsets = sort_reference(leaf, L)
+    assert torch.equal(plan.offsets.cpu().long(), offsets)
+    assert torch.equal(plan.order.cpu().long(), order)
+    assert torch.equal(plan.place.cpu().long().reshape(-1), place)
+    assert plan.num_frames == M and plan.choices == 1 and plan.num_leaves == L
+
+
+def test_sort_by_leaf_of_int64_and_strided(layers):
+    leaf = torch.randint(0, 9, (77, 6), generator=torch.Generator().manual_seed(0))
+    leaf[4, 2] = 2 ** 40
+    leaf[5, 4] = -2 ** 40
+    plan = layers.sort_by_leaf(gpu(leaf)[:, ::2], 9)
+    place, order, offsets = sort_reference(leaf[:, ::2], 9)
+    assert torch.equal(plan.order.cpu().long(), order) and torch.equal(plan.offsets.cpu().long(), offsets)
+    assert torch.equal(plan.place.cpu().long().reshape(-1), place)
+
+
+def exchange_reference(x, ys, leaf, w, L):
+    place, order, offsets = sort_reference(leaf, L)
+    N, k = leaf.shape
+    kept = int(offsets[L])
+    place = place.view(N, k)
+    on = (place < kept)[:, :, None]
+    xs = torch.where(torch.arange(N * k)[:, None] < kept, x.double()[order // k], 0.0)
+    rows = torch.where(on, ys.double()[place], 0.0)
+    wk = torch.where(on, (torch.ones((N, k)) if w is None else w).double()[:, :, None], 0.0)
+    return xs, (wk * rows).sum(1), rows, wk, place, order, kept
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("N,k,D,L", [(1, 1, 1, 1), (5, 2, 3, 4), (64, 1, 32, 25), (33, 3, 100, 7), (130, 2, 256, 64), (17, 4, 257, 5),
+                                     (9, 2, 1030, 3), (1000, 8, 6, 600), (0, 2, 8, 3)])
+def test_dispatch_and_combine(layers, dtype, N, k, D, L):
+    T = TYPES[dtype]
+    x, ys = rand((N, D), T, 1), rand((N * k, D), T, 2)
+    leaf = torch.randint(-1, L, (N, k), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
+    w = torch.rand((N, k), generator=torch.Generator().manual_seed(4)) + 0.1
+    plan = layers.sort_by_leaf(gpu(leaf), L)
+    kept = int(sort_reference(leaf, L)[2][L])
+    ys[kept:] = float("nan")                          # rows of no leaf take part in nothing
+    X, Y, W = (gpu(t).requires_grad_(True) for t in (x, ys, w))
+    xs, y = layers.dispatch(X, plan), layers.combine(Y, plan, W)
+    y1 = layers.combine(Y, plan)
+    want_xs, want_y, rows, wk, place, order, kept = exchange_reference(x, ys, leaf, w, L)
+    assert torch.equal(xs.detach().cpu().double(), want_xs)
+    mag = (wk * rows).abs().sum(1)
+    within(y, want_y, HALF[T] * want_y.abs() + TINY[T] + (k + 16) * 2.0 ** -23 * mag, "y")
+    want1 = rows.sum(1)
+    within(y1, want1, HALF[T] * want1.abs() + TINY[T] + (k + 16) * 2.0 ** -23 * rows.abs().sum(1), "y, weight 1")
+    dxs, dy = rand((N * k, D), T, 5), rand((N, D), T, 6)
+    dxs[kept:] = float("nan")
+    dx, dys, dw = torch.autograd.grad([xs, y], [X, Y, W], [gpu(dxs), gpu(dy)])
+    back = torch.where((place < kept)[:, :, None], dxs.double()[place], 0.0)
+    within(dx, back.sum(1), HALF[T] * back.sum(1).abs() + TINY[T] + (k + 16) * 2.0 ** -23 * back.abs().sum(1), "dx")
+    want = torch.zeros((N * k, D), dtype=torch.float64)
+    want[place.reshape(-1)] = (wk * dy.double()[:, None]).reshape(N * k, D)
+    within(dys, want, (HALF[T] + 2.0 ** -24) * want.abs() + TINY[T], "dys")
+    prod = rows * dy.double()[:, None]
+    within(dw, prod.sum(2), (D + 16) * 2.0 ** -23 * prod.abs().sum(2) + 2.0 ** -149, "dweight")
+    d1, = torch.autograd.grad(y1, Y, gpu(dy))
+    want[place.reshape(-1)] = ((place < kept)[:, :, None] * dy.double()[:, None]).reshape(N * k, D)
+    assert torch.equal(d1.cpu().double(), want)
+
+
+def test_dispatch_and_combine_of_views(layers):
+    """Rows at a wider pitch and off 16 bytes, an expanded gradient, one slot's weight frozen."""
+    leaf = torch.randint(-1, 4, (50, 2), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
+    plan = layers.sort_by_leaf(gpu(leaf), 4)
+    big, bigs = rand((50, 41), torch.bfloat16, 1), rand((100, 41), torch.bfloat16, 2)
+    w = torch.rand((50, 4), generator=torch.Generator().manual_seed(4))
+    X, Y = gpu(big)[:, 1:34].requires_grad_(True), gpu(bigs)[:, 3:36].requires_grad_(True)
+    xs, y = layers.dispatch(X, plan), layers.combine(Y, plan, gpu(w)[:, 1:3])
+    want_xs, want_y, rows, wk, place, _order, kept = exchange_reference(big[:, 1:34], bigs[:, 3:36], leaf, w[:, 1:3], 4)
+    assert torch.equal(xs.detach().cpu().double(), want_xs)
+    within(y, want_y, 2.0 ** -8 * want_y.abs() + 18 * 2.0 ** -23 * (wk * rows).abs().sum(1) + 2.0 ** -133)
+    dx, dys = torch.autograd.grad(xs.sum() + y.sum(), [X, Y])
+    assert torch.equal(dx.cpu().double(), (place < kept).sum(1).double()[:, None].expand(50, 33))
+    want = torch.zeros((100, 33), dtype=torch.float64)
+    want[place.reshape(-1)] = wk.expand(50, 2, 33).reshape(100, 33)
+    within(dys, want, 2.0 ** -8 * want.abs())
+
+
+# ------------------------------------------------------------------------------------------------ dense
+def act64(name, z):
+    if name == "relu":
+        return torch.relu(z), (z > 0).double()
+    if name == "softsign":
+        q = 1 / (1 + z.abs())
+        return z * q, q * q
+    if name == "tanh":
+        return torch.tanh(z), 1 / torch.cosh(z) ** 2
+    if name == "silu":
+        q = torch.sigmoid(z)
+        return z * q, q + z * q * (1 - q)
+    if name == "gelu":
+        c = 0.5 * torch.erfc(-z / math.sqrt(2))
+        return z * c, c + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    return z, torch.ones_like(z)
+
+
+def dense_reference(x, w, b, act, r, bounds, dy):
+    """Values and the bounds of their errors; w (G, n, K), bounds the groups' rows."""
+    T, M, (G, n, K) = x.dtype, x.shape[0], w.shape
+    u, t = HALF[T], TINY[T]
+    out = {}
+    for name, shape in (("y", (M, n)), ("dx", (M, K)), ("dw", (G, n, K)), ("db", (G, n)), ("dr", (M, n))):
+        out[name] = [torch.zeros(shape, dtype=torch.float64), torch.zeros(shape, dtype=torch.float64)]
+    for g in range(G):
+        lo, hi = bounds[g], bounds[g + 1]
+        rows = slice(lo, hi)
+        xg, wg, m = x[rows].double(), w[g].double(), hi - lo
+        bg = torch.zeros(n, dtype=torch.float64) if b is None else b[g].double()
+        rg = torch.zeros((m, n), dtype=torch.float64) if r is None else r[rows].double()
+        z = xg @ wg.t() + bg
+        zoff = (K + 16) * 2.0 ** -23 * (xg.abs() @ wg.abs().t() + bg.abs())
+        a, d = act64(act, z)
+        y = a + rg
+        out["y"][0][rows] = y
+        out["y"][1][rows] = u * y.abs() + t + 1.13 * zoff + 16 * 2.0 ** -24 * (1 + a.abs() + rg.abs()) * (act is not None) \
+            + 2.0 ** -23 * (a.abs() + rg.abs())
+        gy = dy[rows].double()
+        dz = gy * d
+        doff = 2 * zoff + 16 * 2.0 ** -24 if act is not None else torch.zeros_like(z)
+        if act == "relu":
+            doff = (z.abs() <= zoff).double()
+        if act is not None and T is torch.bfloat16:
+            doff = doff + 2.0 ** -11 * d.abs() + 2.0 ** -25
+        raw = gy.abs() * doff + 2.0 ** -23 * dz.abs() * (act is not None)          # of dz before its rounding
+        zz = raw + (u * (dz.abs() + raw) + t) * (act is not None)
+        full = dz.abs() + zz
+        dx = dz @ wg
+        out["dx"][0][rows] = dx
+        off = zz @ wg.abs() + (n + 16) * 2.0 ** -23 * (full @ wg.abs())
+        out["dx"][1][rows] = off + u * (dx.abs() + off) + t
+        dw = dz.t() @ xg
+        off = zz.t() @ xg.abs() + (m + 16) * 2.0 ** -23 * (full.t() @ xg.abs())
+        out["dw"][0][g], out["dw"][1][g] = dw, off + u * (dw.abs() + off) + t
+        db = dz.sum(0)
+        off = raw.sum(0) + (m + 16) * 2.0 ** -23 * (dz.abs() + raw).sum(0)
+        out["db"][0][g], out["db"][1][g] = db, off + u * (db.abs() + off) + t
+        out["dr"][0][rows] = gy
+    return out
+
+
+def check_dense(layers, M, K, n, T, act, bias, residual, sizes=None, seed=0, view=None, poison=True, head=0):
+    """One forward and backward; sizes: rows of each group (None: one weight for all)."""
+    G = 1 if sizes is None else len(sizes)
+    x, w = rand((M, K), T, seed), rand((G, n, K), T, seed + 1, 1 / math.sqrt(K))
+    b = rand((G, n), T, seed + 2, 0.5) if bias else None
+    r = rand((M, n), T, seed + 3) if residual else None
+    dy = rand((M, n), T, seed + 4)
+    bounds = [0, M] if sizes is None else list(head + np.concatenate([[0], np.cumsum(sizes)]))
+    bounds = [int(v) for v in bounds]
+    if poison and sizes is not None:
+        for t in (x, dy) + (() if r is None else (r,)):
+            t[bounds[-1]:] = float("nan")
+            t[:head] = float("inf")
+    want = dense_reference(x, w, b, act, r, bounds, dy)
+    put = view or gpu
+    X = put(x).requires_grad_(True)
+    W = put(w if sizes is not None else w[0]).requires_grad_(True)
+    B = None if b is None else gpu(b if sizes is not None else b[0]).requires_grad_(True)
+    R = None if r is None else put(r).requires_grad_(True)
+    off = None if sizes is None else torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    y = layers.dense(X, W, B, activation=act, residual=R, offsets=off)
+    with torch.no_grad():
+        assert torch.equal(layers.dense(X, W, B, activation=act, residual=R, offsets=off), y.detach())
+    within(y, *want["y"], "y")
+    names = [m for m, t in (("dx", X), ("dw", W), ("db", B), ("dr", R)) if t is not None]
+    leaves = [t for t in (X, W, B, R) if t is not None]
+    for name, got in zip(names, torch.autograd.grad(y, leaves, put(dy))):
+        value, bound = want[name]
+        if sizes is None and name in ("dw", "db"):
+            value, bound = value[0], bound[0]
+        within(got, value, bound, name)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("M,K,n", [(1, 1, 1), (1, 64, 32), (2, 8, 8), (5, 40, 7), (31, 24, 33), (33, 72, 64), (128, 64, 128),
+                                   (129, 128, 136), (127, 65, 129), (300, 100, 40), (70, 250, 130), (257, 520, 30)])
+def test_dense_sizes(layers, dtype, M, K, n):
+    check_dense(layers, M, K, n, TYPES[dtype], "softsign", True, True, seed=M + K + n)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("act", ACTS)
+def test_dense_activations(layers, dtype, act):
+    check_dense(layers, 150, 48, 72, TYPES[dtype], act, True, False, seed=9)
+    check_dense(layers, 37, 48, 72, TYPES[dtype], act, False, True, seed=19)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("M,K,n", [(1, 4096, 32), (8, 4096, 256), (40, 2048, 48), (500, 1000, 64), (2500, 64, 512), (4000, 160, 264)])
+def test_dense_long_sums_and_many_tiles(layers, dtype, M, K, n):
+    check_dense(layers, M, K, n, TYPES[dtype], "gelu", True, True, seed=M)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("sizes,tail,head", [([3], 0, 0), ([0, 5, 0, 1, 70, 0], 4, 0), ([130, 1, 129, 33], 0, 0), ([0, 0, 0], 6, 0),
+                                             ([64, 64], 64, 0), ([1] * 40, 0, 0), ([200, 300, 0, 250], 9, 3), ([7, 0, 12], 0, 5)])
+@pytest.mark.parametrize("K,n", [(64, 128), (50, 31)])
+def test_dense_per_leaf(layers, dtype, sizes, tail, head, K, n):
+    check_dense(layers, head + sum(sizes) + tail, K, n, TYPES[dtype], "silu", True, True, sizes=sizes, seed=sum(sizes), head=head)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_dense_of_views(layers, dtype):
+    """Wider pitches, rows off 16 bytes, transposed operands."""
+    def wide(t):
+        big = torch.full(tuple(t.shape[:-1]) + (t.shape[-1] + 11,), float("nan"), dtype=t.dtype, device="cuda")
+        big[..., 8:8 + t.shape[-1]] = gpu(t)
+        return big[..., 8:8 + t.shape[-1]].detach()
+    def off(t):
+        big = torch.full(tuple(t.shape[:-1]) + (t.shape[-1] + 16,), float("nan"), dtype=t.dtype, device="cuda")
+        big[..., 3:3 + t.shape[-1]] = gpu(t)
+        return big[..., 3:3 + t.shape[-1]].detach()
+    def turned(t):
+        return gpu(t.transpose(-1, -2).contiguous()).transpose(-1, -2)
+    for view in (wide, off, turned):
+        check_dense(layers, 140, 56, 136, TYPES[dtype], "tanh", True, True, seed=3, view=view)
+        check_dense(layers, 140, 56, 136, TYPES[dtype], None, True, True, sizes=[60, 0, 70], seed=3, view=view)
+
+
+def test_dense_shapes_around_a_row(layers):
+    x, w, b = rand((3, 5, 24), torch.float32, 1), rand((16, 24), torch.float32, 2), rand((16,), torch.float32, 3)
+    r = rand((3, 5, 16), torch.float32, 4)
+    y = layers.dense(gpu(x), gpu(w), gpu(b), "relu", gpu(r))
+    flat = layers.dense(gpu(x).reshape(15, 24), gpu(w), gpu(b), "relu", gpu(r).reshape(15, 16))
+    assert y.shape == (3, 5, 16) and torch.equal(y.reshape(15, 16), flat)
+    one = layers.dense(gpu(x)[0, 0], gpu(w), gpu(b))
+    assert one.shape == (16,)
+    empty = layers.dense(gpu(x)[:0], gpu(w).requires_grad_(True), gpu(b))
+    assert empty.shape == (0, 5, 16)
+
+
+@pytest.mark.parametrize("G", [0, 3])
+def test_dense_without_rows(layers, G):
+    w = gpu(rand((G, 8, 16) if G else (8, 16), torch.float32, 1)).requires_grad_(True)
+    b = gpu(rand((G, 8) if G else (8,), torch.float32, 2)).requires_grad_(True)
+    x = torch.empty((0, 16), device="cuda", requires_grad=True)
+    off = torch.zeros(G + 1, dtype=torch.int32, device="cuda") if G else None
+    y = layers.dense(x, w, b, activation="gelu", offsets=off)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.empty((0, 8), device="cuda"))
+    assert y.shape == (0, 8) and dx.shape == (0, 16)
+    assert torch.equal(dw, torch.zeros_like(w)) and torch.equal(db, torch.zeros_like(b))
+
+
+def test_dense_gradient_against_differences(layers):
+    """Central differences of sum(c y) in x, W, b: h^2 / 6 times a third derivative (at most 6 |W|^3 |c| for softsign),
+    and the fp64 reference gives the values themselves, so nothing else enters."""
+    x, w, b = (rand(s, torch.float32, i, 0.5) for i, s in enumerate([(4, 6), (5, 6), (5,)]))
+    c = rand((4, 5), torch.float32, 7)
+    X, W, B = (gpu(t).requires_grad_(True) for t in (x, w, b))
+    y = layers.dense(X, W, B, activation="softsign")
+    grads = torch.autograd.grad(y, [X, W, B], gpu(c))
+    h = 2.0 ** -10
+    base = [t.double() for t in (x, w, b)]
+    def value(v):
+        z = v[0] @ v[1].t() + v[2]
+        return float((c.double() * z / (1 + z.abs())).sum())
+    most = max(float(t.abs().max()) for t in base + [torch.ones(1)])
+    for i, g in enumerate(grads):
+        for j in range(base[i].numel()):
+            up, down = [t.clone() for t in base], [t.clone() for t in base]
+            up[i].view(-1)[j] += h
+            down[i].view(-1)[j] -= h
+            slope = (value(up) - value(down)) / (2 * h)
+            # softsign's second derivative jumps by 4 at 0, where a difference is off by up to h |x|^2 |c| / 2 x 4
+            allowed = float(c.abs().sum()) * most ** 3 * (h * h + 2 * h)
+            assert abs(slope - float(g.view(-1)[j].cpu())) <= allowed
+
+
+def test_dense_with_infinities(layers):
+    """Rows with an infinity or NaN spoil themselves alone; activations at infinity have their limits."""
+    for T in TYPES.values():
+        x = torch.zeros((5, 16), dtype=T)
+        x[0, 3], x[1, 4], x[2, 5], x[3, 0] = float("inf"), -float("inf"), float("nan"), 1.0
+        w = torch.ones((8, 16), dtype=T)
+        for act, at in ((None, [math.inf, -math.inf]), ("relu", [math.inf, 0.0]), ("softsign", [1.0, -1.0]), ("tanh", [1.0, -1.0]),
+                        ("silu", [math.inf, 0.0]), ("gelu", [math.inf, 0.0])):
+            y = layers.dense(gpu(x), gpu(w), activation=act).cpu().double()
+            assert torch.equal(y[0], torch.full((8,), at[0], dtype=torch.float64)), (T, act, y[0])
+            assert torch.equal(y[1], torch.full((8,), at[1], dtype=torch.float64)), (T, act, y[1])
+            assert torch.isnan(y[2]).all() and torch.isfinite(y[3:]).all() and (y[4] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ a run of them together
+def block(layers, phi, x, W1, b1, W2, b2, L, k):
+    """Every frame through the layers of its k likeliest leaves, beside its own value."""
+    leaf, weight = layers.top_leaves(phi, k, num_leaves=L)
+    plan = layers.sort_by_leaf(leaf, L)
+    h = layers.dense(layers.dispatch(x, plan), W1, b1, activation="gelu", offsets=plan.offsets)
+    return x + layers.combine(layers.dense(h, W2, b2, offsets=plan.offsets), plan, weight)
+
+
+def block_inputs(N, D, H, L, cols, seed=0):
+    phi = phi_rows(N, cols, seed)
+    phi = torch.nan_to_num(phi, nan=0.0, posinf=0.0)
+    return [phi, rand((N, D), torch.float32, seed + 1), rand((L, H, D), torch.float32, seed + 2, 0.3), rand((L, H), torch.float32, seed + 3),
+            rand((L, D, H), torch.float32, seed + 4, 0.3), rand((L, D), torch.float32, seed + 5)]
+
+
+def test_layers_together(layers):
+    N, D, H, L, k = 90, 24, 40, 9, 2
+    phi, x, W1, b1, W2, b2 = inputs = block_inputs(N, D, H, L, 32)
+    on = [gpu(t).requires_grad_(True) for t in inputs]
+    y = block(layers, *on, L, k)
+    dy = rand((N, D), torch.float32, 11)
+    got = torch.autograd.grad(y, on, gpu(dy))
+    leaf, _ = top_reference(phi, L, k, True)
+    v = [t.double().requires_grad_(True) for t in inputs]
+    out = []
+    for r in range(N):
+        s, parts = 0.0, []
+        for j in range(k):
+            l = int(leaf[r, j])
+            if l < 0:
+                continue
+            h = v[2][l] @ v[1][r] + v[3][l]
+            h = h * 0.5 * torch.erfc(-h / math.sqrt(2))
+            parts.append(v[0][r, l] * (v[4][l] @ h + v[5][l]))
+            s = s + v[0][r, l]
+        out.append(v[1][r] + (sum(parts) / s if parts else 0.0))
+    ref = torch.stack(out)
+    want = torch.autograd.grad(ref, v, dy.double())
+    # three fp32 sums of at most 56 terms in a row on values of order 1: 1e-4 of the largest value is 10 times their bound;
+    # the gradient of phi is divided by a row's sum of responsibilities
+    within(y, ref.detach(), 1e-4 * float(ref.abs().max()))
+    for g, t, name in zip(got, want, ["dphi", "dx", "dW1", "db1", "dW2", "db2"]):
+        if name == "dphi":
+            total = torch.where(leaf >= 0, torch.gather(phi.double(), 1, leaf.clamp(min=0).long()), 0.0).sum(1, keepdim=True)
+            scale = torch.where(total > 0, 1e-4 * float(ref.abs().max()) * dy.abs().sum(1, keepdim=True).double() / total, 0.0)
+            finite = t.abs() < 3e38
+            within(torch.where(finite, g.cpu().double(), 0.0), torch.where(finite, t, 0.0), torch.where(finite, scale, 0.0), name)
+        else:
+            within(g, t, 1e-4 * float(t.abs().max()), name)
+
+
+def test_layers_in_a_graph(layers):
+    """Forward and backward captured, replayed on new inputs between eager work; every replay equals the eager result."""
+    N, D, H, L, k = 700, 64, 96, 25, 2
+    static = [gpu(t).requires_grad_(i != 0) for i, t in enumerate(block_inputs(N, D, H, L, 32))]
+    dy = gpu(rand((N, D), torch.float32, 3))
+    def step(v):
+        y = block(layers, *v, L, k)
+        return [y] + list(torch.autograd.grad(y, v[1:], dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(static)
+    for turn in range(4):
+        new = [gpu(t) for t in block_inputs(N, D, H, L, 32, seed=20 + turn)]
+        with torch.no_grad():
+            for s, t in zip(static, new):
+                s.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step([t.requires_grad_(i != 0) for i, t in enumerate(new)])
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_layers_on_another_stream_and_in_threads(layers):
+    """Two threads, each on a stream of its own, give the bits of one alone."""
+    N, D, H, L, k = 3000, 64, 64, 64, 2
+    inputs = [[gpu(t).requires_grad_(True) for t in block_inputs(N, D, H, L, 64, seed=s)] for s in (1, 2)]
+    dy = gpu(rand((N, D), torch.float32, 3))
+    def step(v):
+        y = block(layers, *v, L, k)
+        return [y] + list(torch.autograd.grad(y, v, dy))
+    want = [step(v) for v in inputs]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[i] = step(inputs[i])
+            s.synchronize()
+        except Exception as e:                                   # noqa: BLE001 - reported by the main thread
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for a, b in zip(got, want):
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+
+
+def test_same_bits_every_time(layers):
+    for T in TYPES.values():
+        x, w = gpu(rand((5000, 256), T, 1)).requires_grad_(True), gpu(rand((96, 256), T, 2)).requires_grad_(True)
+        b, dy = gpu(rand((96,), T, 3)).requires_grad_(True), gpu(rand((5000, 96), T, 4))
+        first = None
+        for _ in range(10):
+            y = layers.dense(x, w, b, activation="silu")
+            now = [y] + list(torch.autograd.grad(y, [x, w, b], dy))
+            first = first or now
+            for p, q in zip(first, now):
+                assert torch.equal(p, q)

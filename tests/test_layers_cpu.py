@@ -1,0 +1,100 @@
+"""Refusals of the layer operators that need no GPU: the Python checks in front of the library, and the library's own
+checks of sizes, which come before any device call."""
+import ctypes as C
+
+import pytest
+import torch
+
+from bnp_vae_amd import _lib, layers
+
+
+def test_cpu_tensors_are_refused():
+    t = torch.zeros((4, 8))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        layers.top_leaves(t, 2)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        layers.sort_by_leaf(torch.zeros(4, dtype=torch.int32), 3)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        layers.dense(t, torch.zeros((3, 8)))
+    plan = layers.LeafPlan(torch.zeros((4, 1), dtype=torch.int32), torch.zeros(4, dtype=torch.int32),
+                           torch.zeros(4, dtype=torch.int32), 3)
+    for call in (layers.dispatch, layers.combine):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call(t, plan)
+        with pytest.raises(TypeError, match="LeafPlan"):
+            call(t, None)
+    with pytest.raises(TypeError, match="torch tensor"):
+        layers.top_leaves([[0.5, 0.5]], 1)
+
+
+def _fails(rc, text):
+    assert rc == 1
+    assert text in _lib.lib.bnpvi_last_error().decode(), _lib.lib.bnpvi_last_error()
+
+
+class _Ctx(object):
+    """A stand-in for a context (its memory is never looked at before the sizes are)."""
+
+    def __init__(self):
+        self.mem = C.create_string_buffer(4096)
+        self.p = C.c_void_p(C.addressof(self.mem))
+
+
+def test_library_refuses_sizes():
+    lib, c, one = _lib.lib, _Ctx(), C.c_void_p(256)
+    _fails(lib.bnpvi_top_leaves(None, one, 4, 1, 4, 1, 1, one, one, None, None), "ctx")
+    _fails(lib.bnpvi_top_leaves(c.p, one, 3, 1, 4, 1, 1, one, one, None, None), "at least L")
+    _fails(lib.bnpvi_top_leaves(c.p, one, 4, 1, 4, 5, 1, one, one, None, None), "k=5")
+    _fails(lib.bnpvi_top_leaves(c.p, one, 64, 1, 64, 9, 1, one, one, None, None), "k=9")
+    _fails(lib.bnpvi_top_leaves(c.p, one, 64, 1 << 33, 64, 1, 1, one, one, None, None), "N=")
+    _fails(lib.bnpvi_top_leaves(c.p, None, 64, 1, 64, 1, 1, one, one, None, None), "NULL")
+    _fails(lib.bnpvi_top_leaves_backward(c.p, one, one, None, one, 1, 4, 1, 1, one, 4, 4, None), "NULL")
+    _fails(lib.bnpvi_top_leaves_backward(c.p, one, one, one, one, 1, 4, 1, 1, one, 4, 3, None), "cols=3")
+    most = lib.bnpvi_leaf_sort_max_leaves()
+    assert most >= 7776
+    _fails(lib.bnpvi_leaf_sort(c.p, one, 10, most + 1, one, one, one, one, 1 << 40, None), "L=")
+    _fails(lib.bnpvi_leaf_sort(c.p, one, 1 << 31, 4, one, one, one, one, 1 << 40, None), "slots")
+    need = lib.bnpvi_leaf_sort_workspace(100000, 64)
+    assert need > 0 and lib.bnpvi_leaf_sort_workspace(100, 64) == 0
+    assert lib.bnpvi_leaf_sort_workspace(-1, 64) == -1 and lib.bnpvi_leaf_sort_workspace(5, 0) == -1
+    _fails(lib.bnpvi_leaf_sort(c.p, one, 100000, 64, one, one, one, one, need - 1, None), "workspace")
+    _fails(lib.bnpvi_leaf_sort(c.p, one, 100000, 64, one, one, one, None, need, None), "workspace")
+    _fails(lib.bnpvi_rows_to_leaves(c.p, 3, one, 8, 4, 1, 8, one, one, 4, one, 8, None), "dtype")
+    _fails(lib.bnpvi_rows_to_leaves(c.p, 0, one, 7, 4, 1, 8, one, one, 4, one, 8, None), "pitch")
+    _fails(lib.bnpvi_rows_to_leaves(c.p, 0, one, 8, 1 << 30, 2, 8, one, one, 4, one, 8, None), "2^31")
+    _fails(lib.bnpvi_rows_from_leaves(c.p, 0, one, 8, one, None, None, 4, 4, 1, 8, one, 8, None), "NULL")
+    _fails(lib.bnpvi_rows_from_leaves(c.p, 0, one, 8, one, None, one, 4, 4, 0, 8, one, 8, None), "k=0")
+    _fails(lib.bnpvi_rows_from_leaves_backward(c.p, 0, one, 8, one, 8, one, None, one, 4, 4, 1, 8, one, 8, one, None), "NULL")
+
+
+def test_library_refuses_dense():
+    lib, c, one = _lib.lib, _Ctx(), C.c_void_p(256)
+
+    def dense(dtype=0, ldx=8, ldw=8, act=0, offsets=None, G=0, M=4, K=8, n=6, y=one, ldy=6, dact=None, work=one, size=1 << 40):
+        return lib.bnpvi_dense(c.p, dtype, one, ldx, one, ldw, 0, None, 0, act, None, 0, offsets, G, M, K, n, y, ldy, dact, 5,
+                               work, size, None)
+    _fails(dense(dtype=7), "dtype")
+    _fails(dense(act=6), "activation")
+    _fails(dense(ldx=7), "pitches")
+    _fails(dense(ldx=1 << 21), "pitches")
+    _fails(dense(G=2), "offsets")
+    _fails(dense(offsets=one), "offsets")
+    _fails(dense(G=20000, offsets=one), "G=")
+    _fails(dense(K=0), "K=0")
+    _fails(dense(n=(1 << 20) + 1), "n=")
+    _fails(dense(M=1 << 31), "M=")
+    _fails(dense(ldy=5), "pitch of y")
+    _fails(dense(dact=one), "pitch of y")
+    _fails(dense(y=None), "NULL")
+    need = lib.bnpvi_dense_workspace(1, 4096, 4096, 64, 9, 0)
+    assert need > 0
+    _fails(dense(dtype=1, ldx=4096, ldw=4096, K=4096, n=64, ldy=64, M=4096, G=9, offsets=one, size=need - 1), "workspace")
+    _fails(dense(dtype=1, ldx=4096, ldw=4096, K=4096, n=64, ldy=64, M=4096, G=9, offsets=one, work=C.c_void_p(8)), "workspace")
+    assert lib.bnpvi_dense_workspace(5, 1, 1, 1, 0, 0) == -1 and lib.bnpvi_dense_workspace(0, 1, 0, 1, 0, 1) == -1
+
+    def backward(lddy=6, dx=one, work=one, size=1 << 40, dy=one):
+        return lib.bnpvi_dense_backward(c.p, 0, dy, lddy, None, 0, one, 8, one, 8, 0, None, 0, 4, 8, 6, dx, 8, one, one, None, 0,
+                                        work, size, None)
+    _fails(backward(lddy=5), "pitch")
+    _fails(backward(size=0), "workspace")
+    _fails(backward(dy=None), "NULL")
