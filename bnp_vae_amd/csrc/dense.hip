@@ -143,6 +143,7 @@ __global__ __launch_bounds__(1024) void db_kernel(const float* __restrict__ part
   const int64_t t1 = first != nullptr ? clamp_row(first[g + 1], t0, tiles) : tiles;
   float acc = 0.f;
   if (col < n)
+    #pragma unroll 8
     for (int64_t t = t0 + ty; t < t1; t += 16) acc += part[t * n + col];
   sums[ty][tx] = acc;
   __syncthreads();
@@ -175,10 +176,11 @@ __global__ __launch_bounds__(256) void split_epilogue_kernel(const float* __rest
     float z = 0.f;
     for (int k = 0; k < splits; ++k) z += slab[k * elems + i];
     if (a.bias != nullptr) z += (float)reinterpret_cast<const T*>(a.bias)[col];
-    float y, d;
-    activate(a.act, z, y, d);
+    float v[1] = {z}, d[1];
+    activate<sizeof(T) == 2, 1>(a.act, v, d);
+    float y = v[0];
     if (a.res != nullptr) y += (float)reinterpret_cast<const T*>(a.res)[row * a.ldres + col];
-    if (a.dact != nullptr) reinterpret_cast<DT*>(a.dact)[row * a.lddact + col] = (DT)d;
+    if (a.dact != nullptr) reinterpret_cast<DT*>(a.dact)[row * a.lddact + col] = (DT)d[0];
     reinterpret_cast<T*>(a.C)[row * a.ldc + col] = (T)y;
   }
 }
@@ -192,6 +194,10 @@ struct GemmPlan {
 };
 
 static void tile_size(int tile, int& br, int& bc) {
+  if (tile == kTile256) {
+    br = bc = 256;
+    return;
+  }
   br = tile == kTile128 || tile == kTileTall ? 128 : tile == kTile64 ? 64 : 32;
   bc = tile == kTile128 || tile == kTileFlat ? 128 : tile == kTile64 ? 64 : 32;
 }
@@ -210,6 +216,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
     p.tile = kTile64;
   else
     p.tile = ceil_div(rows, 128) * ceil_div(cols, 128) * (kind == kDw ? z : 1) >= 200 || K >= 8192 ? kTile128 : kTile64;
+  if (const char* f = dev_getenv(kind == kFwd ? "BNPVI_TILE_FWD" : kind == kDx ? "BNPVI_TILE_DX" : "BNPVI_TILE_DW")) p.tile = atoi(f);
   int br, bc;
   tile_size(p.tile, br, bc);
   p.row_tiles = ceil_div(rows, br) + (grouped && kind != kDw ? G + 2 : 0);
@@ -223,6 +230,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
     s = std::min(s, per / (4 * bk));
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
   }
+  if (const char* f = dev_getenv(kind == kFwd ? "BNPVI_SPLIT_FWD" : kind == kDx ? "BNPVI_SPLIT_DX" : "BNPVI_SPLIT_DW")) p.splits = atoi(f);
   p.slab = p.splits > 1 ? (size_t)z * p.splits * rows * cols * 4 : 0;
   if (!(kind == kDw) && grouped) p.slab = 0;
   return p;

@@ -17,7 +17,7 @@ typedef f16_t elem_t;
 template <int KIND, int BR, int BC, int WR, int WC, bool DIRECT>
 static int launch_one(const GemmArgs& a, int device, int64_t grid, hipStream_t s) {
   static LdsLimit limit;
-  constexpr int lds = gemm_lds_bytes<BR, BC, WR, WC>();
+  constexpr int lds = gemm_lds_bytes<BR, BC>();
   auto kernel = gemm_kernel<elem_t, KIND, BR, BC, WR, WC, DIRECT>;
   if (lds > 64 * 1024) BNPVI_HIP(limit.raise((const void*)kernel, device));
   kernel<<<(unsigned)grid, (BR / WR) * (BC / WC) * 64, lds, s>>>(a);
@@ -30,6 +30,9 @@ static int launch_tile(const GemmArgs& a, int tile, int device, int64_t grid, hi
   switch (tile) {
     case kTile128:
       return launch_one<KIND, 128, 128, 64, 64, DIRECT>(a, device, grid, s);
+    case kTile256:
+      if constexpr (DIRECT && sizeof(elem_t) == 2) return launch_one<KIND, 256, 256, 128, 64, DIRECT>(a, device, grid, s);
+      return BNPVI_EINVAL;
     case kTile64:
       return launch_one<KIND, 64, 64, 32, 32, DIRECT>(a, device, grid, s);
     case kTileFlat:

@@ -13,8 +13,8 @@
 // Operands whose rows do not start on 16 bytes take the same way through registers in narrower pieces.
 //
 // Products: v_mfma_f32_32x32x16 (bf16, f16) and v_mfma_f32_32x32x2_f32, fp32 accumulation.  S is the first operand of
-// the instruction, so a lane ends with four consecutive columns of one row; the accumulators pass through LDS once
-// more so that the epilogue reads and writes whole 16-byte pieces of rows.
+// the instruction, so a lane ends with four consecutive columns of one row, and after an exchange between lanes with
+// eight: the epilogue reads and writes 16-byte pieces of rows without another pass through LDS.
 #pragma once
 
 #include "layers_common.h"
@@ -39,7 +39,7 @@ struct Deriv<bf16_t> {
 };
 
 enum { kFwd = 0, kDx = 1, kDw = 2 };
-enum { kTile128 = 0, kTile64 = 1, kTileFlat = 2, kTileTall = 3 };      // 128x128, 64x64, 32x128, 128x32
+enum { kTile128 = 0, kTile64 = 1, kTileFlat = 2, kTileTall = 3, kTile256 = 4 };      // 128x128, 64x64, 32x128, 128x32, 256x256
 
 struct GemmArgs {
   const void* R;
@@ -66,41 +66,71 @@ struct GemmArgs {
   float* slab;                 // [group x split][rows][cols] partial sums, or nullptr
 };
 
-__device__ __forceinline__ void activate(int act, float z, float& a, float& d) {
-  switch (act) {
-    case BNPVI_ACT_RELU:
-      a = z > 0.f ? z : (z != z ? z : 0.f);
-      d = z > 0.f ? 1.f : 0.f;
-      break;
-    case BNPVI_ACT_SOFTSIGN: {
-      const float q = 1.f / (1.f + fabsf(z));
-      a = fabsf(z) < __builtin_inff() ? z * q : (z != z ? z : copysignf(1.f, z));
-      d = q * q;
-      break;
+// act(z) and act'(z).  16-bit results (FAST) take the hardware's exp2 and reciprocal (1 ulp each) and the normal
+// distribution function from formula 7.1.26 of Abramowitz and Stegun (|error| of erf below 1.5e-7), whose
+// exp(-z^2 / 2) the derivative of gelu needs anyway: 2^-11 of the largest error a rounding makes.  The accurate
+// functions took as long as the product itself (gelu, 33.5M values: 90 of 195 us).
+template <bool FAST>
+__device__ __forceinline__ float exp_of(float v) {
+  return FAST ? __builtin_amdgcn_exp2f(v * 1.4426950408889634f) : expf(v);
+}
+template <bool FAST>
+__device__ __forceinline__ float inverse(float v) {
+  return FAST ? __builtin_amdgcn_rcpf(v) : 1.f / v;
+}
+
+// v: z -> act(z), d: act'(z)
+template <bool FAST, int E>
+__device__ __forceinline__ void activate(int act, float (&v)[E], float (&d)[E]) {
+  const float inf = __builtin_inff();
+  if (act == BNPVI_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) d[i] = 1.f;
+  } else if (act == BNPVI_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      d[i] = v[i] > 0.f ? 1.f : 0.f;
+      v[i] = v[i] < 0.f ? 0.f : v[i];
     }
-    case BNPVI_ACT_TANH: {
-      // 1 - tanh^2 = 4 e / (1 + e)^2 with e = exp(-2 |z|): no cancellation where tanh is close to 1
-      const float e = expf(-2.f * fabsf(z)), q = 1.f / (1.f + e);
-      a = tanhf(z);
-      d = 4.f * e * q * q;
-      break;
+  } else if (act == BNPVI_ACT_SOFTSIGN) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float z = v[i], q = inverse<FAST>(1.f + fabsf(z));
+      v[i] = fabsf(z) < inf ? z * q : (z != z ? z : copysignf(1.f, z));
+      d[i] = q * q;
     }
-    case BNPVI_ACT_SILU: {
-      const float e = expf(-fabsf(z)), q = 1.f / (1.f + e);     // never overflows
+  } else if (act == BNPVI_ACT_TANH) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      // with e = exp(-2 |z|): tanh = (1 - e) / (1 + e), 1 - tanh^2 = 4 e / (1 + e)^2 without cancellation near 1
+      const float z = v[i], e = exp_of<FAST>(-2.f * fabsf(z)), q = inverse<FAST>(1.f + e);
+      v[i] = FAST ? (fabsf(z) < 0.02f ? z * (1.f - z * z * (1.f / 3.f)) : copysignf((1.f - e) * q, z)) : tanhf(z);
+      d[i] = 4.f * e * q * q;
+    }
+  } else if (act == BNPVI_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float z = v[i], e = exp_of<FAST>(-fabsf(z)), q = inverse<FAST>(1.f + e);     // never overflows
       const float s = z >= 0.f ? q : e * q;
-      a = z == -__builtin_inff() ? 0.f : z * s;
-      d = fabsf(z) < __builtin_inff() ? s * (1.f + z * (1.f - s)) : s;
-      break;
+      v[i] = z == -inf ? 0.f : z * s;
+      d[i] = fabsf(z) < inf ? s * (1.f + z * (1.f - s)) : s;
     }
-    case BNPVI_ACT_GELU: {
-      const float c = 0.5f * erfcf(-0.70710678118654752f * z);
-      a = z == -__builtin_inff() ? 0.f : z * c;
-      d = fabsf(z) < __builtin_inff() ? c + z * (0.39894228040143268f * expf(-0.5f * z * z)) : c;
-      break;
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float z = v[i], e = exp_of<FAST>(-0.5f * z * z);
+      float c;
+      if (FAST) {
+        const float t = inverse<true>(1.f + 0.3275911f * 0.70710678f * fabsf(z));
+        const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float h = 0.5f * p * e;                                          // of the tail beyond |z|
+        c = z >= 0.f ? 1.f - h : (z != z ? z : h);
+      } else {
+        c = 0.5f * erfcf(-0.70710678118654752f * z);
+      }
+      v[i] = z == -inf ? 0.f : z * c;
+      d[i] = fabsf(z) < inf ? c + z * (0.39894228040143268f * e) : c;
     }
-    default:
-      a = z;
-      d = 1.f;
   }
 }
 
@@ -281,11 +311,9 @@ struct Reader {
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 // Workgroup tile BR x BC, wave tile WR x WC.  Two LDS stages: while one is multiplied the other is filled; one barrier
 // a stage.
-template <int BR, int BC, int WR, int WC>
+template <int BR, int BC>
 constexpr int gemm_lds_bytes() {
-  constexpr int stages = 2 * (BR + BC) * 128;
-  constexpr int ep = (BR / WR) * (BC / WC) * WR * (WC + 4) * 4;
-  return stages > ep ? stages : ep;
+  return 2 * (BR + BC) * 128;
 }
 
 template <typename T, int KIND, int BR, int BC, int WR, int WC, bool DIRECT>
@@ -406,91 +434,95 @@ __global__ __launch_bounds__((BR / WR) * (BC / WC) * 64) void gemm_kernel(const 
     }
   }
 
-  // ---- epilogue: the wave's tile through its own part of the LDS
-  __syncthreads();
-  constexpr int P = WC + 4;                  // floats between rows: 16-byte aligned, rows on different banks
-  float* mine = reinterpret_cast<float*>(lds) + wave * WR * P;
-  const int lane = threadIdx.x & 63;
+  // ---- epilogue.  A lane has four consecutive columns (4 h + 0 .. 3 of every eight) of one row; exchanging the upper
+  // half of one four with the lower half of the next between lanes 32 apart makes them eight consecutive ones.
+  const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
-  for (int i = 0; i < FR; ++i)
+  for (int j = 0; j < FC; ++j) {
 #pragma unroll
-    for (int j = 0; j < FC; ++j)
+    for (int p = 0; p < 2; ++p) {
+      const int cl = wc + 32 * j + 16 * p + 8 * h;
+      const int64_t col = col0 + cl;
+      const int left = nc - cl < 8 ? nc - cl : 8;
+      const bool vec = a.cvec && left == 8;
+      float b[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const f32x4 v = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-        *reinterpret_cast<f32x4*>(mine + (32 * i + (lane & 31)) * P + 32 * j + 8 * e + 4 * (lane >> 5)) = v;
+      for (int e = 0; e < 8; ++e) b[e] = 0.f;
+      if (KIND == kFwd && a.bias != nullptr && a.slab == nullptr && g >= 0) {
+        const T* bp = reinterpret_cast<const T*>(a.bias) + g * a.bias_group + col;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) b[e] = (float)bp[e];
       }
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the wave reads only what it wrote itself
-  constexpr int LPR = WC / 8, RPI = 64 / LPR;
-  const int c = (lane % LPR) * 8;
-  const int cl = wc + c;
-  const int64_t col = col0 + cl;
-  if (cl >= nc) return;
-  const int left = nc - cl < 8 ? nc - cl : 8;
-  const bool vec = a.cvec && left == 8;
-  float b[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) b[e] = 0.f;
-  if (KIND == kFwd && a.bias != nullptr && a.slab == nullptr && g >= 0)
-    for (int e = 0; e < left; ++e) b[e] = (float)reinterpret_cast<const T*>(a.bias)[g * a.bias_group + col + e];
-#pragma unroll 2
-  for (int it = 0; it < WR / RPI; ++it) {
-    const int rl = it * RPI + lane / LPR;
-    if (wr + rl >= nr) continue;
-    const int64_t row = row0 + wr + rl;
-    float v[8];
-    const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + rl * P + c), v1 = *reinterpret_cast<const f32x4*>(mine + rl * P + c + 4);
+      for (int i = 0; i < FR; ++i) {
+        float v[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = v0[e];
-      v[e + 4] = v1[e];
-    }
-    if (a.slab != nullptr) {
-      float* out = a.slab + ((int64_t)z * a.rows + row) * a.cols + col;
-      if (left == 8 && a.cols % 4 == 0) {
-        *reinterpret_cast<f32x4*>(out) = v0;
-        *reinterpret_cast<f32x4*>(out + 4) = v1;
-      } else {
-        for (int e = 0; e < left; ++e) out[e] = v[e];
-      }
-      continue;
-    }
-    T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? g * a.c_group : 0) + row * a.ldc + col;
-    if (KIND == kFwd) {
-      typedef typename Deriv<T>::type DT;
-      float d[8], r[8];
-      const T* rp = a.res == nullptr ? nullptr : reinterpret_cast<const T*>(a.res) + row * a.ldres + col;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        r[e] = 0.f;
-        d[e] = 0.f;
-      }
-      if (g >= 0) {
-        if (rp != nullptr) {
-          if (vec)
-            load_vec<T, 8>(rp, r);
-          else
-            for (int e = 0; e < left; ++e) r[e] = (float)rp[e];
+        for (int t = 0; t < 4; ++t) {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][8 * p + t]), __float_as_uint(acc[i][j][8 * p + 4 + t]),
+                                                          false, false);
+          v[t] = __uint_as_float(x[0]);
+          v[t + 4] = __uint_as_float(x[1]);
         }
+        const int rl = wr + 32 * i + (lane & 31);
+        if (rl >= nr || left <= 0) continue;
+        const int64_t row = row0 + rl;
+        if (a.slab != nullptr) {
+          float* out = a.slab + ((int64_t)z * a.rows + row) * a.cols + col;
+          if (left == 8 && a.cols % 4 == 0) {
+            *reinterpret_cast<f32x4*>(out) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4*>(out + 4) = f32x4{v[4], v[5], v[6], v[7]};
+          } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float y;
-          activate(a.act, v[e] + b[e], y, d[e]);
-          v[e] = y + r[e];
+            for (int e = 0; e < 8; ++e)
+              if (e < left) out[e] = v[e];
+          }
+          continue;
+        }
+        T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? g * a.c_group : 0) + row * a.ldc + col;
+        if (KIND == kFwd) {
+          typedef typename Deriv<T>::type DT;
+          constexpr bool FAST = sizeof(T) == 2;
+          float d[8], r[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) r[e] = d[e] = 0.f;
+          if (g >= 0) {
+            if (a.res != nullptr) {
+              const T* rp = reinterpret_cast<const T*>(a.res) + row * a.ldres + col;
+              if (vec) {
+                load_vec<T, 8>(rp, r);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (e < left) r[e] = (float)rp[e];
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += b[e];
+            activate<FAST, 8>(a.act, v, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+          }
+          if (a.dact != nullptr) {
+            DT* dp = reinterpret_cast<DT*>(a.dact) + row * a.lddact + col;
+            if (vec) {
+              store_vec<DT, 8>(dp, d);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (e < left) dp[e] = (DT)d[e];
+            }
+          }
+        }
+        if (vec) {
+          store_vec<T, 8>(out, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < left) out[e] = (T)v[e];
         }
       }
-      if (a.dact != nullptr) {
-        DT* dp = reinterpret_cast<DT*>(a.dact) + row * a.lddact + col;
-        if (vec)
-          store_vec<DT, 8>(dp, d);
-        else
-          for (int e = 0; e < left; ++e) dp[e] = (DT)d[e];
-      }
     }
-    if (vec)
-      store_vec<T, 8>(out, v);
-    else
-      for (int e = 0; e < left; ++e) out[e] = (T)v[e];
   }
 }
 
