@@ -284,17 +284,17 @@ static int access_elems(const void* p, int64_t ld, int64_t group, int64_t extent
 
 static bool wide(const void* p, int64_t ld, int e) { return p == nullptr || ((uintptr_t)p % 16 == 0 && ld * e % 16 == 0); }
 
-static int run_gemm(int kind, int dtype, const GemmPlan& p, GemmArgs& a, int device, hipStream_t s) {
+static int run_gemm(int kind, int dtype, const GemmPlan& p, GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s) {
   const int e = dtype_bytes(dtype);
   a.rv = access_elems(a.R, a.ldr, 0, kind == kDw ? a.rows : a.K, e);
   a.sv = access_elems(a.S, a.lds, a.s_group, kind == kFwd ? a.K : a.cols, e);
-  a.row_tiles = p.row_tiles;
+  a.row_tiles = (int)p.row_tiles;
   a.col_tiles = p.col_tiles;
   a.splits = p.splits;
   const bool direct = a.rv * e == 16 && a.sv * e == 16;
-  return dtype == BNPVI_F32    ? launch_gemm_f32(kind, p.tile, direct, a, device, s)
-         : dtype == BNPVI_BF16 ? launch_gemm_bf16(kind, p.tile, direct, a, device, s)
-                               : launch_gemm_f16(kind, p.tile, direct, a, device, s);
+  return dtype == BNPVI_F32    ? launch_gemm_f32(kind, p.tile, direct, a, ctx, s)
+         : dtype == BNPVI_BF16 ? launch_gemm_bf16(kind, p.tile, direct, a, ctx, s)
+                               : launch_gemm_f16(kind, p.tile, direct, a, ctx, s);
 }
 
 static int row_tiles(const int32_t* offsets, int G, int64_t M, int tile, int64_t ntiles, void* map, void* first, int device,
@@ -413,7 +413,7 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
     a.map = (const int4*)(wk + p.fwd_map);
   }
   if (p.fwd.slab) a.slab = (float*)(wk + p.fwd_slab);
-  const int r = run_gemm(kFwd, dtype, p.fwd, a, ctx->device, s);
+  const int r = run_gemm(kFwd, dtype, p.fwd, a, ctx, s);
   if (r) return r;
   if (p.fwd.slab) {
     const unsigned g = flat_grid(M * n);
@@ -509,7 +509,7 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
       a.map = (const int4*)(wk + p.dx_map);
     }
     if (p.dx.slab) a.slab = (float*)(wk + p.slab);
-    r = run_gemm(kDx, dtype, p.dx, a, ctx->device, s);
+    r = run_gemm(kDx, dtype, p.dx, a, ctx, s);
     if (r) return r;
     if (p.dx.slab) {
       // no epilogue: a plain sum over the splits into rows of pitch lddx
@@ -541,7 +541,7 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.c_group = n * K;
     a.cvec = wide(dw, K, e) && (groups == 1 || n * K * e % 16 == 0);
     if (p.dw.slab) a.slab = (float*)(wk + p.slab);
-    r = run_gemm(kDw, dtype, p.dw, a, ctx->device, s);
+    r = run_gemm(kDw, dtype, p.dw, a, ctx, s);
     if (r) return r;
     if (p.dw.slab) {
       if (dtype == BNPVI_F32)

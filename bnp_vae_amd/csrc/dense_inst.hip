@@ -15,46 +15,47 @@ typedef f16_t elem_t;
 #endif
 
 template <int KIND, int BR, int BC, int WR, int WC, bool DIRECT>
-static int launch_one(const GemmArgs& a, int device, int64_t grid, hipStream_t s) {
+static int launch_one(const GemmArgs& a, const bnpvi_ctx* ctx, int64_t tiles, hipStream_t s) {
   static LdsLimit limit;
-  constexpr int lds = gemm_lds_bytes<BR, BC>();
-  auto kernel = gemm_kernel<elem_t, KIND, BR, BC, WR, WC, DIRECT>;
-  if (lds > 64 * 1024) BNPVI_HIP(limit.raise((const void*)kernel, device));
-  kernel<<<(unsigned)grid, (BR / WR) * (BC / WC) * 64, lds, s>>>(a);
+  constexpr int threads = (BR / WR) * (BC / WC) * 64, lds = Rings<BR, BC, 128, KIND, DIRECT>::kBytes;
+  auto kernel = gemm_kernel<elem_t, KIND, BR, BC, WR, WC, 128, DIRECT>;
+  if (lds > 64 * 1024) BNPVI_HIP(limit.raise((const void*)kernel, ctx->device));
+  // as many workgroups as fit a CU (LDS; two waves a SIMD of the larger tiles fill the registers), no more than tiles
+  const int64_t per_cu = std::min(kMaxLdsBytes / lds, 1024 / threads);
+  kernel<<<(unsigned)std::min<int64_t>(tiles, per_cu * ctx->num_cu), threads, lds, s>>>(a, (uint32_t)tiles);
   BNPVI_LAUNCH_CHECK();
   return BNPVI_OK;
 }
 
 template <int KIND, bool DIRECT>
-static int launch_tile(const GemmArgs& a, int tile, int device, int64_t grid, hipStream_t s) {
+static int launch_tile(const GemmArgs& a, int tile, const bnpvi_ctx* ctx, int64_t tiles, hipStream_t s) {
   switch (tile) {
-    case kTile128:
-      return launch_one<KIND, 128, 128, 64, 64, DIRECT>(a, device, grid, s);
     case kTile256:
-      if constexpr (DIRECT && sizeof(elem_t) == 2) return launch_one<KIND, 256, 256, 128, 64, DIRECT>(a, device, grid, s);
+      if constexpr (DIRECT && sizeof(elem_t) == 2) return launch_one<KIND, 256, 256, 128, 64, DIRECT>(a, ctx, tiles, s);
       return BNPVI_EINVAL;
+    case kTile128:
+      return launch_one<KIND, 128, 128, 64, 64, DIRECT>(a, ctx, tiles, s);
     case kTile64:
-      return launch_one<KIND, 64, 64, 32, 32, DIRECT>(a, device, grid, s);
+      return launch_one<KIND, 64, 64, 32, 32, DIRECT>(a, ctx, tiles, s);
     case kTileFlat:
-      return launch_one<KIND, 32, 128, 32, 32, DIRECT>(a, device, grid, s);
+      return launch_one<KIND, 32, 128, 32, 32, DIRECT>(a, ctx, tiles, s);
     default:
-      return launch_one<KIND, 128, 32, 32, 32, DIRECT>(a, device, grid, s);
+      return launch_one<KIND, 128, 32, 32, 32, DIRECT>(a, ctx, tiles, s);
   }
 }
 
-int BNPVI_GEMM_LAUNCH(int kind, int tile, bool direct, const GemmArgs& a, int device, hipStream_t s) {
-  const int64_t z = kind == kDw ? (int64_t)a.G * a.splits : a.splits;
-  const int64_t grid = a.row_tiles * a.col_tiles * z;
-  if (grid <= 0) return BNPVI_OK;
-  BNPVI_REQUIRE(grid < (int64_t(1) << 31), "dense: %lld workgroups", (long long)grid);
+int BNPVI_GEMM_LAUNCH(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s) {
+  const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles * (kind == kDw ? (int64_t)a.G * a.splits : a.splits);
+  if (tiles <= 0) return BNPVI_OK;
+  BNPVI_REQUIRE(tiles < (int64_t(1) << 31), "dense: %lld tiles", (long long)tiles);
   if (direct) {
-    if (kind == kFwd) return launch_tile<kFwd, true>(a, tile, device, grid, s);
-    if (kind == kDx) return launch_tile<kDx, true>(a, tile, device, grid, s);
-    return launch_tile<kDw, true>(a, tile, device, grid, s);
+    if (kind == kFwd) return launch_tile<kFwd, true>(a, tile, ctx, tiles, s);
+    if (kind == kDx) return launch_tile<kDx, true>(a, tile, ctx, tiles, s);
+    return launch_tile<kDw, true>(a, tile, ctx, tiles, s);
   }
-  if (kind == kFwd) return launch_tile<kFwd, false>(a, tile, device, grid, s);
-  if (kind == kDx) return launch_tile<kDx, false>(a, tile, device, grid, s);
-  return launch_tile<kDw, false>(a, tile, device, grid, s);
+  if (kind == kFwd) return launch_tile<kFwd, false>(a, tile, ctx, tiles, s);
+  if (kind == kDx) return launch_tile<kDx, false>(a, tile, ctx, tiles, s);
+  return launch_tile<kDw, false>(a, tile, ctx, tiles, s);
 }
 
 }  // namespace bnpvi

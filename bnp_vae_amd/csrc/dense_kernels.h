@@ -13,8 +13,8 @@
 // Operands whose rows do not start on 16 bytes take the same way through registers in narrower pieces.
 //
 // Products: v_mfma_f32_32x32x16 (bf16, f16) and v_mfma_f32_32x32x2_f32, fp32 accumulation.  S is the first operand of
-// the instruction, so a lane ends with four consecutive columns of one row, and after an exchange between lanes with
-// eight: the epilogue reads and writes 16-byte pieces of rows without another pass through LDS.
+// the instruction, so a lane ends with four consecutive columns of one row; the accumulators pass through LDS once
+// more so that the epilogue reads and writes whole 16-byte pieces of rows, eight lanes and more a row.
 #pragma once
 
 #include "layers_common.h"
@@ -50,8 +50,7 @@ struct GemmArgs {
   const int32_t* offsets;      // groups' bounds (kDw) or nullptr
   const int4* map;             // row tiles {group, first row, end row} (kFwd, kDx with groups) or nullptr
   int G, splits;
-  int64_t row_tiles;
-  int col_tiles;
+  int row_tiles, col_tiles;
   int rv, sv;                  // elements per access of R and S where a row does not start on 16 bytes
   int cvec;                    // C, residual and derivative take 16-byte accesses
   void* C;
@@ -79,10 +78,11 @@ __device__ __forceinline__ float inverse(float v) {
   return FAST ? __builtin_amdgcn_rcpf(v) : 1.f / v;
 }
 
-// v: z -> act(z), d: act'(z)
+// v: z -> act(z), d: act'(z).  Limits at infinities come from clamped factors, not branches; NaN passes through.
+__device__ __forceinline__ float clamped(float v, float at) { return __builtin_amdgcn_fmed3f(v, -at, at); }
+
 template <bool FAST, int E>
 __device__ __forceinline__ void activate(int act, float (&v)[E], float (&d)[E]) {
-  const float inf = __builtin_inff();
   if (act == BNPVI_ACT_NONE) {
 #pragma unroll
     for (int i = 0; i < E; ++i) d[i] = 1.f;
@@ -95,9 +95,9 @@ __device__ __forceinline__ void activate(int act, float (&v)[E], float (&d)[E]) 
   } else if (act == BNPVI_ACT_SOFTSIGN) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float z = v[i], q = inverse<FAST>(1.f + fabsf(z));
-      v[i] = fabsf(z) < inf ? z * q : (z != z ? z : copysignf(1.f, z));
-      d[i] = q * q;
+      const float z = v[i], m = fminf(fabsf(z), 1e30f), q = inverse<FAST>(1.f + m);
+      v[i] = z != z ? z : copysignf(m * q, z);
+      d[i] = z != z ? z : q * q;
     }
   } else if (act == BNPVI_ACT_TANH) {
 #pragma unroll
@@ -110,10 +110,9 @@ __device__ __forceinline__ void activate(int act, float (&v)[E], float (&d)[E]) 
   } else if (act == BNPVI_ACT_SILU) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float z = v[i], e = exp_of<FAST>(-fabsf(z)), q = inverse<FAST>(1.f + e);     // never overflows
-      const float s = z >= 0.f ? q : e * q;
-      v[i] = z == -inf ? 0.f : z * s;
-      d[i] = fabsf(z) < inf ? s * (1.f + z * (1.f - s)) : s;
+      const float z = v[i], s = inverse<FAST>(1.f + exp_of<FAST>(-z));         // exp may be infinite: s = 0
+      v[i] = s * fmaxf(z, -3e38f);
+      d[i] = s * (1.f + clamped(z, 1e4f) * (1.f - s));
     }
   } else {
 #pragma unroll
@@ -124,12 +123,12 @@ __device__ __forceinline__ void activate(int act, float (&v)[E], float (&d)[E]) 
         const float t = inverse<true>(1.f + 0.3275911f * 0.70710678f * fabsf(z));
         const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
         const float h = 0.5f * p * e;                                          // of the tail beyond |z|
-        c = z >= 0.f ? 1.f - h : (z != z ? z : h);
+        c = z < 0.f ? h : 1.f - h;
       } else {
         c = 0.5f * erfcf(-0.70710678118654752f * z);
       }
-      v[i] = z == -inf ? 0.f : z * c;
-      d[i] = fabsf(z) < inf ? c + z * (0.39894228040143268f * e) : c;
+      v[i] = c * fmaxf(z, -3e38f);
+      d[i] = c + clamped(z, 1e4f) * (0.39894228040143268f * e);
     }
   }
 }
@@ -144,50 +143,55 @@ __device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t r, char* l,
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)l, 16, off, 0, 0, 0);
 }
 
-// Where the 16-byte pieces of one operand stage come from.  B rows (KM) or columns (MM), P pieces a lane.
-template <typename T, bool KM, int B, int THREADS>
+// piece c of KM row r sits at c ^ swizzle(r): eight consecutive rows, read at the same k, fall on different 16 bytes of
+// the 128 that one cycle of the LDS serves
+template <int KB>
+__device__ __forceinline__ int swizzle(int r) {
+  return KB == 128 ? r & 7 : (r >> 1) & 3;
+}
+
+// Where the 16-byte pieces of one operand stage (KB bytes of k) come from.  B rows (KM) or columns (MM), P pieces a lane.
+template <typename T, bool KM, int B, int THREADS, int KB>
 struct Source {
-  static constexpr int kP = B * 8 / THREADS;
+  static constexpr int kP = B * (KB / 16) / THREADS;
   static constexpr int kPer = 16 / (int)sizeof(T);                 // elements of a piece
-  static constexpr int kBK = 128 / (int)sizeof(T);                 // k's of a stage
-  static constexpr int kRow = KM ? 8 : B * (int)sizeof(T) / 16;    // pieces of an LDS row
+  static constexpr int kBK = KB / (int)sizeof(T);                  // k's of a stage
+  static constexpr int kRow = KM ? KB / 16 : B * (int)sizeof(T) / 16;    // pieces of an LDS row
   static constexpr int kUnits = B / 16;                            // 32-byte units of a 16-bit MM row
-  static_assert(B * 8 % THREADS == 0, "whole pieces per lane");
+  static_assert(kP > 0 && B * (KB / 16) % THREADS == 0, "whole pieces per lane");
 
   const char* base;      // first element of the tile's rows (KM) / columns (MM) at k = 0
   int64_t pitch;         // bytes
-  int n, k;              // rows / columns left in the matrix, k's of this workgroup
-  int row[kP], piece[kP];
+  int n, k;              // rows / columns left in the matrix, k's of this tile
+  uint32_t off[kP];      // of a lane's pieces from the stage's first byte; kOutside behind the last row / column
 
+  static __device__ __forceinline__ int row(int q) { return (q * THREADS + (int)threadIdx.x) / kRow; }
+  static __device__ __forceinline__ int piece(int q) {
+    const int r = row(q), c = (q * THREADS + (int)threadIdx.x) % kRow;
+    if (KM) return c ^ swizzle<KB>(r);
+    if (sizeof(T) == 2) return (((c >> 1) ^ (r & (kUnits - 1))) << 1) | (c & 1);
+    return c;
+  }
   __device__ __forceinline__ void init(const void* p, int64_t ld, int left, int kext) {
     base = reinterpret_cast<const char*>(p);
     pitch = ld * (int64_t)sizeof(T);
     n = left;
     k = kext;
 #pragma unroll
-    for (int q = 0; q < kP; ++q) {
-      const int i = q * THREADS + threadIdx.x;
-      const int r = i / kRow, c = i % kRow;
-      row[q] = r;
-      if (KM)
-        piece[q] = c ^ (r & 7);
-      else if (sizeof(T) == 2)
-        piece[q] = (((c >> 1) ^ (r & (kUnits - 1))) << 1) | (c & 1);
-      else
-        piece[q] = c;
-    }
+    for (int q = 0; q < kP; ++q)
+      off[q] = (KM ? row(q) : piece(q) * kPer) < n ? (uint32_t)row(q) * (uint32_t)pitch + (uint32_t)piece(q) * 16u : kOutside;
   }
   // every piece of stage kt straight into LDS (wave-uniform base + 16 bytes a lane)
   __device__ __forceinline__ void to_lds(int kt, char* lds) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const char* at = base + (KM ? (int64_t)kt * 128 : (int64_t)kt * kBK * pitch);
-    const __amdgpu_buffer_rsrc_t rs = rsrc_of(at);
+    const __amdgpu_buffer_rsrc_t rs = rsrc_of(base + (KM ? (int64_t)kt * KB : (int64_t)kt * kBK * pitch));
+    if (kt * kBK + kBK <= k) {
 #pragma unroll
-    for (int q = 0; q < kP; ++q) {
-      const int kk = kt * kBK + (KM ? piece[q] * kPer : row[q]);
-      const int nn = KM ? row[q] : piece[q] * kPer;
-      const uint32_t off = (uint32_t)row[q] * (uint32_t)pitch + (uint32_t)piece[q] * 16u;
-      buffer_to_lds(rs, lds + (q * THREADS + wave * 64) * 16, kk < k && nn < n ? off : kOutside);
+      for (int q = 0; q < kP; ++q) buffer_to_lds(rs, lds + (q * THREADS + wave * 64) * 16, off[q]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kP; ++q)
+        buffer_to_lds(rs, lds + (q * THREADS + wave * 64) * 16, kt * kBK + (KM ? piece(q) * kPer : row(q)) < k ? off[q] : kOutside);
     }
   }
   // the same through registers, V elements an access (V divides the pitch, the base and the contiguous extent)
@@ -203,10 +207,10 @@ struct Source {
       x.u = u32x4{0, 0, 0, 0};
 #pragma unroll
       for (int e = 0; e < kPer / V; ++e) {
-        const int kk = kt * kBK + (KM ? piece[q] * kPer + e * V : row[q]);
-        const int nn = KM ? row[q] : piece[q] * kPer + e * V;
+        const int kk = kt * kBK + (KM ? piece(q) * kPer + e * V : row(q));
+        const int nn = KM ? row(q) : piece(q) * kPer + e * V;
         if (kk < k && nn < n) {
-          const int64_t r = KM ? row[q] : kk, c = KM ? kk : nn;
+          const int64_t r = KM ? row(q) : kk, c = KM ? kk : nn;
           x.v[e] = *reinterpret_cast<const vec*>(base + r * pitch + c * (int64_t)sizeof(T));
         }
       }
@@ -272,7 +276,7 @@ struct Frag<f16_t> {
 
 // Fragment `f` (32 rows) of an operand stage for k-step s: lane (i = lane % 32, h = lane / 32) gets row 32 f + i, and
 // k = (2 s + h) kPer + 0 .. kPer - 1 -- the same k's for both kinds of operand, which is all a product needs.
-template <typename T, bool KM, int B>
+template <typename T, bool KM, int B, int KB>
 struct Reader {
   int off[4];      // KM: byte offset of each k-step's piece; 16-bit MM: of each pair (first / second four k's)
   int lane;
@@ -281,7 +285,7 @@ struct Reader {
     const int i = lane & 31, h = lane >> 5;
     if (KM) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) off[s] = (row0 + i) * 128 + (((2 * s + h) ^ (i & 7)) << 4);
+      for (int s = 0; s < KB / 32; ++s) off[s] = (row0 + i) * KB + (((2 * s + h) ^ swizzle<KB>(i)) << 4);
     } else if (sizeof(T) == 2) {
       off[0] = (h * 8 + ((lane & 15) >> 2)) * (B * 2) + (lane & 3) * 8;     // the unit is added per fragment
       off[1] = row0 / 16 + ((lane >> 4) & 1);
@@ -291,7 +295,7 @@ struct Reader {
   }
   __device__ __forceinline__ typename Frag<T>::type get(const char* lds, int f, int s) const {
     if constexpr (KM) {
-      return *reinterpret_cast<const typename Frag<T>::type*>(lds + off[s] + f * 32 * 128);
+      return *reinterpret_cast<const typename Frag<T>::type*>(lds + off[s] + f * 32 * KB);
     } else if constexpr (sizeof(T) == 2) {
       constexpr int U = B / 16;
       const int kk = (lane & 15) >> 2, u = off[1] + 2 * f;
@@ -308,205 +312,318 @@ struct Reader {
   }
 };
 
-// ---- the kernel ----------------------------------------------------------------------------------------------------
-// Workgroup tile BR x BC, wave tile WR x WC.  Two LDS stages: while one is multiplied the other is filled; one barrier
-// a stage.
-template <int BR, int BC>
-constexpr int gemm_lds_bytes() {
-  return 2 * (BR + BC) * 128;
+// at most N vector memory operations of this wave still on their way (expcnt and lgkmcnt left alone)
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <typename T, int KIND, int BR, int BC, int WR, int WC, bool DIRECT>
-__global__ __launch_bounds__((BR / WR) * (BC / WC) * 64) void gemm_kernel(const GemmArgs a) {
-  constexpr int THREADS = (BR / WR) * (BC / WC) * 64;
-  constexpr bool RKM = KIND != kDw, SKM = KIND == kFwd;
-  constexpr int FR = WR / 32, FC = WC / 32, BK = 128 / (int)sizeof(T);
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+// ---- the kernel ----------------------------------------------------------------------------------------------------
+// Workgroup tile BR x BC, wave tile WR x WC, stages of KB bytes of k.  The operand that comes from far (x or dz in the
+// forward and dx products, x in the dW product) has a ring of three stages in LDS, the other one of two; through
+// registers both have two.  One barrier a stage.
+template <int BR, int BC, int KB, int KIND, bool DIRECT>
+struct Rings {
+  static constexpr int kR = DIRECT && KIND != kDw ? 3 : 2, kS = DIRECT && KIND == kDw ? 3 : 2;
+  static constexpr int kBytes = (kR * BR + kS * BC) * KB;
+};
 
-  // Workgroups go to the eight XCDs in turn; each XCD gets a contiguous run of tiles, columns first, so that the tiles
-  // that share rows of R share an L2.
-  const int64_t total = (int64_t)gridDim.x;
-  const int64_t x = blockIdx.x & 7, q8 = total >> 3, rem = total & 7;
-  const int64_t lin = x * q8 + (x < rem ? x : rem) + (blockIdx.x >> 3);
-  const int ct = (int)(lin % a.col_tiles);
-  const int64_t rt = (lin / a.col_tiles) % a.row_tiles;
-  const int z = (int)(lin / a.col_tiles / a.row_tiles);
-  const int split = z % a.splits;
-  int g = z / a.splits;
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
-  int64_t row0 = rt * BR, row_end = a.rows;
-  const int64_t col0 = (int64_t)ct * BC;
-  int64_t k_lo = 0, k_hi = a.K;
+// One output tile: its place in C, its group, its part of the sum.
+struct Tile {
+  int64_t row0, col0, k_lo;
+  int nr, nc, kext, g, z;
+  // stages of the sum; an empty one is one stage of zeros
+  __device__ __forceinline__ int stages(int bk) const { return kext > bk ? (kext + bk - 1) / bk : 1; }
+};
+
+template <int KIND, int BR, int BC, int BK>
+__device__ __forceinline__ bool find_tile(const GemmArgs& a, uint32_t lin, Tile& t) {
+  // divisions are done by the vector unit: their results are told to be the same in every lane
+  const uint32_t row = uniform(lin / (uint32_t)a.col_tiles), ct = lin - row * (uint32_t)a.col_tiles;
+  const uint32_t zz = uniform(row / (uint32_t)a.row_tiles), rt = row - zz * (uint32_t)a.row_tiles;
+  t.z = (int)zz;
+  t.g = (int)uniform(zz / (uint32_t)a.splits);
+  const int split = (int)zz - t.g * a.splits;
+  t.row0 = (int64_t)rt * BR;
+  t.col0 = (int64_t)ct * BC;
+  int64_t row_end = a.rows, k_lo = 0, k_hi = a.K;
   if (KIND == kDw) {
     if (a.offsets != nullptr) {
-      const int64_t M = a.K;
-      int64_t lo = a.offsets[g], hi = a.offsets[g + 1];
+      const int64_t M = a.K, lo = a.offsets[t.g], hi = a.offsets[t.g + 1];
       k_lo = lo < 0 ? 0 : lo > M ? M : lo;
       k_hi = hi < k_lo ? k_lo : hi > M ? M : hi;
     }
   } else if (a.map != nullptr) {
     const int4 m = a.map[rt];
-    g = m.x;
-    row0 = m.y;
+    t.g = m.x;
+    t.row0 = m.y;
     row_end = m.z;
-    if (row0 >= row_end) return;
+    if (t.row0 >= row_end) return false;
   }
   if (a.splits > 1) {
-    const int64_t per = ((k_hi - k_lo + a.splits - 1) / a.splits + BK - 1) / BK * BK;
+    const uint32_t each = uniform((uint32_t)(k_hi - k_lo + a.splits - 1) / (uint32_t)a.splits);      // k's: below 2^31
+    const int64_t per = ((int64_t)each + BK - 1) / BK * BK;
     k_lo = k_lo + split * per < k_hi ? k_lo + split * per : k_hi;
     k_hi = k_lo + per < k_hi ? k_lo + per : k_hi;
   }
-  const int nr = (int)(row_end - row0 < BR ? row_end - row0 : BR);
-  const int nc = (int)(a.cols - col0 < BC ? a.cols - col0 : BC);
-  const int kext = g < 0 ? 0 : (int)(k_hi - k_lo);           // a tile of rows without a leaf has nothing to add up
-  const int gs = g < 0 ? 0 : g;
+  t.nr = (int)(row_end - t.row0 < BR ? row_end - t.row0 : BR);
+  t.nc = (int)(a.cols - t.col0 < BC ? a.cols - t.col0 : BC);
+  t.k_lo = k_lo;
+  t.kext = t.g < 0 ? 0 : (int)(k_hi - k_lo);           // a tile of rows without a leaf has nothing to add up
+  return true;
+}
 
-  const T* Rp = reinterpret_cast<const T*>(a.R) + (RKM ? row0 * a.ldr + k_lo : k_lo * a.ldr + row0);
-  const T* Sp = reinterpret_cast<const T*>(a.S) + (KIND == kDw ? 0 : gs * a.s_group) +
-                (SKM ? col0 * a.lds + k_lo : k_lo * a.lds + col0);
-  Source<T, RKM, BR, THREADS> sr;
-  Source<T, SKM, BC, THREADS> ss;
-  sr.init(Rp, a.ldr, nr, kext);
-  ss.init(Sp, a.lds, nc, kext);
+// The stages of one operand, tile after tile of this workgroup, in the order in which they are multiplied.
+template <typename T, int KIND, int BR, int BC, int KB, int THREADS, bool ROWS>
+struct Stream {
+  static constexpr bool kKM = ROWS ? KIND != kDw : KIND == kFwd;
+  static constexpr int kBK = KB / (int)sizeof(T);
+  typedef Source<T, kKM, ROWS ? BR : BC, THREADS, KB> Src;
+  Src src;
+  uint32_t lin, last, step;
+  int kt, nk;
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __device__ __forceinline__ void begin(const GemmArgs& a, uint32_t first, uint32_t end, uint32_t every) {
+    lin = first;
+    last = end;
+    step = every;
+    enter(a);
+  }
+  __device__ __forceinline__ void enter(const GemmArgs& a) {
+    Tile t;
+    kt = 0;
+    for (; lin < last; lin += step)
+      if (find_tile<KIND, BR, BC, kBK>(a, lin, t)) {
+        lin += step;
+        const int g = t.g < 0 ? 0 : t.g;
+        if (ROWS)
+          src.init(reinterpret_cast<const T*>(a.R) + (kKM ? t.row0 * a.ldr + t.k_lo : t.k_lo * a.ldr + t.row0), a.ldr, t.nr, t.kext);
+        else
+          src.init(reinterpret_cast<const T*>(a.S) + (KIND == kDw ? 0 : g * a.s_group) +
+                       (kKM ? t.col0 * a.lds + t.k_lo : t.k_lo * a.lds + t.col0),
+                   a.lds, t.nc, t.kext);
+        nk = t.stages(kBK);
+        return;
+      }
+    src.k = 0;                 // behind the last tile: zeros, so that the count of loads on their way stays the same
+    nk = 0x7fffffff;
+  }
+  __device__ __forceinline__ void step_on(const GemmArgs& a) {
+    if (++kt == nk) enter(a);
+  }
+};
+
+// The grid is as many workgroups as the chip holds at once; each takes tile after tile.  Workgroups go to the eight
+// XCDs in turn; every XCD owns a contiguous run of tiles, columns first, which its workgroups walk side by side, so that
+// the tiles that share rows of R share an L2.  The operands' stages follow each other across tiles, so the next tile
+// arrives while the last stages of this one are multiplied and while its epilogue runs.
+template <typename T, int KIND, int BR, int BC, int WR, int WC, int KB, bool DIRECT>
+__global__ __launch_bounds__((BR / WR) * (BC / WC) * 64) __attribute__((amdgpu_waves_per_eu(BR * BC >= 128 * 128 ? 2 : 4)))
+void gemm_kernel(const GemmArgs a, uint32_t tiles) {
+  constexpr int THREADS = (BR / WR) * (BC / WC) * 64, WAVES = THREADS / 64;
+  constexpr bool RKM = KIND != kDw, SKM = KIND == kFwd;
+  constexpr int FR = WR / 32, FC = WC / 32, BK = KB / (int)sizeof(T);
+  typedef Rings<BR, BC, KB, KIND, DIRECT> Ring;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char* const ring_s = lds + Ring::kR * BR * KB;
+
+  const uint32_t xcd = blockIdx.x & 7, q8 = tiles >> 3, rem = tiles & 7;
+  const uint32_t step = (gridDim.x + 7 - xcd) >> 3;
+  const uint32_t first = xcd * q8 + (xcd < rem ? xcd : rem), last = first + q8 + (xcd < rem ? 1 : 0);
+  uint32_t lin = first + (blockIdx.x >> 3);
+  if (lin >= last) return;
+  Stream<T, KIND, BR, BC, KB, THREADS, true> sr;
+  Stream<T, KIND, BR, BC, KB, THREADS, false> ss;
+  sr.begin(a, lin, last, step);
+  ss.begin(a, lin, last, step);
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave / (BC / WC) * WR, wc = wave % (BC / WC) * WC;
-  Reader<T, RKM, BR> rr;
-  Reader<T, SKM, BC> rs;
+  Reader<T, RKM, BR, KB> rr;
+  Reader<T, SKM, BC, KB> rs;
   rr.init(wr);
   rs.init(wc);
 
-  f32x16 acc[FR][FC];
-#pragma unroll
-  for (int i = 0; i < FR; ++i)
-#pragma unroll
-    for (int j = 0; j < FC; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
-  constexpr int STAGE = (BR + BC) * 128;
-  const int nk = (kext + BK - 1) / BK;
-  auto multiply = [&](const char* stage) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      typename Frag<T>::type fr[FR], fc[FC];
-#pragma unroll
-      for (int i = 0; i < FR; ++i) fr[i] = rr.get(stage, i, s);
-#pragma unroll
-      for (int j = 0; j < FC; ++j) fc[j] = rs.get(stage + BR * 128, j, s);
-#pragma unroll
-      for (int i = 0; i < FR; ++i)
-#pragma unroll
-        for (int j = 0; j < FC; ++j) Frag<T>::mma(fc[j], fr[i], acc[i][j]);
+  u32x4 hr[DIRECT ? 1 : decltype(sr.src)::kP], hs[DIRECT ? 1 : decltype(ss.src)::kP];
+  int fill_r = 0, fill_s = 0, use_r = 0, use_s = 0;          // ring positions
+  auto load_r = [&] {
+    if constexpr (DIRECT) {
+      sr.src.to_lds(sr.kt, lds + fill_r * (BR * KB));
+      fill_r = fill_r == Ring::kR - 1 ? 0 : fill_r + 1;
+    } else {
+      sr.src.fetch_any(a.rv, sr.kt, hr);
     }
+    sr.step_on(a);
   };
-  if constexpr (DIRECT) {
-    if (nk > 0) {
-      sr.to_lds(0, lds);
-      ss.to_lds(0, lds + BR * 128);
+  auto load_s = [&] {
+    if constexpr (DIRECT) {
+      ss.src.to_lds(ss.kt, ring_s + fill_s * (BC * KB));
+      fill_s = fill_s == Ring::kS - 1 ? 0 : fill_s + 1;
+    } else {
+      ss.src.fetch_any(a.sv, ss.kt, hs);
     }
-    for (int kt = 0; kt < nk; ++kt) {
-      // this stage has arrived, and every wave is done reading the other one (its stage kt - 1)
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (kt + 1 < nk) {
-        char* next = lds + ((kt + 1) & 1) * STAGE;
-        sr.to_lds(kt + 1, next);
-        ss.to_lds(kt + 1, next + BR * 128);
-      }
-      multiply(lds + (kt & 1) * STAGE);
-    }
-  } else {
-    u32x4 hr[decltype(sr)::kP], hs[decltype(ss)::kP];
-    if (nk > 0) {
-      sr.fetch_any(a.rv, 0, hr);
-      ss.fetch_any(a.sv, 0, hs);
-    }
-    for (int kt = 0; kt < nk; ++kt) {
-      char* stage = lds + (kt & 1) * STAGE;
-      sr.put(stage, hr);
-      ss.put(stage + BR * 128, hs);
-      __syncthreads();                       // the stage written two turns ago is free: its readers passed this barrier
-      if (kt + 1 < nk) {
-        sr.fetch_any(a.rv, kt + 1, hr);
-        ss.fetch_any(a.sv, kt + 1, hs);
-      }
-      multiply(stage);
-    }
-  }
+    ss.step_on(a);
+  };
+  // the operand with the longer ring is loaded last: its newest stage is what may still be on its way at a barrier
+  constexpr bool DEEP_R = Ring::kR == 3, DEEP_S = Ring::kS == 3;
+  constexpr int AHEAD = DEEP_R ? decltype(sr.src)::kP : DEEP_S ? decltype(ss.src)::kP : 0;
+  load_r();
+  load_s();
+  if (DEEP_R) load_r();
+  if (DEEP_S) load_s();
 
-  // ---- epilogue.  A lane has four consecutive columns (4 h + 0 .. 3 of every eight) of one row; exchanging the upper
-  // half of one four with the lower half of the next between lanes 32 apart makes them eight consecutive ones.
-  const int lane = threadIdx.x & 63, h = lane >> 5;
+  // vector stores of a full tile's epilogue that a wave issues behind its loads (0: unknown, wait for all of them)
+  constexpr int LPR = WC / 8, RPI = 64 / LPR, SLOTS = WC / 4;
+  constexpr int Y_OPS = FR * (32 / RPI) * (int)sizeof(T) / 2;
+  constexpr int D_OPS = FR * (32 / RPI) * (int)sizeof(typename Deriv<T>::type) / 2;
+  int behind = 0;
+
+  Tile t;
+  for (; lin < last; lin += step) {
+    if (!find_tile<KIND, BR, BC, BK>(a, lin, t)) continue;
+    f32x16 acc[FR][FC];
 #pragma unroll
-  for (int j = 0; j < FC; ++j) {
+    for (int i = 0; i < FR; ++i)
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int cl = wc + 32 * j + 16 * p + 8 * h;
-      const int64_t col = col0 + cl;
-      const int left = nc - cl < 8 ? nc - cl : 8;
-      const bool vec = a.cvec && left == 8;
-      float b[8];
+      for (int j = 0; j < FC; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = 0.f;
-      if (KIND == kFwd && a.bias != nullptr && a.slab == nullptr && g >= 0) {
-        const T* bp = reinterpret_cast<const T*>(a.bias) + g * a.bias_group + col;
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    const int nk = t.stages(BK);
+    for (int kt = 0; kt < nk; ++kt) {
+      char* const at_r = lds + use_r * (BR * KB);
+      char* const at_s = ring_s + use_s * (BC * KB);
+      if constexpr (!DIRECT) {
+        sr.src.put(at_r, hr);
+        ss.src.put(at_s, hs);
+      } else {
+        // this stage of both operands has arrived (vector memory operations end in the order of their issue)
+        if (behind == 0)
+          wait_loads<AHEAD>();
+        else if (behind == 1)
+          wait_loads<AHEAD + Y_OPS>();
+        else
+          wait_loads<AHEAD + Y_OPS + D_OPS>();
+        behind = 0;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // ... and all waves are done with the one before
+      typename Frag<T>::type fr[2][FR], fc[2][FC];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < left) b[e] = (float)bp[e];
+      for (int i = 0; i < FR; ++i) fr[0][i] = rr.get(at_r, i, 0);
+#pragma unroll
+      for (int j = 0; j < FC; ++j) fc[0][j] = rs.get(at_s, j, 0);
+      if (DEEP_S) {
+        load_r();
+        load_s();
+      } else {
+        load_s();
+        load_r();
       }
 #pragma unroll
-      for (int i = 0; i < FR; ++i) {
-        float v[8];
+      for (int s = 0; s < KB / 32; ++s) {       // the next k-step's fragments are read while this one's are multiplied
+        if (s + 1 < KB / 32) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][8 * p + t]), __float_as_uint(acc[i][j][8 * p + 4 + t]),
-                                                          false, false);
-          v[t] = __uint_as_float(x[0]);
-          v[t + 4] = __uint_as_float(x[1]);
+          for (int i = 0; i < FR; ++i) fr[(s + 1) & 1][i] = rr.get(at_r, i, s + 1);
+#pragma unroll
+          for (int j = 0; j < FC; ++j) fc[(s + 1) & 1][j] = rs.get(at_s, j, s + 1);
         }
-        const int rl = wr + 32 * i + (lane & 31);
-        if (rl >= nr || left <= 0) continue;
-        const int64_t row = row0 + rl;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FR; ++i)
+#pragma unroll
+          for (int j = 0; j < FC; ++j) Frag<T>::mma(fc[s & 1][j], fr[s & 1][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      use_r = use_r == Ring::kR - 1 ? 0 : use_r + 1;
+      use_s = use_s == Ring::kS - 1 ? 0 : use_s + 1;
+    }
+
+    // ---- epilogue, 32 rows of the wave's tile at a time through the stages just multiplied, which nothing fills before
+    // the next barrier.  A lane holds four consecutive columns of one row; 16-byte slot s of row r lies at
+    // s ^ (r mod slots), so that eight rows written at the same column fall on different banks.
+    constexpr int EP = 32 * WC * 4, R_WAVES = BR * KB / EP < WAVES ? BR * KB / EP : WAVES;
+    static_assert(R_WAVES + BC * KB / EP >= WAVES, "the epilogue fits the two stages");
+    char* const mine = wave < R_WAVES ? lds + (use_r == 0 ? Ring::kR - 1 : use_r - 1) * (BR * KB) + wave * EP
+                                      : ring_s + (use_s == 0 ? Ring::kS - 1 : use_s - 1) * (BC * KB) + (wave - R_WAVES) * EP;
+    const int c = lane % LPR, cl = wc + 8 * c;
+    const int64_t col = t.col0 + cl;
+    const int left = t.nc - cl < 8 ? t.nc - cl : 8;
+    const bool vec = a.cvec && left == 8;
+    float b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = 0.f;
+    if (KIND == kFwd && a.bias != nullptr && a.slab == nullptr && t.g >= 0) {
+      const T* bp = reinterpret_cast<const T*>(a.bias) + t.g * a.bias_group + col;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) b[e] = (float)bp[e];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wave is done reading the stages
+#pragma unroll
+    for (int i = 0; i < FR; ++i) {
+      if (wr + 32 * i >= t.nr) break;          // uniform over the wave
+#pragma unroll
+      for (int j = 0; j < FC; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = lane & 31, s = 8 * j + 2 * e + (lane >> 5);
+          *reinterpret_cast<f32x4*>(mine + r * (WC * 4) + ((s ^ (r & (SLOTS - 1))) << 4)) =
+              f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the wave reads only what it wrote itself
+#pragma unroll 1
+      for (int it = 0; it < 32 / RPI; ++it) {
+        const int r = it * RPI + lane / LPR, rl = wr + 32 * i + r;
+        if (rl >= t.nr || left <= 0) continue;
+        const int64_t row = t.row0 + rl;
+        const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + r * (WC * 4) + (((2 * c) ^ (r & (SLOTS - 1))) << 4));
+        const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + r * (WC * 4) + (((2 * c + 1) ^ (r & (SLOTS - 1))) << 4));
         if (a.slab != nullptr) {
-          float* out = a.slab + ((int64_t)z * a.rows + row) * a.cols + col;
+          float* out = a.slab + ((int64_t)t.z * a.rows + row) * a.cols + col;
           if (left == 8 && a.cols % 4 == 0) {
-            *reinterpret_cast<f32x4*>(out) = f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4*>(out + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            *reinterpret_cast<f32x4*>(out) = v0;
+            *reinterpret_cast<f32x4*>(out + 4) = v1;
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (e < left) out[e] = v[e];
+              if (e < left) out[e] = e < 4 ? v0[e] : v1[e - 4];
           }
           continue;
         }
-        T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? g * a.c_group : 0) + row * a.ldc + col;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = v0[e];
+          v[e + 4] = v1[e];
+        }
+        T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? t.g * a.c_group : 0) + row * a.ldc + col;
         if (KIND == kFwd) {
           typedef typename Deriv<T>::type DT;
-          constexpr bool FAST = sizeof(T) == 2;
-          float d[8], r[8];
+          float d[8], q[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) r[e] = d[e] = 0.f;
-          if (g >= 0) {
+          for (int e = 0; e < 8; ++e) q[e] = d[e] = 0.f;
+          if (t.g >= 0) {
             if (a.res != nullptr) {
               const T* rp = reinterpret_cast<const T*>(a.res) + row * a.ldres + col;
               if (vec) {
-                load_vec<T, 8>(rp, r);
+                load_vec<T, 8>(rp, q);
               } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  if (e < left) r[e] = (float)rp[e];
+                  if (e < left) q[e] = (float)rp[e];
               }
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += b[e];
-            activate<FAST, 8>(a.act, v, d);
+            activate<sizeof(T) == 2, 8>(a.act, v, d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += r[e];
+            for (int e = 0; e < 8; ++e) v[e] += q[e];
           }
           if (a.dact != nullptr) {
             DT* dp = reinterpret_cast<DT*>(a.dact) + row * a.lddact + col;
             if (vec) {
-              store_vec<DT, 8>(dp, d);
+              store_stream<DT, 8>(dp, d);
             } else {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
@@ -515,7 +632,7 @@ __global__ __launch_bounds__((BR / WR) * (BC / WC) * 64) void gemm_kernel(const 
           }
         }
         if (vec) {
-          store_vec<T, 8>(out, v);
+          store_stream<T, 8>(out, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -523,11 +640,14 @@ __global__ __launch_bounds__((BR / WR) * (BC / WC) * 64) void gemm_kernel(const 
         }
       }
     }
+    // a full tile in 16-byte pieces: the number of its stores is known
+    behind = a.cvec && a.slab == nullptr && t.nr == BR && t.nc == BC ? (KIND == kFwd && a.dact != nullptr ? 2 : 1) : 0;
   }
+  if constexpr (DIRECT) wait_loads<0>();         // the zeros behind the last tile: nothing may write into the next workgroup's LDS
 }
 
-int launch_gemm_f32(int kind, int tile, bool direct, const GemmArgs& a, int device, hipStream_t s);
-int launch_gemm_bf16(int kind, int tile, bool direct, const GemmArgs& a, int device, hipStream_t s);
-int launch_gemm_f16(int kind, int tile, bool direct, const GemmArgs& a, int device, hipStream_t s);
+int launch_gemm_f32(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
+int launch_gemm_bf16(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
+int launch_gemm_f16(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
 
 }  // namespace bnpvi

@@ -73,6 +73,20 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[E]) {
   *reinterpret_cast<vec*>(p) = q;
 }
 
+// the same past the caches' reuse order: results that are as large as the caches and written once
+template <typename T, int E>
+__device__ __forceinline__ void store_stream(T* p, const float (&v)[E]) {
+  typedef T vec __attribute__((ext_vector_type(E)));
+  union {
+    vec t;
+    u32x4 u[sizeof(vec) / 16];
+  } q;
+#pragma unroll
+  for (int e = 0; e < E; ++e) q.t[e] = (T)v[e];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(vec) / 16); ++i) __builtin_nontemporal_store(q.u[i], reinterpret_cast<u32x4*>(p) + i);
+}
+
 // The value another lane of the same 16 holds (data-parallel primitive `CTRL`); all lanes take part.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
