@@ -10,12 +10,14 @@
 // behind the descriptor's range and arrives as zeros).  The loader cannot pad, so conflicts are avoided by permuting
 // the pieces it fetches: KM piece c of row r sits at c ^ (r & 7); 16-bit MM 32-byte unit u of row k at u ^ (k mod
 // units).  Fragments: KM one 16-byte LDS read; 16-bit MM two transposing 8-byte reads; fp32 MM four 4-byte reads.
-// Operands whose rows do not start on 16 bytes take the same way through registers in narrower pieces.
+// Operands whose rows do not start on 16 bytes come through registers into the same places.
 //
 // Products: v_mfma_f32_32x32x16 (bf16, f16) and v_mfma_f32_32x32x2_f32, fp32 accumulation.  S is the first operand of
 // the instruction, so a lane ends with four consecutive columns of one row; the accumulators pass through LDS once
 // more so that the epilogue reads and writes whole 16-byte pieces of rows, eight lanes and more a row.
 #pragma once
+
+#include <type_traits>
 
 #include "layers_common.h"
 
@@ -51,7 +53,6 @@ struct GemmArgs {
   const int4* map;             // row tiles {group, first row, end row} (kFwd, kDx with groups) or nullptr
   int G, splits;
   int row_tiles, col_tiles;
-  int rv, sv;                  // elements per access of R and S where a row does not start on 16 bytes
   int cvec;                    // C, residual and derivative take 16-byte accesses
   void* C;
   int64_t ldc;
@@ -63,6 +64,8 @@ struct GemmArgs {
   int64_t lddact;
   int act;
   float* slab;                 // [group x split][rows][cols] partial sums, or nullptr
+  void* db;                    // kDw: [group][rows] sums of R over k, or nullptr
+  float* db_slab;              // the same per group x split (with `slab`)
 };
 
 // act(z) and act'(z).  16-bit results (FAST) take the hardware's exp2 and reciprocal (1 ulp each) and the normal
@@ -194,38 +197,32 @@ struct Source {
         buffer_to_lds(rs, lds + (q * THREADS + wave * 64) * 16, kt * kBK + (KM ? piece(q) * kPer : row(q)) < k ? off[q] : kOutside);
     }
   }
-  // the same through registers, V elements an access (V divides the pitch, the base and the contiguous extent)
-  template <int V>
+  // The same through registers, for rows that start anywhere: global loads take any address.  A piece that crosses the
+  // end of its row (KM) or of the columns (MM) is put together element by element.
   __device__ __forceinline__ void fetch(int kt, u32x4 (&reg)[kP]) const {
-    typedef T vec __attribute__((ext_vector_type(V)));
-    union {
-      u32x4 u;
-      vec v[kPer / V];
-    } x;
 #pragma unroll
     for (int q = 0; q < kP; ++q) {
-      x.u = u32x4{0, 0, 0, 0};
+      const int kk = kt * kBK + (KM ? piece(q) * kPer : row(q)), nn = KM ? row(q) : piece(q) * kPer;
+      const int inside = nn < n && kk < k ? (KM ? k - kk : n - nn) : 0;           // elements of this piece
+      const char* at = base + (KM ? (int64_t)nn * pitch + (int64_t)kk * sizeof(T) : (int64_t)kk * pitch + (int64_t)nn * sizeof(T));
+      reg[q] = u32x4{0, 0, 0, 0};
+      if (inside >= kPer) {
+        const u32x4_anywhere v = *reinterpret_cast<const u32x4_anywhere*>(at);
+        reg[q] = u32x4{v[0], v[1], v[2], v[3]};
+      } else if (inside > 0) {
 #pragma unroll
-      for (int e = 0; e < kPer / V; ++e) {
-        const int kk = kt * kBK + (KM ? piece(q) * kPer + e * V : row(q));
-        const int nn = KM ? row(q) : piece(q) * kPer + e * V;
-        if (kk < k && nn < n) {
-          const int64_t r = KM ? row(q) : kk, c = KM ? kk : nn;
-          x.v[e] = *reinterpret_cast<const vec*>(base + r * pitch + c * (int64_t)sizeof(T));
+        for (int w = 0; w < 4; ++w) {
+          uint32_t v = 0;
+          if (sizeof(T) == 4) {
+            if (w < inside) v = reinterpret_cast<const uint32_t*>(at)[w];
+          } else {
+            if (2 * w < inside) v = reinterpret_cast<const uint16_t*>(at)[2 * w];
+            if (2 * w + 1 < inside) v |= (uint32_t)reinterpret_cast<const uint16_t*>(at)[2 * w + 1] << 16;
+          }
+          reg[q][w] = v;
         }
       }
-      reg[q] = x.u;
     }
-  }
-  __device__ __forceinline__ void fetch_any(int v, int kt, u32x4 (&reg)[kP]) const {
-    if (v >= kPer)
-      fetch<kPer>(kt, reg);
-    else if (v >= kPer / 2)
-      fetch<kPer / 2>(kt, reg);
-    else if (v >= 2)
-      fetch<2>(kt, reg);
-    else
-      fetch<1>(kt, reg);
   }
   __device__ __forceinline__ void put(char* lds, const u32x4 (&reg)[kP]) const {
 #pragma unroll
@@ -239,16 +236,25 @@ struct Frag;
 template <>
 struct Frag<float> {
   typedef f32x4 type;
-  static __device__ __forceinline__ void mma(const f32x4& a, const f32x4& b, f32x16& c) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+  static constexpr int kSteps = 4;
+  static __device__ __forceinline__ void mma(const f32x4& a, const f32x4& b, f32x16& c, int t) {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float sum(const f32x4& a, float c) { return c + ((a[0] + a[1]) + (a[2] + a[3])); }
 };
 template <>
 struct Frag<bf16_t> {
   typedef bf16x8 type;
-  static __device__ __forceinline__ void mma(const bf16x8& a, const bf16x8& b, f32x16& c) {
+  static constexpr int kSteps = 1;
+  static __device__ __forceinline__ void mma(const bf16x8& a, const bf16x8& b, f32x16& c, int) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float sum(const bf16x8& a, float c) {
+    typedef bf16_t two __attribute__((ext_vector_type(2)));
+    const two one = {(bf16_t)1.f, (bf16_t)1.f};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_fdot2_f32_bf16(two{a[2 * t], a[2 * t + 1]}, one, c, false);
+    return c;
   }
   static __device__ __forceinline__ bf16x8 transposed(const char* p0, const char* p1) {
     typedef __attribute__((address_space(3))) bf16x4* at;
@@ -259,8 +265,16 @@ struct Frag<bf16_t> {
 template <>
 struct Frag<f16_t> {
   typedef f16x8v type;
-  static __device__ __forceinline__ void mma(const f16x8v& a, const f16x8v& b, f32x16& c) {
+  static constexpr int kSteps = 1;
+  static __device__ __forceinline__ void mma(const f16x8v& a, const f16x8v& b, f32x16& c, int) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float sum(const f16x8v& a, float c) {
+    typedef f16_t two __attribute__((ext_vector_type(2)));
+    const two one = {(f16_t)1.f, (f16_t)1.f};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_fdot2(two{a[2 * t], a[2 * t + 1]}, one, c, false);
+    return c;
   }
   static __device__ __forceinline__ f16x8v transposed(const char* p0, const char* p1) {
     typedef __attribute__((address_space(3))) f16x4s* at;
@@ -329,6 +343,10 @@ struct Rings {
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// the dW kernel can add up the rows of R for the bias, but not where its accumulators already fill the registers
+template <int KIND, int BR>
+constexpr bool kRowSums = KIND == kDw && BR < 256;
 
 // One output tile: its place in C, its group, its part of the sum.
 struct Tile {
@@ -453,7 +471,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
       sr.src.to_lds(sr.kt, lds + fill_r * (BR * KB));
       fill_r = fill_r == Ring::kR - 1 ? 0 : fill_r + 1;
     } else {
-      sr.src.fetch_any(a.rv, sr.kt, hr);
+      sr.src.fetch(sr.kt, hr);
     }
     sr.step_on(a);
   };
@@ -462,7 +480,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
       ss.src.to_lds(ss.kt, ring_s + fill_s * (BC * KB));
       fill_s = fill_s == Ring::kS - 1 ? 0 : fill_s + 1;
     } else {
-      ss.src.fetch_any(a.sv, ss.kt, hs);
+      ss.src.fetch(ss.kt, hs);
     }
     ss.step_on(a);
   };
@@ -490,7 +508,13 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
       for (int j = 0; j < FC; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    // the bias gradient where dz is dy: row sums of R, by the waves that hold the first columns
+    const bool row_sums = kRowSums<KIND, BR> && (a.db != nullptr || a.db_slab != nullptr) && t.col0 == 0 && wc == 0;
+    float rsum[FR];
+#pragma unroll
+    for (int i = 0; i < FR; ++i) rsum[i] = 0.f;
     const int nk = t.stages(BK);
+    auto add_up = [&](auto with_sums) {
     for (int kt = 0; kt < nk; ++kt) {
       char* const at_r = lds + use_r * (BR * KB);
       char* const at_s = ring_s + use_s * (BC * KB);
@@ -530,13 +554,41 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < FR; ++i)
+        for (int u = 0; u < Frag<T>::kSteps; ++u)
 #pragma unroll
-          for (int j = 0; j < FC; ++j) Frag<T>::mma(fc[s & 1][j], fr[s & 1][i], acc[i][j]);
+          for (int i = 0; i < FR; ++i)
+#pragma unroll
+            for (int j = 0; j < FC; ++j) Frag<T>::mma(fc[s & 1][j], fr[s & 1][i], acc[i][j], u);
+        if constexpr (decltype(with_sums)::value) {
+#pragma unroll
+          for (int i = 0; i < FR; ++i) rsum[i] = Frag<T>::sum(fr[s & 1][i], rsum[i]);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       use_r = use_r == Ring::kR - 1 ? 0 : use_r + 1;
       use_s = use_s == Ring::kS - 1 ? 0 : use_s + 1;
+    }
+    };
+    if constexpr (kRowSums<KIND, BR>) {
+      if (row_sums)
+        add_up(std::true_type());
+      else
+        add_up(std::false_type());
+    } else {
+      add_up(std::false_type());
+    }
+    if (kRowSums<KIND, BR> && row_sums) {
+#pragma unroll
+      for (int i = 0; i < FR; ++i) {
+        const float sum = rsum[i] + __shfl_xor(rsum[i], 32);
+        const int rl = wr + 32 * i + lane;
+        if (lane < 32 && rl < t.nr) {
+          if (a.db_slab != nullptr)
+            a.db_slab[(int64_t)t.z * a.rows + t.row0 + rl] = sum;
+          else
+            reinterpret_cast<T*>(a.db)[(int64_t)t.g * a.rows + t.row0 + rl] = (T)sum;
+        }
+      }
     }
 
     // ---- epilogue, 32 rows of the wave's tile at a time through the stages just multiplied, which nothing fills before

@@ -17,6 +17,7 @@ typedef _Float16 f16_t;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_anywhere __attribute__((ext_vector_type(4), aligned(2)));      // global loads take any address
 
 inline int dtype_bytes(int dtype) { return dtype == BNPVI_F32 ? 4 : dtype == BNPVI_BF16 || dtype == BNPVI_F16 ? 2 : 0; }
 

@@ -98,45 +98,59 @@ __global__ __launch_bounds__(256) void top_leaves_kernel(const float* __restrict
   }
 }
 
-template <int LPR, int VEC>
+// The gradient writes every column of every row: bound by those stores, which pass the caches, and by the wait for the
+// few values of a row in front of them, so a lane takes R rows at once.
+template <int K, int LPR, int VEC>
 __global__ __launch_bounds__(256) void top_leaves_bwd_kernel(const int32_t* __restrict__ leaf, const float* __restrict__ weight,
                                                              const float* __restrict__ total, const float* __restrict__ dweight,
-                                                             int64_t N, int L, int k, int renorm, float* __restrict__ dphi,
-                                                             int64_t ld, int cols) {
-  constexpr int RPB = 256 / LPR;
+                                                             int64_t N, int k, int renorm, float* __restrict__ dphi, int64_t ld,
+                                                             int cols) {
+  constexpr int RPB = 256 / LPR, R = K <= 2 ? 4 : K <= 4 ? 2 : 1;
   const int sub = threadIdx.x % LPR, r = threadIdx.x / LPR;
-  for (int64_t n = (int64_t)blockIdx.x * RPB + r; n < N; n += (int64_t)gridDim.x * RPB) {
-    int at[kTopMax];
-    float g[kTopMax];
-    double dot = 0.0;
+  for (int64_t n0 = (int64_t)blockIdx.x * RPB * R + r; n0 < N; n0 += (int64_t)gridDim.x * RPB * R) {
+    int at[R][K];
+    float g[R][K], w[R][K], s[R];
 #pragma unroll
-    for (int j = 0; j < kTopMax; ++j) {
-      at[j] = -1;
-      g[j] = 0.f;
-      if (j < k) {
-        at[j] = leaf[n * k + j];
-        g[j] = dweight[n * k + j];
-        if (renorm && at[j] >= 0) dot += (double)g[j] * (double)weight[n * k + j];
+    for (int i = 0; i < R; ++i) {
+      const int64_t n = n0 + i * RPB;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        const bool on = j < k && n < N;
+        at[i][j] = on ? leaf[n * k + j] : -1;
+        g[i][j] = on ? dweight[n * k + j] : 0.f;
+        w[i][j] = on && renorm ? weight[n * k + j] : 0.f;
       }
+      s[i] = renorm && n < N ? total[n] : 0.f;
     }
-    if (renorm) {
-      const float s = total[n];
 #pragma unroll
-      for (int j = 0; j < kTopMax; ++j) g[j] = s > 0.f ? (float)(((double)g[j] - dot) / (double)s) : 0.f;
-    }
-    float* row = dphi + n * ld;
-    for (int c = sub * VEC; c < cols; c += LPR * VEC) {
-      f32x4 q = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < R; ++i) {
+      const int64_t n = n0 + i * RPB;
+      if (n >= N) break;
+      if (renorm) {
+        float dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < kTopMax; ++j) {
+        for (int j = 0; j < K; ++j) dot = at[i][j] >= 0 ? fmaf(g[i][j], w[i][j], dot) : dot;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (at[j] == c + e) q[e] = g[j];
+        for (int j = 0; j < K; ++j) g[i][j] = s[i] > 0.f ? (g[i][j] - dot) / s[i] : 0.f;
       }
-      if (VEC == 4)
-        *reinterpret_cast<f32x4*>(row + c) = q;
-      else
-        row[c] = q[0];
+      float* row = dphi + n * ld;
+      for (int c = sub * VEC; c < cols; c += LPR * VEC) {
+        f32x4 q = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          const int e = at[i][j] - c;          // leaves differ, so at most one lands on each column
+          q[0] = e == 0 ? g[i][j] : q[0];
+          if (VEC == 4) {
+            q[1] = e == 1 ? g[i][j] : q[1];
+            q[2] = e == 2 ? g[i][j] : q[2];
+            q[3] = e == 3 ? g[i][j] : q[3];
+          }
+        }
+        if (VEC == 4)
+          __builtin_nontemporal_store(q, reinterpret_cast<f32x4*>(row + c));
+        else
+          row[c] = q[0];
+      }
     }
   }
 }
@@ -149,7 +163,7 @@ __global__ __launch_bounds__(256) void top_leaves_bwd_kernel(const int32_t* __re
 // another's row, so nothing is added atomically and the result is the stable order itself.
 __device__ __forceinline__ int bin_of(int32_t l, int L) { return (uint32_t)l < (uint32_t)L ? l : L; }
 
-__global__ __launch_bounds__(256) void leaf_count_kernel(const int32_t* __restrict__ leaf, int64_t M, int L, int64_t chunk,
+__global__ __launch_bounds__(1024) void leaf_count_kernel(const int32_t* __restrict__ leaf, int64_t M, int L, int64_t chunk,
                                                          int32_t* __restrict__ hist) {
   extern __shared__ int32_t cnt[];
   const int B = L + 1;
@@ -161,22 +175,35 @@ __global__ __launch_bounds__(256) void leaf_count_kernel(const int32_t* __restri
   for (int i = threadIdx.x; i < B; i += blockDim.x) hist[(int64_t)blockIdx.x * B + i] = cnt[i];
 }
 
-// hist[b][bin] -> slots of that bin in the chunks before b; totals[bin] = slots of that bin.  64 bins a workgroup, 16
-// waves that share the chunks.
-__global__ __launch_bounds__(1024) void leaf_scan_kernel(int32_t* __restrict__ hist, int nb, int B, int32_t* __restrict__ totals) {
+// hist[b][bin] -> slots of that bin in the chunks before b; start[bin] = slots of the lower bins of its 64, sums[i] =
+// slots of the i-th 64 bins.  64 bins a workgroup, 16 waves that share the chunks.
+__global__ __launch_bounds__(1024) void leaf_scan_kernel(int32_t* __restrict__ hist, int nb, int B, int32_t* __restrict__ start,
+                                                         int32_t* __restrict__ sums) {
   __shared__ int32_t part[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int bin = blockIdx.x * 64 + lane;
   const int per = (nb + 15) / 16, b0 = min(nb, w * per), b1 = min(nb, b0 + per);
   int32_t sum = 0;
-  if (bin < B)
+  if (bin < B) {
+#pragma unroll 8
     for (int b = b0; b < b1; ++b) sum += hist[(int64_t)b * B + bin];
+  }
   part[w][lane] = sum;
   __syncthreads();
   int32_t run = 0;
   for (int i = 0; i < w; ++i) run += part[i][lane];
+  if (w == 15) {
+    const int32_t all = run + sum;
+    int32_t inc = all;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int32_t o = __shfl_up(inc, d);
+      if (lane >= d) inc += o;
+    }
+    if (bin < B) start[bin] = inc - all;
+    if (lane == 63) sums[blockIdx.x] = inc;
+  }
   if (bin < B) {
-    if (w == 15) totals[bin] = run + sum;
+#pragma unroll 8
     for (int b = b0; b < b1; ++b) {
       const int32_t h = hist[(int64_t)b * B + bin];
       hist[(int64_t)b * B + bin] = run;
@@ -185,12 +212,12 @@ __global__ __launch_bounds__(1024) void leaf_scan_kernel(int32_t* __restrict__ h
   }
 }
 
-// exclusive scan of src[0 .. B) into dst (LDS), whole workgroup; red: one int per wave
-__device__ void scan_bins(const int32_t* src, int32_t* dst, int B, int32_t* red) {
-  const int T = blockDim.x, t = threadIdx.x, lane = t & 63, w = t >> 6, W = T >> 6;
-  const int per = (B + T - 1) / T, i0 = min(B, t * per), i1 = min(B, i0 + per);
+// Exclusive scan of a[0 .. n) in LDS by the whole workgroup; red: one int per wave.
+__device__ void scan_in_lds(int32_t* a, int n, int32_t* red) {
+  const int T = blockDim.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int per = (n + T - 1) / T, i0 = min(n, t * per), i1 = min(n, i0 + per);
   int32_t sum = 0;
-  for (int i = i0; i < i1; ++i) sum += src[i];
+  for (int i = i0; i < i1; ++i) sum += a[i];
   int32_t inc = sum;
   for (int d = 1; d < 64; d <<= 1) {
     const int32_t o = __shfl_up(inc, d);
@@ -199,46 +226,52 @@ __device__ void scan_bins(const int32_t* src, int32_t* dst, int B, int32_t* red)
   if (lane == 63) red[w] = inc;
   __syncthreads();
   int32_t run = inc - sum;
-  for (int i = 0; i < w && i < W; ++i) run += red[i];
+  for (int i = 0; i < w; ++i) run += red[i];
   for (int i = i0; i < i1; ++i) {
-    const int32_t v = src[i];               // src may be dst: each thread reads an entry before it writes it
-    dst[i] = run;
+    const int32_t v = a[i];
+    a[i] = run;
     run += v;
   }
   __syncthreads();
 }
 
-// LDS: base[W][B] | red[W].  One workgroup (hist == nullptr) does the whole sort: counts, scan, places.
+// LDS: base[W][B] | sums[max(B, bins of 64)] | red[16].  The first W waves place, all of them do the work over the bins.
+// One workgroup (hist == nullptr) does the whole sort: counts, scan, places.
 __global__ __launch_bounds__(1024) void leaf_place_kernel(const int32_t* __restrict__ leaf, int64_t M, int L, int64_t chunk, int bits,
-                                                          const int32_t* __restrict__ hist, const int32_t* __restrict__ totals,
-                                                          int32_t* __restrict__ place, int32_t* __restrict__ order,
-                                                          int32_t* __restrict__ offsets) {
+                                                          int W, const int32_t* __restrict__ hist, const int32_t* __restrict__ start,
+                                                          const int32_t* __restrict__ sums, int32_t* __restrict__ place,
+                                                          int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
   extern __shared__ int32_t lds[];
-  const int B = L + 1, W = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int B = L + 1, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int nsum = (B + 63) / 64;
   int32_t* mine = lds + (size_t)w * B;
-  int32_t* start = lds + (size_t)W * B;              // [B] first place of each bin
-  int32_t* red = start + B;
+  int32_t* firsts = lds + (size_t)W * B;               // of the bins (one workgroup) or of each 64 bins
+  int32_t* red = firsts + (hist != nullptr ? nsum : B);
   const int64_t lo = (int64_t)blockIdx.x * chunk, hi = min(M, lo + chunk);
   const int64_t per = ((hi - lo + W - 1) / W + 63) / 64 * 64;
-  const int64_t s0 = min(hi, lo + w * per), s1 = min(hi, s0 + per);
+  const int64_t s0 = w < W ? min(hi, lo + w * per) : hi, s1 = min(hi, s0 + per);
   for (int i = threadIdx.x; i < W * B; i += blockDim.x) lds[i] = 0;
+  if (hist != nullptr)
+    for (int i = threadIdx.x; i < nsum; i += blockDim.x) firsts[i] = sums[i];
   __syncthreads();
   for (int64_t s = s0 + lane; s < s1; s += 64) atomicAdd(&mine[bin_of(leaf[s], L)], 1);
   __syncthreads();
   if (hist != nullptr) {
-    scan_bins(totals, start, B, red);
+    scan_in_lds(firsts, nsum, red);
   } else {
     for (int i = threadIdx.x; i < B; i += blockDim.x) {
       int32_t sum = 0;
       for (int v = 0; v < W; ++v) sum += lds[(size_t)v * B + i];
-      start[i] = sum;
+      firsts[i] = sum;
     }
     __syncthreads();
-    scan_bins(start, start, B, red);
+    scan_in_lds(firsts, B, red);
   }
+#pragma unroll 2
   for (int i = threadIdx.x; i < B; i += blockDim.x) {
-    if (blockIdx.x == 0) offsets[i] = start[i];      // offsets[L] = slots with a leaf = first place without one
-    int32_t run = start[i] + (hist != nullptr ? hist[(int64_t)blockIdx.x * B + i] : 0);
+    const int32_t at = hist != nullptr ? firsts[i >> 6] + start[i] : firsts[i];
+    if (blockIdx.x == 0) offsets[i] = at;            // offsets[L] = slots with a leaf = first place without one
+    int32_t run = at + (hist != nullptr ? hist[(int64_t)blockIdx.x * B + i] : 0);
     for (int v = 0; v < W; ++v) {
       const int32_t c = lds[(size_t)v * B + i];
       lds[(size_t)v * B + i] = run;
@@ -302,14 +335,22 @@ __global__ __launch_bounds__(256) void rows_from_leaves_kernel(const T* __restri
       float acc[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
-      for (int j = 0; j < k; ++j) {
-        const int32_t p = place[n * k + j];
-        if ((uint32_t)p >= (uint32_t)kept) continue;
-        const float w = weight != nullptr ? weight[n * k + j] : 1.f;
-        float v[E];
-        load_vec<T, E>(ys + (int64_t)p * ldys + c, v);
+      for (int j0 = 0; j0 < k; j0 += 4) {          // four rows under way at once, added in order
+        float v[4][E], w[4];
+        bool in[4];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+        for (int j = 0; j < 4; ++j) {
+          const int32_t p = j0 + j < k ? place[n * k + j0 + j] : -1;
+          in[j] = (uint32_t)p < (uint32_t)kept;
+          w[j] = in[j] ? (weight != nullptr ? weight[n * k + j0 + j] : 1.f) : 0.f;
+          if (in[j]) load_vec<T, E>(ys + (int64_t)p * ldys + c, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (in[j]) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(w[j], v[j][e], acc[e]);
+          }
       }
       store_vec<T, E>(y + n * ldy + c, acc);
     }
@@ -376,6 +417,19 @@ static void launch_top(const bnpvi_ctx* ctx, const float* phi, int64_t ld, int64
     top_leaves_kernel<4, LPR, VEC><<<g, 256, 0, s>>>(phi, ld, N, L, k, renorm, leaf, weight, total);
   else
     top_leaves_kernel<8, LPR, VEC><<<g, 256, 0, s>>>(phi, ld, N, L, k, renorm, leaf, weight, total);
+}
+
+template <int K>
+static void launch_top_bwd(const bnpvi_ctx* ctx, const int32_t* leaf, const float* weight, const float* total, const float* dweight,
+                           int64_t N, int k, int renorm, float* dphi, int64_t ld, int cols, bool vec, hipStream_t s) {
+  if (vec && cols <= 32)
+    top_leaves_bwd_kernel<K, 8, 4><<<grid_for(ctx, ceil_div(N, 32)), 256, 0, s>>>(leaf, weight, total, dweight, N, k, renorm, dphi, ld, cols);
+  else if (vec && cols <= 128)
+    top_leaves_bwd_kernel<K, 16, 4><<<grid_for(ctx, ceil_div(N, 16)), 256, 0, s>>>(leaf, weight, total, dweight, N, k, renorm, dphi, ld, cols);
+  else if (vec)
+    top_leaves_bwd_kernel<K, 64, 4><<<grid_for(ctx, ceil_div(N, 4)), 256, 0, s>>>(leaf, weight, total, dweight, N, k, renorm, dphi, ld, cols);
+  else
+    top_leaves_bwd_kernel<K, 64, 1><<<grid_for(ctx, ceil_div(N, 4)), 256, 0, s>>>(leaf, weight, total, dweight, N, k, renorm, dphi, ld, cols);
 }
 
 // the widest access (16, 8, 4 or 2 bytes) at which every row of both arrays starts and a row's bytes divide
@@ -447,7 +501,7 @@ int bnpvi_top_leaves(bnpvi_ctx* ctx, const float* phi, int64_t ldphi, int64_t N,
   if (vec) {
     if (L <= 32)
       launch_top<8, 4>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
-    else if (L <= 128)
+    else if (L <= 1024)      // four rows a wave: the rounds cost the same for one row or four (150k x 512, k = 4: 99 us one row a wave)
       launch_top<16, 4>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
     else
       launch_top<64, 4>(ctx, phi, ldphi, N, L, k, renormalize, leaf, weight, total, s);
@@ -473,60 +527,60 @@ int bnpvi_top_leaves_backward(bnpvi_ctx* ctx, const int32_t* leaf, const float* 
   BNPVI_HIP(on.status());
   hipStream_t s = (hipStream_t)stream;
   const bool vec = lddphi % 4 == 0 && cols % 4 == 0 && ((uintptr_t)dphi & 15) == 0;
-  if (vec) {
-    if (cols <= 32)
-      top_leaves_bwd_kernel<8, 4><<<grid_for(ctx, ceil_div(N, 32)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
-                                                                                  dphi, lddphi, cols);
-    else if (cols <= 128)
-      top_leaves_bwd_kernel<16, 4><<<grid_for(ctx, ceil_div(N, 16)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
-                                                                                   dphi, lddphi, cols);
-    else
-      top_leaves_bwd_kernel<64, 4><<<grid_for(ctx, ceil_div(N, 4)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
-                                                                                  dphi, lddphi, cols);
-  } else {
-    top_leaves_bwd_kernel<64, 1><<<grid_for(ctx, ceil_div(N, 4)), 256, 0, s>>>(leaf, weight, total, dweight, N, L, k, renormalize,
-                                                                                dphi, lddphi, cols);
-  }
+  if (k == 1)
+    launch_top_bwd<1>(ctx, leaf, weight, total, dweight, N, k, renormalize, dphi, lddphi, cols, vec, s);
+  else if (k == 2)
+    launch_top_bwd<2>(ctx, leaf, weight, total, dweight, N, k, renormalize, dphi, lddphi, cols, vec, s);
+  else if (k <= 4)
+    launch_top_bwd<4>(ctx, leaf, weight, total, dweight, N, k, renormalize, dphi, lddphi, cols, vec, s);
+  else
+    launch_top_bwd<8>(ctx, leaf, weight, total, dweight, N, k, renormalize, dphi, lddphi, cols, vec, s);
   BNPVI_LAUNCH_CHECK();
   return BNPVI_OK;
 }
 
 // ---- sort: sizes of one call ---------------------------------------------------------------------------------------
 struct SortPlan {
-  int waves, bits, nb;
+  int waves, threads, bits, nb;
   int64_t chunk;
   size_t lds;
 };
 
 static SortPlan sort_plan(int64_t M, int L) {
   SortPlan p;
-  const int B = L + 1;
+  const int B = L + 1, nsum = (B + 63) / 64;
   p.bits = 1;
   while ((int64_t(1) << p.bits) < B) ++p.bits;
-  // the counters of all waves and one row of bin starts share the LDS
-  p.waves = (size_t)5 * B * 4 + 64 <= (size_t)kMaxLdsBytes ? 4 : 1;
-  if (M <= 8192 && (size_t)17 * B * 4 + 128 <= (size_t)kMaxLdsBytes) {
+  if (M <= 8192 && (size_t)17 * B * 4 + 64 <= (size_t)kMaxLdsBytes) {
     p.nb = 1;                                // a minibatch: one workgroup, one launch
     p.waves = M <= 1024 ? 4 : 16;
+    p.threads = p.waves * 64;
     p.chunk = M < 1 ? 1 : M;
-  } else {
-    // a chunk at least as long as its row of counters (they are written and read once each), at most 1024 chunks
-    int64_t c = B > 2048 ? B : 2048;
-    if (ceil_div(M, c) > 1024) c = ceil_div(M, 1024);
-    p.chunk = (c + 255) / 256 * 256;
-    p.nb = (int)ceil_div(M, p.chunk);
-    if (p.nb < 1) p.nb = 1;
+    p.lds = ((size_t)(p.waves + 1) * B + 16) * 4;
+    return p;
   }
-  p.lds = ((size_t)(p.waves + 1) * B + p.waves) * 4;
+  // The counters of all placing waves have to fit the LDS.  Work over many bins is shared by 16 waves.
+  p.waves = (size_t)(4 * B + nsum + 16) * 4 <= (size_t)kMaxLdsBytes ? 4 : 2;
+  p.threads = B > 1024 ? 1024 : 256;
+  // chunks of 2048 slots, longer where that makes more than 1024 of them, or -- where a chunk's counters outweigh its
+  // slots -- more than one a CU (900k slots, 7776 leaves: 89 us with chunks of 7936, one for 43 % of the CUs)
+  int64_t c = 2048;
+  const int64_t most = B > 2048 ? 256 : 1024;
+  if (ceil_div(M, c) > most) c = ceil_div(M, most);
+  p.chunk = (c + 255) / 256 * 256;
+  p.nb = (int)std::max<int64_t>(1, ceil_div(M, p.chunk));
+  p.lds = ((size_t)p.waves * B + nsum + 16) * 4;
   return p;
 }
+
+static bool one_launch(const SortPlan& p, int64_t M) { return p.nb == 1 && p.chunk == (M < 1 ? 1 : M); }
 
 int bnpvi_leaf_sort_max_leaves(void) { return kSortMaxLeaves; }
 
 int64_t bnpvi_leaf_sort_workspace(int64_t M, int L) {
   if (M < 0 || M > INT32_MAX || L < 1 || L > kSortMaxLeaves) return -1;
   const SortPlan p = sort_plan(M, L);
-  return p.nb == 1 && M <= 8192 ? 0 : (int64_t)(p.nb + 1) * (L + 1) * 4;
+  return M <= 8192 && one_launch(p, M) ? 0 : ((int64_t)(p.nb + 1) * (L + 1) + (L + 64) / 64) * 4;
 }
 
 int bnpvi_leaf_sort(bnpvi_ctx* ctx, const int32_t* leaf, int64_t M, int L, int32_t* place, int32_t* order, int32_t* offsets,
@@ -546,14 +600,15 @@ int bnpvi_leaf_sort(bnpvi_ctx* ctx, const int32_t* leaf, int64_t M, int L, int32
   static LdsLimit place_limit, count_limit;
   BNPVI_HIP(place_limit.raise((const void*)leaf_place_kernel, ctx->device));
   if (need == 0) {
-    leaf_place_kernel<<<1, p.waves * 64, p.lds, s>>>(leaf, M, L, p.chunk, p.bits, nullptr, nullptr, place, order, offsets);
+    leaf_place_kernel<<<1, p.threads, p.lds, s>>>(leaf, M, L, p.chunk, p.bits, p.waves, nullptr, nullptr, nullptr, place, order, offsets);
   } else {
     BNPVI_HIP(count_limit.raise((const void*)leaf_count_kernel, ctx->device));
     int32_t* hist = (int32_t*)work;
-    int32_t* totals = hist + (size_t)p.nb * B;
-    leaf_count_kernel<<<p.nb, 256, (size_t)B * 4, s>>>(leaf, M, L, p.chunk, hist);
-    leaf_scan_kernel<<<(B + 63) / 64, 1024, 0, s>>>(hist, p.nb, B, totals);
-    leaf_place_kernel<<<p.nb, p.waves * 64, p.lds, s>>>(leaf, M, L, p.chunk, p.bits, hist, totals, place, order, offsets);
+    int32_t* start = hist + (size_t)p.nb * B;
+    int32_t* sums = start + B;
+    leaf_count_kernel<<<p.nb, p.threads, (size_t)B * 4, s>>>(leaf, M, L, p.chunk, hist);
+    leaf_scan_kernel<<<(B + 63) / 64, 1024, 0, s>>>(hist, p.nb, B, start, sums);
+    leaf_place_kernel<<<p.nb, p.threads, p.lds, s>>>(leaf, M, L, p.chunk, p.bits, p.waves, hist, start, sums, place, order, offsets);
   }
   BNPVI_LAUNCH_CHECK();
   return BNPVI_OK;

@@ -48,8 +48,15 @@ def _ctx(device):
     return c
 
 
+try:                                                  # the handle alone: a Stream object costs 2 us a call
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
 
 
 def _on_gpu(what, **tensors):
