@@ -10,36 +10,45 @@ namespace bnpvi {
 // groups' tile counts, then every tile finds its group by bisection.
 __device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-__global__ __launch_bounds__(1024) void row_tiles_kernel(const int32_t* __restrict__ offsets, int G, int64_t M, int tile, int64_t ntiles,
-                                                         int4* __restrict__ map, int32_t* __restrict__ first) {
-  extern __shared__ int32_t start[];        // [G + 1] | [16]
-  int32_t* red = start + G + 1;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int per = (G + 1023) / 1024, g0 = min(G, t * per), g1 = min(G, g0 + per);
-  int32_t sum = 0;
-  for (int g = g0; g < g1; ++g) {
-    const int64_t lo = clamp_row(offsets[g], 0, M), hi = clamp_row(offsets[g + 1], lo, M);
-    sum += (int32_t)((hi - lo + tile - 1) / tile);
-  }
-  int32_t inc = sum;
+// Exclusive scan of one value per thread over the workgroup of 1024; the sum of all in `total`.
+__device__ int32_t scan_threads(int32_t v, int32_t* red, int32_t& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int32_t inc = v;
   for (int d = 1; d < 64; d <<= 1) {
     const int32_t o = __shfl_up(inc, d);
     if (lane >= d) inc += o;
   }
   if (lane == 63) red[w] = inc;
   __syncthreads();
-  int32_t run = inc - sum;
-  for (int i = 0; i < w; ++i) run += red[i];
+  int32_t run = inc - v;
+  total = 0;
+  for (int i = 0; i < 16; ++i) {
+    if (i < w) run += red[i];
+    total += red[i];
+  }
+  __syncthreads();
+  return run;
+}
+
+__device__ void row_tiles(const int32_t* __restrict__ offsets, int G, int64_t M, int tile, int64_t ntiles, int4* __restrict__ map,
+                          int32_t* __restrict__ first, int32_t* start, int32_t* red) {
+  const int t = threadIdx.x;
+  const int per = (G + 1023) / 1024, g0 = min(G, t * per), g1 = min(G, g0 + per);
+  int32_t sum = 0, used;
+  for (int g = g0; g < g1; ++g) {
+    const int64_t lo = clamp_row(offsets[g], 0, M), hi = clamp_row(offsets[g + 1], lo, M);
+    sum += (int32_t)((hi - lo + tile - 1) / tile);
+  }
+  int32_t run = scan_threads(sum, red, used);
   for (int g = g0; g < g1; ++g) {
     const int64_t lo = clamp_row(offsets[g], 0, M), hi = clamp_row(offsets[g + 1], lo, M);
     start[g] = run;
     run += (int32_t)((hi - lo + tile - 1) / tile);
   }
-  if (g1 == G && g0 < g1) start[G] = run;
+  if (t == 0) start[G] = used;
   __syncthreads();
   if (first != nullptr)
     for (int g = t; g <= G; g += 1024) first[g] = start[g];
-  const int32_t used = start[G];
   const int64_t head = clamp_row(offsets[0], 0, M), tail = clamp_row(offsets[G], 0, M);
   const int64_t nhead = (head + tile - 1) / tile;
   for (int64_t i = t; i < ntiles; i += 1024) {
@@ -69,6 +78,98 @@ __global__ __launch_bounds__(1024) void row_tiles_kernel(const int32_t* __restri
       }
     }
     map[i] = m;
+  }
+}
+
+// ---- pieces of the groups' sums (dW) ---------------------------------------------------------------------------------
+// Groups differ in length, and dW's tiles all have their group's: a group of more than `piece` frames is summed in pieces,
+// whose partial results lie in `part`s of their own and are added in order afterwards.  map[e] = {group, first frame, end
+// frame, part or -1}: the full pieces first, then the rest by quarters of a piece's length, so that the long ones start
+// first and every eighth entry -- one XCD's share -- is a like mixture.  sums[i] = {group, first part, parts} of the groups
+// in pieces; count = {entries, groups in pieces}.
+__device__ void sum_pieces(const int32_t* __restrict__ offsets, int G, int64_t M, int64_t piece, int entries, int most, int4* __restrict__ map,
+                           int4* __restrict__ sums, int32_t* __restrict__ count, int32_t* red) {
+  const int t = threadIdx.x;
+  const int per = (G + 1023) / 1024, g0 = min(G, t * per), g1 = min(G, g0 + per);
+  int32_t full = 0, parts = 0, split = 0, rest[4] = {0, 0, 0, 0};
+  auto look = [&](int g, int64_t& lo, int32_t& n, int64_t& left, int& quarter, bool& tail) {
+    lo = clamp_row(offsets[g], 0, M);
+    const int64_t len = clamp_row(offsets[g + 1], lo, M) - lo;
+    n = (int32_t)(len / piece);
+    left = len - n * piece;
+    tail = left > 0 || len == 0;
+    quarter = 3 - (int)(4 * left / piece);
+  };
+  int64_t lo, left;
+  int32_t n;
+  int quarter;
+  bool tail;
+  for (int g = g0; g < g1; ++g) {
+    look(g, lo, n, left, quarter, tail);
+    full += n;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rest[q] += tail && quarter == q;
+    if (n + tail > 1) {
+      parts += n + tail;
+      ++split;
+    }
+  }
+  int32_t all, at_full = scan_threads(full, red, all), base = all, at_rest[4], unused;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    at_rest[q] = base + scan_threads(rest[q], red, all);
+    base += all;
+  }
+  int32_t at_part = scan_threads(parts, red, unused), at_split = scan_threads(split, red, all);
+  if (t == 0) {
+    count[0] = base < entries ? base : entries;
+    count[1] = all < most ? all : most;
+  }
+  for (int g = g0; g < g1; ++g) {
+    look(g, lo, n, left, quarter, tail);
+    // the bounds hold wherever the offsets ascend; others are not followed out of the workspace
+    const bool many = n + tail > 1 && (uint32_t)at_part < (uint32_t)(2 * most) && n + tail <= 2 * most - at_part;
+    for (int32_t i = 0; i < n; ++i, ++at_full)
+      if ((uint32_t)at_full < (uint32_t)entries) map[at_full] = int4{g, (int)(lo + i * piece), (int)(lo + (i + 1) * piece), many ? at_part + i : -1};
+    if (tail) {
+      int32_t at = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (quarter == q) at = at_rest[q]++;
+      if ((uint32_t)at < (uint32_t)entries) map[at] = int4{g, (int)(lo + n * piece), (int)(lo + n * piece + left), many ? at_part + n : -1};
+    }
+    if (many) {
+      if ((uint32_t)at_split < (uint32_t)most) sums[at_split] = int4{g, at_part, n + tail, 0};
+      ++at_split;
+      at_part += n + tail;
+    }
+  }
+}
+
+// All maps of a call in one launch, a workgroup each.
+struct MapArgs {
+  const int32_t* offsets;
+  int G;
+  int64_t M;
+  int tile[2];                 // row tiles: two maps at most
+  int64_t ntiles[2];
+  int4* map[2];
+  int32_t* first[2];
+  int64_t piece;               // pieces of the sums
+  int entries, most;
+  int4* pieces;
+  int4* sums;
+  int32_t* count;
+};
+
+__global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
+  extern __shared__ int32_t start[];        // [G + 1] | [16]
+  int32_t* red = start + a.G + 1;
+  if (blockIdx.x < 2) {
+    if (a.map[blockIdx.x] != nullptr)
+      row_tiles(a.offsets, a.G, a.M, a.tile[blockIdx.x], a.ntiles[blockIdx.x], a.map[blockIdx.x], a.first[blockIdx.x], start, red);
+  } else if (a.pieces != nullptr) {
+    sum_pieces(a.offsets, a.G, a.M, a.piece, a.entries, a.most, a.pieces, a.sums, a.count, red);
   }
 }
 
@@ -156,14 +257,27 @@ __global__ __launch_bounds__(1024) void db_kernel(const float* __restrict__ part
 
 // ---- sums over the splits of the reduce axis, in order -------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict__ slab, int splits, int64_t elems, int64_t groups,
-                                                        T* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems * groups; i += (int64_t)gridDim.x * 256) {
-    const int64_t g = i / elems, e = i % elems;
-    const float* p = slab + g * splits * elems + e;
+__global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict__ slab, int splits, int64_t elems, T* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256) {
     float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += p[k * elems];
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) s += slab[k * elems + i];
     out[i] = (T)s;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void piece_sum_kernel(const float* __restrict__ slab, const int4* __restrict__ sums,
+                                                        const int32_t* __restrict__ count, int64_t elems, T* __restrict__ out) {
+  for (int i = blockIdx.y; i < count[1]; i += gridDim.y) {
+    const int4 m = sums[i];
+    const float* p = slab + m.y * elems;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < elems; e += (int64_t)gridDim.x * 256) {
+      float s = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < m.z; ++k) s += p[k * elems + e];
+      out[m.x * elems + e] = (T)s;
+    }
   }
 }
 
@@ -284,6 +398,8 @@ struct GemmPlan {
   int64_t row_tiles;
   int col_tiles;
   size_t slab;                 // bytes
+  int64_t piece;               // kDw with groups: frames of a piece, entries of its map and parts at most
+  int64_t entries, parts;
 };
 
 static void tile_size(int tile, int& br, int& bc) {
@@ -303,16 +419,18 @@ static void tile_size(int tile, int& br, int& bc) {
 // 560 / 760 outputs a nanosecond and stage, so the large tile wins wherever it fills the chip; fp32 is bound by its matrix
 // rate), and a tile its first load and its epilogue.  65536 x 4096 -> 256: 207 us in tiles of 128, 173 in tiles of 256;
 // 16384 x 512 -> 512: 15 us in tiles of 128, 22 in tiles of 256.  Splitting the sum costs a launch and two passes over the
-// parts.  Leaves are unequal: a chip that holds every tile of a grouped dW at once waits for the largest leaf, counted as
-// two turns (131072 rows, 64 leaves, 512 x 512: 141 / 104 / 255 us for tiles of 64 / 128 / 256).  Transposing reads
-// cost the large tile's stages a tenth more (8192^3: 938 / 1035 / 1100 us forward, dx, dW).
+// parts.  Transposing reads cost the large tile's stages a tenth more (8192^3: 938 / 1035 / 1100 us forward, dx, dW).
+//
+// dW with groups: leaves are unequal, and a launch waits for its longest tile.  A leaf longer than `piece` frames is summed
+// in pieces; the shorter they are the evener the end (half a piece is idle on average), the more partial results pass
+// through memory.
 static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64_t K, bool grouped, int G, bool direct) {
   GemmPlan p;
   const int e = dtype_bytes(dtype), bk = 128 / e;
   const bool by_rows = grouped && kind != kDw;
-  const int64_t z = grouped && kind == kDw ? G : 1;
+  const bool by_sum = grouped && kind == kDw;
   const int64_t per_group = by_rows ? ceil_div(rows, G) : rows;
-  const int64_t sum = grouped && kind == kDw ? ceil_div(K, G) : K;
+  p.piece = p.entries = p.parts = 0;
   p.splits = 1;
   if (cols <= 32 && per_group > 32) {
     p.tile = kTileTall;
@@ -327,26 +445,46 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
   static const double kTileCost[] = {5.0, 3.5, 8.0};
   static const int kPerCu[] = {2, 4, 1};
   auto row_of = [](int tile) { return tile == kTile128 ? 0 : tile == kTile256 ? 2 : 1; };
-  const int64_t stages = std::max<int64_t>(1, ceil_div(sum, bk));
+  const int64_t stages = std::max<int64_t>(1, ceil_div(K, bk));
   auto tiles_of = [&](int tile) {
     int br, bc;
     tile_size(tile, br, bc);
-    return (ceil_div(rows, br) + (by_rows ? G / 2 : 0)) * ceil_div(cols, bc) * z;
+    return (ceil_div(rows, br) + (by_rows ? G / 2 : 0)) * ceil_div(cols, bc);
   };
   auto cost = [&](int tile, int64_t s) {
     const int r = row_of(tile);
     const int64_t n = tiles_of(tile) * s;
     const int each = (int)std::min<int64_t>(kPerCu[r], std::max<int64_t>(1, ceil_div(n, kNumCU)));
-    double turns = (double)ceil_div(n, (int64_t)each * kNumCU);
-    if (grouped && kind == kDw) turns = std::max((double)n / (each * kNumCU), 2.0 / s);
-    return turns * ((double)ceil_div(stages, s) * (e == 4 ? k32 : k16)[r][each - 1] * (r == 2 ? 1.0 + 0.08 * kind : 1.0) + kTileCost[r]) +
-           (s > 1 ? 4.0 + 8.0 * s * rows * cols * z / 4.0e6 : 0.0);
+    const double turns = (double)ceil_div(n, (int64_t)each * kNumCU), stage = (e == 4 ? k32 : k16)[r][each - 1] * (r == 2 ? 1.0 + 0.08 * kind : 1.0);
+    return turns * ((double)ceil_div(stages, s) * stage + kTileCost[r]) + (s > 1 ? 4.0 + 8.0 * s * rows * cols / 4.0e6 : 0.0);
   };
-  const int64_t most = by_rows ? 1 : std::min<int64_t>(64, std::max<int64_t>(1, stages / 2));
+  // groups of the sum, `len` stages a piece: the work, the pieces' first loads and epilogues, half a piece at the end, the
+  // parts -- nearly all pieces where they are shorter than a leaf is on average, else those of the long leaves
+  auto cost_of_pieces = [&](int tile, int64_t len) {
+    const int r = row_of(tile);
+    const double slots = (double)kPerCu[r] * kNumCU, tiles = (double)tiles_of(tile), work = tiles * (double)(stages + G / 2) / slots;
+    const double full = (double)stages / (double)len, stage = (e == 4 ? k32 : k16)[r][kPerCu[r] - 1] * (r == 2 ? 1.16 : 1.0);
+    const double parts = stages >= len * G ? full + G / 2 : 0.3 * full;
+    return work * stage + (full + G) * tiles / slots * kTileCost[r] + 0.5 * len * stage + 4.0 + 8.0 * parts * rows * cols / 4.0e6;
+  };
+  const int64_t most = grouped ? 1 : std::min<int64_t>(64, std::max<int64_t>(1, stages / 2));
   const int tried[] = {p.tile, kTile128, kTile256};
   double best = 1e300;
   int tile = p.tile;
-  for (int i = 0; i < (p.tile == kTile64 ? (direct && e == 2 ? 3 : 2) : 1); ++i)
+  for (int i = 0; i < (p.tile == kTile64 ? (direct && e == 2 ? 3 : 2) : 1); ++i) {
+    if (by_sum) {
+      const int r = row_of(tried[i]);
+      const int64_t even = std::max<int64_t>(8, tiles_of(tried[i]) * stages / (kPerCu[r] * kNumCU));
+      for (int64_t len = std::max<int64_t>(8, even / 2); len <= 8 * even; len *= 2) {
+        const double c = cost_of_pieces(tried[i], len);
+        if (c < best * 0.98) {
+          best = c;
+          tile = tried[i];
+          p.piece = len * bk;
+        }
+      }
+      continue;
+    }
     for (int64_t s = 1; s <= most; s *= 2) {
       const double c = cost(tried[i], s);
       if (c < best * 0.98) {
@@ -355,6 +493,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
         p.splits = (int)s;
       }
     }
+  }
   p.tile = tile;
   if (const char* f = dev_getenv(kind == kFwd ? "BNPVI_TILE_FWD" : kind == kDx ? "BNPVI_TILE_DX" : "BNPVI_TILE_DW")) p.tile = atoi(f);
   if (const char* f = dev_getenv(kind == kFwd ? "BNPVI_SPLIT_FWD" : kind == kDx ? "BNPVI_SPLIT_DX" : "BNPVI_SPLIT_DW")) p.splits = atoi(f);
@@ -362,7 +501,12 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
   tile_size(p.tile, br, bc);
   p.row_tiles = ceil_div(rows, br) + (by_rows ? G + 2 : 0);
   p.col_tiles = (int)ceil_div(cols, bc);
-  p.slab = p.splits > 1 ? (size_t)z * p.splits * rows * cols * 4 : 0;
+  p.slab = p.splits > 1 ? (size_t)p.splits * rows * cols * 4 : 0;
+  if (by_sum) {
+    p.entries = K / p.piece + G;                                 // every group has one entry at least, and one that is not full
+    p.parts = K > p.piece ? 2 * (K / p.piece) : 0;               // a group of more than a piece has two at most per full one
+    p.slab = (size_t)p.parts * rows * cols * 4;
+  }
   return p;
 }
 
@@ -374,7 +518,7 @@ struct DensePlan {
   int64_t dz_tiles;
   // byte offsets of the workspace's parts
   size_t fwd_map, fwd_slab, fwd_bytes;
-  size_t dz_map, dz_first, dx_map, part, dz, slab, db_slab, bwd_bytes;
+  size_t dz_map, dz_first, dx_map, dw_map, dw_sums, dw_count, part, dz, slab, db_slab, bwd_bytes;
 };
 
 static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, bool direct) {
@@ -399,10 +543,13 @@ static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, b
   p.dz_map = take(p.grouped ? p.dz_tiles * sizeof(int4) : 0);
   p.dz_first = take(p.grouped ? (size_t)(G + 1) * 4 : 0);
   p.dx_map = take(p.grouped ? p.dx.row_tiles * sizeof(int4) : 0);
+  p.dw_map = take((size_t)p.dw.entries * sizeof(int4));
+  p.dw_sums = take((size_t)p.dw.parts / 2 * sizeof(int4));
+  p.dw_count = take(p.grouped ? 8 : 0);
   p.part = take((size_t)p.dz_tiles * n * 4);
   p.dz = take((size_t)M * n * e);
   p.slab = take(std::max(p.dx.slab, p.dw.slab));
-  p.db_slab = take(p.dw.splits > 1 ? (size_t)(G > 0 ? G : 1) * p.dw.splits * n * 4 : 0);
+  p.db_slab = take((size_t)(p.grouped ? p.dw.parts : p.dw.splits > 1 ? p.dw.splits : 0) * n * 4);
   p.bwd_bytes = at;
   return p;
 }
@@ -423,12 +570,11 @@ static int run_gemm(int kind, int dtype, const GemmPlan& p, bool direct, GemmArg
                                : launch_gemm_f16(kind, p.tile, direct, a, ctx, s);
 }
 
-static int row_tiles(const int32_t* offsets, int G, int64_t M, int tile, int64_t ntiles, void* map, void* first, int device,
-                     hipStream_t s) {
+static int launch_maps(const MapArgs& a, int device, hipStream_t s) {
   static LdsLimit limit;
-  const size_t lds = (size_t)(G + 1 + 16) * 4;
-  if (lds > 64 * 1024) BNPVI_HIP(limit.raise((const void*)row_tiles_kernel, device));
-  row_tiles_kernel<<<1, 1024, lds, s>>>(offsets, G, M, tile, ntiles, (int4*)map, (int32_t*)first);
+  const size_t lds = (size_t)(a.G + 1 + 16) * 4;
+  if (lds > 64 * 1024) BNPVI_HIP(limit.raise((const void*)maps_kernel, device));
+  maps_kernel<<<a.pieces ? 3 : a.map[1] ? 2 : 1, 1024, lds, s>>>(a);
   BNPVI_LAUNCH_CHECK();
   return BNPVI_OK;
 }
@@ -456,8 +602,14 @@ static void launch_db(const float* part, const int32_t* first, int64_t tiles, in
 }
 
 template <typename T>
-static void launch_split_sum(const float* slab, int splits, int64_t elems, int64_t groups, void* out, hipStream_t s) {
-  split_sum_kernel<T><<<flat_grid(elems * groups), 256, 0, s>>>(slab, splits, elems, groups, (T*)out);
+static void launch_sums(const float* slab, const GemmPlan& p, bool grouped, const int4* sums, const int32_t* count, int64_t elems, void* out,
+                        hipStream_t s) {
+  if (grouped)
+    piece_sum_kernel<T><<<dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(elems, 256), 1024)),
+                               (unsigned)std::min<int64_t>(p.parts / 2, 64)),
+                          256, 0, s>>>(slab, sums, count, elems, (T*)out);
+  else
+    split_sum_kernel<T><<<flat_grid(elems), 256, 0, s>>>(slab, p.splits, elems, (T*)out);
 }
 
 constexpr int64_t kMaxPitchBytes = int64_t(1) << 22;       // 256 rows of a tile stay below 2^31 bytes
@@ -544,9 +696,15 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
     return BNPVI_OK;
   }
   if (G > 0) {
-    int br, bc;
-    tile_size(p.fwd.tile, br, bc);
-    const int r = row_tiles(offsets, G, M, br, p.fwd.row_tiles, wk + p.fwd_map, nullptr, ctx->device, s);
+    int bc;
+    MapArgs m = {};
+    m.offsets = offsets;
+    m.G = G;
+    m.M = M;
+    tile_size(p.fwd.tile, m.tile[0], bc);
+    m.ntiles[0] = p.fwd.row_tiles;
+    m.map[0] = (int4*)(wk + p.fwd_map);
+    const int r = launch_maps(m, ctx->device, s);
     if (r) return r;
     a.map = (const int4*)(wk + p.fwd_map);
   }
@@ -597,10 +755,34 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   // (16385 x 64 -> 4096 fp32: 70 us of 450 were a pass over dy for that)
   const bool db_in_dw = db && dw && !dact && p.dw.tile != kTile256;
   const bool need_dz = (dact != nullptr && (dx || dw)) || (db && !db_in_dw) || dres;
-  if (need_dz && G > 0) {
-    first = (int32_t*)(wk + p.dz_first);
-    dz_map = (const int4*)(wk + p.dz_map);
-    r = row_tiles(offsets, G, M, kDzRows, p.dz_tiles, wk + p.dz_map, first, ctx->device, s);
+  if (G > 0) {
+    MapArgs m = {};
+    int bc;
+    m.offsets = offsets;
+    m.G = G;
+    m.M = M;
+    if (need_dz) {
+      first = (int32_t*)(wk + p.dz_first);
+      dz_map = (const int4*)(wk + p.dz_map);
+      m.tile[0] = kDzRows;
+      m.ntiles[0] = p.dz_tiles;
+      m.map[0] = (int4*)(wk + p.dz_map);
+      m.first[0] = first;
+    }
+    if (dx && !none) {
+      tile_size(p.dx.tile, m.tile[1], bc);
+      m.ntiles[1] = p.dx.row_tiles;
+      m.map[1] = (int4*)(wk + p.dx_map);
+    }
+    if (dw) {
+      m.piece = p.dw.piece;
+      m.entries = (int)p.dw.entries;
+      m.most = (int)(p.dw.parts / 2);
+      m.pieces = (int4*)(wk + p.dw_map);
+      m.sums = (int4*)(wk + p.dw_sums);
+      m.count = (int32_t*)(wk + p.dw_count);
+    }
+    r = launch_maps(m, ctx->device, s);
     if (r) return r;
   }
   const void* dz = dy;
@@ -645,13 +827,7 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.C = dx;
     a.ldc = lddx;
     a.cvec = wide(dx, lddx, e);
-    if (G > 0) {
-      int br, bc;
-      tile_size(p.dx.tile, br, bc);
-      r = row_tiles(offsets, G, M, br, p.dx.row_tiles, wk + p.dx_map, nullptr, ctx->device, s);
-      if (r) return r;
-      a.map = (const int4*)(wk + p.dx_map);
-    }
+    if (G > 0) a.map = (const int4*)(wk + p.dx_map);
     if (p.dx.slab) a.slab = (float*)(wk + p.slab);
     r = run_gemm(kDx, dtype, p.dx, direct, a, ctx, s);
     if (r) return r;
@@ -679,7 +855,11 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.cols = K;
     a.K = M;
     a.G = groups;
-    a.offsets = offsets;
+    if (G > 0) {
+      a.map = (const int4*)(wk + p.dw_map);
+      a.used = (const int32_t*)(wk + p.dw_count);
+      a.entries = (int)p.dw.entries;
+    }
     a.C = dw;
     a.ldc = K;
     a.c_group = n * K;
@@ -692,22 +872,19 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     r = run_gemm(kDw, dtype, p.dw, direct, a, ctx, s);
     if (r) return r;
     if (p.dw.slab) {
-      if (dtype == BNPVI_F32)
-        launch_split_sum<float>(a.slab, p.dw.splits, n * K, groups, dw, s);
-      else if (dtype == BNPVI_BF16)
-        launch_split_sum<bf16_t>(a.slab, p.dw.splits, n * K, groups, dw, s);
-      else
-        launch_split_sum<f16_t>(a.slab, p.dw.splits, n * K, groups, dw, s);
-      BNPVI_LAUNCH_CHECK();
-      if (db_in_dw) {
+      const int4* sums = (const int4*)(wk + p.dw_sums);
+      const int32_t* count = (const int32_t*)(wk + p.dw_count);
+      auto add = [&](const float* slab, int64_t elems, void* out) {
         if (dtype == BNPVI_F32)
-          launch_split_sum<float>(a.db_slab, p.dw.splits, n, groups, db, s);
+          launch_sums<float>(slab, p.dw, G > 0, sums, count, elems, out, s);
         else if (dtype == BNPVI_BF16)
-          launch_split_sum<bf16_t>(a.db_slab, p.dw.splits, n, groups, db, s);
+          launch_sums<bf16_t>(slab, p.dw, G > 0, sums, count, elems, out, s);
         else
-          launch_split_sum<f16_t>(a.db_slab, p.dw.splits, n, groups, db, s);
-        BNPVI_LAUNCH_CHECK();
-      }
+          launch_sums<f16_t>(slab, p.dw, G > 0, sums, count, elems, out, s);
+      };
+      add(a.slab, n * K, dw);
+      if (db_in_dw) add(a.db_slab, n, db);
+      BNPVI_LAUNCH_CHECK();
     }
   }
   return BNPVI_OK;

@@ -45,7 +45,7 @@ static int launch_tile(const GemmArgs& a, int tile, const bnpvi_ctx* ctx, int64_
 }
 
 int BNPVI_GEMM_LAUNCH(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s) {
-  const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles * (kind == kDw ? (int64_t)a.G * a.splits : a.splits);
+  const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles * (kind == kDw && a.map != nullptr ? a.entries : a.splits);
   if (tiles <= 0) return BNPVI_OK;
   BNPVI_REQUIRE(tiles < (int64_t(1) << 31), "dense: %lld tiles", (long long)tiles);
   if (direct) {

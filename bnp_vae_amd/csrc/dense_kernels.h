@@ -50,7 +50,10 @@ struct GemmArgs {
   int64_t rows, cols, K;       // rows of C (all groups), columns, reduce extent (kDw with groups: all frames)
   int64_t s_group, c_group;    // elements between the groups' S (kFwd, kDx) or C (kDw)
   const int32_t* offsets;      // groups' bounds (kDw) or nullptr
-  const int4* map;             // row tiles {group, first row, end row} (kFwd, kDx with groups) or nullptr
+  const int4* map;             // with groups -- kFwd, kDx: row tiles {group, first row, end row}; kDw: pieces of the sum
+                               // {group, first frame, end frame, part or -1}
+  const int32_t* used;         // kDw with groups: entries of the map in use
+  int entries;                 // at most
   int G, splits;
   int row_tiles, col_tiles;
   int cvec;                    // C, residual and derivative take 16-byte accesses
@@ -356,24 +359,38 @@ struct Tile {
   __device__ __forceinline__ int stages(int bk) const { return kext > bk ? (kext + bk - 1) / bk : 1; }
 };
 
+// One XCD's share of a grouped dW, a like mixture of the pieces for all eight: every eighth piece with all its tiles, which
+// then share an L2, or where there are few pieces of many tiles an eighth of every piece's.
+struct Share {
+  uint32_t per, tile0, entry0, every;
+};
+
 template <int KIND, int BR, int BC, int BK>
-__device__ __forceinline__ bool find_tile(const GemmArgs& a, uint32_t lin, Tile& t) {
+__device__ __forceinline__ bool find_tile(const GemmArgs& a, uint32_t lin, const Share& sh, Tile& t) {
   // divisions are done by the vector unit: their results are told to be the same in every lane
+  if (KIND == kDw && a.map != nullptr) {
+    const uint32_t e = uniform(lin / sh.per), rest = sh.tile0 + lin - e * sh.per;
+    const uint32_t rt = uniform(rest / (uint32_t)a.col_tiles), ct = rest - rt * (uint32_t)a.col_tiles;
+    const int4 m = a.map[sh.entry0 + sh.every * e];
+    t.g = m.x;
+    t.z = m.w;
+    t.row0 = (int64_t)rt * BR;
+    t.col0 = (int64_t)ct * BC;
+    t.k_lo = m.y;
+    t.kext = m.z - m.y;
+    t.nr = (int)(a.rows - t.row0 < BR ? a.rows - t.row0 : BR);
+    t.nc = (int)(a.cols - t.col0 < BC ? a.cols - t.col0 : BC);
+    return true;
+  }
   const uint32_t row = uniform(lin / (uint32_t)a.col_tiles), ct = lin - row * (uint32_t)a.col_tiles;
   const uint32_t zz = uniform(row / (uint32_t)a.row_tiles), rt = row - zz * (uint32_t)a.row_tiles;
-  t.z = (int)zz;
-  t.g = (int)uniform(zz / (uint32_t)a.splits);
-  const int split = (int)zz - t.g * a.splits;
+  const int split = (int)zz;
+  t.z = split;
+  t.g = 0;
   t.row0 = (int64_t)rt * BR;
   t.col0 = (int64_t)ct * BC;
   int64_t row_end = a.rows, k_lo = 0, k_hi = a.K;
-  if (KIND == kDw) {
-    if (a.offsets != nullptr) {
-      const int64_t M = a.K, lo = a.offsets[t.g], hi = a.offsets[t.g + 1];
-      k_lo = lo < 0 ? 0 : lo > M ? M : lo;
-      k_hi = hi < k_lo ? k_lo : hi > M ? M : hi;
-    }
-  } else if (a.map != nullptr) {
+  if (KIND != kDw && a.map != nullptr) {
     const int4 m = a.map[rt];
     t.g = m.x;
     t.row0 = m.y;
@@ -401,10 +418,12 @@ struct Stream {
   typedef Source<T, kKM, ROWS ? BR : BC, THREADS, KB> Src;
   Src src;
   uint32_t lin, last, step;
+  Share sh;
   int kt, nk;
 
-  __device__ __forceinline__ void begin(const GemmArgs& a, uint32_t first, uint32_t end, uint32_t every) {
+  __device__ __forceinline__ void begin(const GemmArgs& a, uint32_t first, uint32_t end, uint32_t every, const Share& of) {
     lin = first;
+    sh = of;
     last = end;
     step = every;
     enter(a);
@@ -413,7 +432,7 @@ struct Stream {
     Tile t;
     kt = 0;
     for (; lin < last; lin += step)
-      if (find_tile<KIND, BR, BC, kBK>(a, lin, t)) {
+      if (find_tile<KIND, BR, BC, kBK>(a, lin, sh, t)) {
         lin += step;
         const int g = t.g < 0 ? 0 : t.g;
         if (ROWS)
@@ -449,13 +468,26 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
 
   const uint32_t xcd = blockIdx.x & 7, q8 = tiles >> 3, rem = tiles & 7;
   const uint32_t step = (gridDim.x + 7 - xcd) >> 3;
-  const uint32_t first = xcd * q8 + (xcd < rem ? xcd : rem), last = first + q8 + (xcd < rem ? 1 : 0);
+  uint32_t first = xcd * q8 + (xcd < rem ? xcd : rem), last = first + q8 + (xcd < rem ? 1 : 0);
+  Share sh = {1, 0, 0, 1};
+  if (KIND == kDw && a.map != nullptr) {
+    const int32_t u = *a.used;
+    const uint32_t used = u < 0 ? 0 : u < a.entries ? u : a.entries, per = (uint32_t)a.row_tiles * (uint32_t)a.col_tiles;
+    first = 0;
+    if (per >= 64 && used < 64) {
+      sh = Share{(per >> 3) + (xcd < (per & 7) ? 1 : 0), xcd * (per >> 3) + (xcd < (per & 7) ? xcd : per & 7), 0, 1};
+      last = used * sh.per;
+    } else {
+      sh = Share{per, 0, xcd, 8};
+      last = used > xcd ? (used - xcd + 7) / 8 * per : 0;
+    }
+  }
   uint32_t lin = first + (blockIdx.x >> 3);
   if (lin >= last) return;
   Stream<T, KIND, BR, BC, KB, THREADS, true> sr;
   Stream<T, KIND, BR, BC, KB, THREADS, false> ss;
-  sr.begin(a, lin, last, step);
-  ss.begin(a, lin, last, step);
+  sr.begin(a, lin, last, step, sh);
+  ss.begin(a, lin, last, step, sh);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave / (BC / WC) * WR, wc = wave % (BC / WC) * WC;
@@ -500,7 +532,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
 
   Tile t;
   for (; lin < last; lin += step) {
-    if (!find_tile<KIND, BR, BC, BK>(a, lin, t)) continue;
+    if (!find_tile<KIND, BR, BC, BK>(a, lin, sh, t)) continue;
     f32x16 acc[FR][FC];
 #pragma unroll
     for (int i = 0; i < FR; ++i)
@@ -583,7 +615,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
         const float sum = rsum[i] + __shfl_xor(rsum[i], 32);
         const int rl = wr + 32 * i + lane;
         if (lane < 32 && rl < t.nr) {
-          if (a.db_slab != nullptr)
+          if (a.db_slab != nullptr && t.z >= 0)
             a.db_slab[(int64_t)t.z * a.rows + t.row0 + rl] = sum;
           else
             reinterpret_cast<T*>(a.db)[(int64_t)t.g * a.rows + t.row0 + rl] = (T)sum;
@@ -631,7 +663,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
         const int64_t row = t.row0 + rl;
         const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + r * (WC * 4) + (((2 * c) ^ (r & (SLOTS - 1))) << 4));
         const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + r * (WC * 4) + (((2 * c + 1) ^ (r & (SLOTS - 1))) << 4));
-        if (a.slab != nullptr) {
+        if (a.slab != nullptr && t.z >= 0) {
           float* out = a.slab + ((int64_t)t.z * a.rows + row) * a.cols + col;
           if (left == 8 && a.cols % 4 == 0) {
             *reinterpret_cast<f32x4*>(out) = v0;
