@@ -304,6 +304,16 @@ class DeviceVI(object):
                                 _ptr(self.gate_s2), self._stream()), "bnpvi_leaf_s2")
         vdist.allreduce_sum_(self.gate_s2, self.group)
 
+    def leaf_routes(self, k, renormalize=True):
+        """The k likeliest leaves of every frame by the responsibilities on the device, and the plan that brings the
+        frames of one leaf together: (leaf [N, k] int32, weight [N, k] float32, layers.LeafPlan)."""
+        from . import layers
+        if self.phi is None or self.tree is None:
+            raise RuntimeError("leaf_routes: no responsibilities on the device yet")
+        L = self.tree.L
+        leaf, weight = layers.top_leaves(self.phi, k, num_leaves=L, renormalize=renormalize)
+        return leaf, weight, layers.sort_by_leaf(leaf, L)
+
     def params_prior(self):
         """node parameters + gamma-step + prior table (+ leaf operands) in one call."""
         K, Lp = self.tree.K, self.tree.Lp

@@ -33,11 +33,50 @@ def _flatten(nodes_list):
     return order, parent, is_leaf, alpha
 
 
-def closest_frames(nodes_list, z, K, device=None):
+ENCODE_ROWS = 1 << 18            # features are encoded this many rows at a time
+
+
+def _latents(z, encoder, device):
+    """z itself, or with `encoder` -- [(weight (n, F), bias (n,) or None, activation), ...] on the GPU, applied in turn --
+    the latents that its dense layers make of the features z (the encoder of src/model.py:70-83 is one such layer with
+    softsign): a float32 tensor on the GPU."""
+    if encoder is None:
+        return z
+    import torch
+    from . import layers
+    encoder = [tuple(layer) for layer in encoder]
+    if not encoder or any(len(layer) != 3 for layer in encoder):
+        raise ValueError("encoder must be a sequence of (weight, bias, activation) layers")
+    weight = encoder[0][0]
+    if device is not None and weight.device.index != torch.device("cuda", device if isinstance(device, int) else device.index).index:
+        raise ValueError("encoder is on %s, the call on GPU %s" % (weight.device, device))
+    x = z if isinstance(z, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(z))
+    out = torch.empty((x.shape[0], encoder[-1][0].shape[0]), dtype=torch.float32, device=weight.device)
+    with torch.no_grad():
+        for lo in range(0, x.shape[0], ENCODE_ROWS):
+            h = x[lo:lo + ENCODE_ROWS].to(device=weight.device, dtype=weight.dtype)
+            for w, b, activation in encoder:
+                h = layers.dense(h, w, b, activation)
+            out[lo:lo + ENCODE_ROWS] = h
+    return out
+
+
+def _rows_by_leaf(assign, L):
+    """Row indices in the order of their leaves, rows ascending within a leaf."""
+    import torch
+    from . import layers
+    from ._lib import lib
+    if L <= lib.bnpvi_leaf_sort_max_leaves() and assign.shape[0] < 1 << 31:
+        return layers.sort_by_leaf(assign, L).order.to(torch.int64)
+    return torch.sort(assign.to(torch.int64), stable=True).indices
+
+
+def closest_frames(nodes_list, z, K, device=None, encoder=None):
     """For every node of the hierarchy: the (up to) K frames closest to its alpha among the frames
     whose nearest leaf lies below it (src/create_hierarchy.py:40-53, 82-91).
 
-    z: (N, D) latent codes (NumPy or torch).  Returns (path_assignments, node_to_frames):
+    z: (N, D) latent codes (NumPy or torch), or with `encoder` -- a sequence of (weight, bias, activation) dense layers on
+    the GPU, see layers.dense -- the features (N, F) they are computed from.  Returns (path_assignments, node_to_frames):
       path_assignments  (N,) int  index of the nearest leaf, leaves numbered depth-first
                                   (:82-84; the reference numbers them in the Python-2 order of a
                                   dict keyed by Node objects, which is address dependent)
@@ -49,7 +88,8 @@ def closest_frames(nodes_list, z, K, device=None):
     from . import _lib
     from .engine import DeviceVI
     order, parent, is_leaf, alpha = _flatten(nodes_list)
-    dev = DeviceVI(device=device)
+    z = _latents(z, encoder, device)
+    dev = DeviceVI(device=device if encoder is None else z.device)
     try:
         N = int(z.shape[0])
         dev.set_latents(z, np.zeros(N, dtype=np.int32), 1)
@@ -58,7 +98,7 @@ def closest_frames(nodes_list, z, K, device=None):
         node, dist = dev.path_distances(assign)
         depth = node.shape[1]
         # candidates in the reference's order: leaves depth-first, rows ascending within a leaf
-        rows = torch.sort(assign.to(torch.int64), stable=True).indices
+        rows = _rows_by_leaf(assign, dev.tree.L)
         cand_node = node[rows].reshape(-1).to(torch.int64)
         cand_dist = dist[rows].reshape(-1)
         cand_row = rows.repeat_interleave(depth)
@@ -81,13 +121,15 @@ def closest_frames(nodes_list, z, K, device=None):
         dev.close()
 
 
-def nearest_leaf(nodes_list, z, device=None):
+def nearest_leaf(nodes_list, z, device=None, encoder=None):
     """(N,) index of the nearest leaf (leaves depth-first) of every row of z:
-    src/compute_acc_frame_avg_dynamic.py:49-52 / :127-128 on the device (hard-mode E-step)."""
+    src/compute_acc_frame_avg_dynamic.py:49-52 / :127-128 on the device (hard-mode E-step).  encoder: as in
+    `closest_frames`."""
     from . import _lib
     from .engine import DeviceVI
     order, parent, is_leaf, alpha = _flatten(nodes_list)
-    dev = DeviceVI(device=device)
+    z = _latents(z, encoder, device)
+    dev = DeviceVI(device=device if encoder is None else z.device)
     try:
         N = int(z.shape[0])
         dev.set_latents(z, np.zeros(N, dtype=np.int32), 1)
@@ -98,7 +140,7 @@ def nearest_leaf(nodes_list, z, device=None):
         dev.close()
 
 
-def class_vote(nodes_list, z_train, train_labels, z_test, decay_factor=0.0, device=None):
+def class_vote(nodes_list, z_train, train_labels, z_test, decay_factor=0.0, device=None, encoder=None):
     """Tree-decayed class vote of src/compute_acc_frame_avg_dynamic.py:49-129.
 
     Frames vote for the class of their nearest leaf (:61-63); votes are summed up the tree
@@ -106,7 +148,7 @@ def class_vote(nodes_list, z_train, train_labels, z_test, decay_factor=0.0, devi
     ancestor (:89-108); leaves without any score borrow the class of the nearest leaf (by alpha)
     that has one (:114-122); test frames get the class of their nearest leaf (:124-129).
     train_labels: (N,) integer classes 0..C-1.  Returns (path2class [L], predicted [N_test]);
-    leaves are numbered depth-first.  The O(N) parts (both nearest-leaf passes, the vote
+    leaves are numbered depth-first.  encoder: as in `closest_frames`, for both sets.  The O(N) parts (both nearest-leaf passes, the vote
     histogram) run on the device, the O(L*C) tree arithmetic on the host."""
     import torch
     order, parent, is_leaf, alpha = _flatten(nodes_list)
@@ -114,7 +156,7 @@ def class_vote(nodes_list, z_train, train_labels, z_test, decay_factor=0.0, devi
     L = len(leaves)
     labels = np.asarray(train_labels).astype(np.int64)
     C = len(np.unique(labels))                                          # :47
-    assign = nearest_leaf(nodes_list, z_train, device)
+    assign = nearest_leaf(nodes_list, z_train, device, encoder)
     flat = torch.from_numpy(assign * C + labels)
     counts = torch.bincount(flat, minlength=L * C).numpy().reshape(L, C).astype(np.float64)
     cumulative = np.zeros((len(order), C))
@@ -139,5 +181,5 @@ def class_vote(nodes_list, z_train, train_labels, z_test, decay_factor=0.0, devi
                 dist[m] = np.inf
                 m = int(np.argmin(dist))
             path2class[j] = path2class[m]
-    predicted = path2class[nearest_leaf(nodes_list, z_test, device)]
+    predicted = path2class[nearest_leaf(nodes_list, z_test, device, encoder)]
     return path2class, predicted

@@ -797,6 +797,18 @@ class VarInf(object):
         got = dev.phi.index_select(0, r).index_select(1, c).to('cpu').numpy().astype(np.float64)
         return got * np.asarray(scale, dtype=np.float64)[None, :]
 
+    def leaf_routes(self, k, renormalize=True):
+        """The k likeliest leaves of every frame by the current responsibilities, as device tensors, and the plan that
+        brings the frames of one leaf together: (leaf (N, k) int32, weight (N, k) float32, layers.LeafPlan).  Leaves are
+        numbered depth-first (the order of `get_alpha_leaves`), rows are the frames in `vidid_frameid_to_idx` order (of
+        this rank, in a process group).  It is what `layers.dispatch`, `layers.dense` and `layers.combine` take to run
+        every frame through weights of its own leaves."""
+        dev = self._engine()
+        if dev.Z is None:
+            raise RuntimeError("leaf_routes: no latent codes on the device yet")
+        self._sync_phi()
+        return dev.leaf_routes(k, renormalize)
+
     def get_phi_leaves(self, idx):                               # src/var_inf.py:38-48
         result = {}
         unvisited = [self.root]
