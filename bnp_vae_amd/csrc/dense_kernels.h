@@ -647,6 +647,43 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
 #pragma unroll
     for (int i = 0; i < FR; ++i) {
       if (wr + 32 * i >= t.nr) break;          // uniform over the wave
+      if constexpr (KIND != kFwd && sizeof(T) == 2) {
+        // nothing is added to dx and dW any more: rounded first, half as much passes through LDS
+        if (a.slab == nullptr || t.z < 0) {
+          typedef T four __attribute__((ext_vector_type(4)));
+#pragma unroll
+          for (int j = 0; j < FC; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = lane & 31, s = 4 * j + e;
+              const f32x16& v = acc[i][j];
+              *reinterpret_cast<four*>(mine + r * (WC * 2) + ((s ^ (r & (WC / 8 - 1))) << 4) + 8 * (lane >> 5)) =
+                  four{(T)v[4 * e], (T)v[4 * e + 1], (T)v[4 * e + 2], (T)v[4 * e + 3]};
+            }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+          for (int it = 0; it < 32 / RPI; ++it) {
+            const int r = it * RPI + lane / LPR, rl = wr + 32 * i + r;
+            if (rl >= t.nr || left <= 0) continue;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * (WC * 2) + ((c ^ (r & (WC / 8 - 1))) << 4));
+            T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? t.g * a.c_group : 0) + (t.row0 + rl) * a.ldc + col;
+            if (vec) {
+              __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out));
+            } else {
+              union {
+                u32x4 u;
+                T t[8];
+              } x;
+              x.u = v;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (e < left) out[e] = x.t[e];
+            }
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next 32 rows are written
+          continue;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < FC; ++j)
 #pragma unroll
