@@ -179,11 +179,11 @@ __global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
 // dy, 0 in the rows of no group.
 constexpr int kDzRows = 128;
 
-template <typename T, int E>
+template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64_t lddy, const typename Deriv<T>::type* __restrict__ d,
                                                  int64_t ldd, const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz,
                                                  int64_t lddz, T* __restrict__ dres, int64_t lddres, float* __restrict__ part) {
-  constexpr int CT = 32;                     // threads across
+  constexpr int CT = 32, E = 8;              // threads across, columns a thread
   __shared__ float sums[8][CT * E + 1];
   const int tx = threadIdx.x % CT, ty = threadIdx.x / CT;
   int64_t r0 = (int64_t)blockIdx.x * kDzRows, r1 = min(M, r0 + kDzRows);
@@ -194,26 +194,28 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
     r0 = m.y;
     r1 = m.z;
   }
-  const int c = ((int)blockIdx.y * CT + tx) * E;
+  const int c = ((int)blockIdx.y * CT + tx) * E, inside = n - c;
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (c < n) {
+  if (inside > 0) {
+#pragma unroll 2
     for (int64_t r = r0 + ty; r < r1; r += 8) {
       float v[E], o[E];
       if (g < 0) {
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.f;
-        if (dres != nullptr) store_vec<T, E>(dres + r * lddres + c, o);
+        if (dres != nullptr) store_any<false, T, E>(dres + r * lddres + c, inside, o);
         continue;
       }
-      load_vec<T, E>(dy + r * lddy + c, v);
-      if (dres != nullptr) store_vec<T, E>(dres + r * lddres + c, v);
+      load_any<T, E>(dy + r * lddy + c, inside, v);
+      if (dres != nullptr) store_any<false, T, E>(dres + r * lddres + c, inside, v);
       if (d != nullptr) {
-        load_vec<typename Deriv<T>::type, E>(d + r * ldd + c, o);
+        load_any<typename Deriv<T>::type, E>(d + r * ldd + c, inside, o);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] *= o[e];
-        if (dz != nullptr) store_vec<T, E>(dz + r * lddz + c, v);
+        // rows of dz end on 16 bytes, with zeros behind column n
+        if (dz != nullptr) store_any<false, T, E>(dz + r * lddz + c, (int)(lddz - c), v);
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] += v[e];
@@ -231,6 +233,32 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
       for (int k = 0; k < 8; ++k) s += sums[k][i];
       part[(int64_t)blockIdx.x * n + col] = s;
     }
+  }
+}
+
+// ---- rows copied to a pitch of whole 16 bytes, zeros behind their end ------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t group, int64_t per_group, int64_t rows,
+                                                       int width, int pieces, T* __restrict__ dst) {
+  constexpr int PER = 16 / (int)sizeof(T);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / pieces, g = r / per_group;
+    const int c = (int)(i - r * pieces) * PER, inside = width - c;
+    const T* p = src + g * group + (r - g * per_group) * ld + c;
+    union {
+      u32x4 u;
+      T t[PER];
+    } q;
+    if (inside >= PER) {
+      const u32x4_anywhere v = *reinterpret_cast<const u32x4_anywhere*>(p);
+      q.u = u32x4{v[0], v[1], v[2], v[3]};
+    } else {
+      q.u = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (e < inside) q.t[e] = p[e];
+    }
+    reinterpret_cast<u32x4*>(dst)[i] = q.u;
   }
 }
 
@@ -512,22 +540,38 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
 
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
+// Which operands lie on 16 bytes, or will after they are copied there
+struct Ways {
+  bool fwd, dx, dw;            // the products may load straight into LDS
+  bool copy_fwd, copy_bwd;     // operands that do not lie so are copied first
+};
+
 struct DensePlan {
   GemmPlan fwd, dx, dw;
   bool grouped;
-  int64_t dz_tiles;
+  int64_t dz_tiles, Kp, np;    // pitches of whole 16 bytes
   // byte offsets of the workspace's parts
-  size_t fwd_map, fwd_slab, fwd_bytes;
+  size_t fwd_map, fwd_slab, fwd_x, fwd_w, fwd_bytes, bwd_x, bwd_w;
   size_t dz_map, dz_first, dx_map, dw_map, dw_sums, dw_count, part, dz, slab, db_slab, bwd_bytes;
 };
 
-static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, bool direct) {
+// Copying pays where the products are large: through registers they run at 0.3 PFLOP/s where straight loads reach 0.65
+// (dW: 0.17 against 0.75; 32768 x 1023 -> 1021 in bf16: 225 / 267 / 399 us forward, dx, dW through registers, 107 / 90 / 90
+// from rows of 1024, 30 us for the copy), and cost a launch and two passes over the operand.
+static bool copy_pays(double flops_fwd, double flops_bwd, int e, int64_t M, int64_t Kp, int64_t weights) {
+  return flops_fwd * 1.7e-9 + flops_bwd * 3.1e-9 > 10.0 + 2.0 * e * ((double)M * Kp + (double)weights * Kp) / 4.7e6;
+}
+
+static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, const Ways& ways) {
   DensePlan p;
-  const int e = dtype_bytes(dtype);
+  const int e = dtype_bytes(dtype), per = 16 / e;
+  const int64_t weights = n * (G > 0 ? G : 1);
   p.grouped = G > 0;
-  p.fwd = gemm_plan(kFwd, dtype, M, n, K, p.grouped, G, direct);
-  p.dx = gemm_plan(kDx, dtype, M, K, n, p.grouped, G, direct);
-  p.dw = gemm_plan(kDw, dtype, n, K, M, p.grouped, G, direct);
+  p.Kp = (K + per - 1) / per * per;
+  p.np = (n + per - 1) / per * per;
+  p.fwd = gemm_plan(kFwd, dtype, M, n, K, p.grouped, G, ways.fwd);
+  p.dx = gemm_plan(kDx, dtype, M, K, n, p.grouped, G, ways.dx);
+  p.dw = gemm_plan(kDw, dtype, n, K, M, p.grouped, G, ways.dw);
   p.dz_tiles = ceil_div(M, kDzRows) + (p.grouped ? G + 2 : 0);
   const bool vector = !p.grouped && M <= kGemvRows;
   size_t at = 0;
@@ -538,6 +582,8 @@ static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, b
   };
   p.fwd_map = take(p.grouped ? p.fwd.row_tiles * sizeof(int4) : 0);
   p.fwd_slab = take(vector ? 0 : p.fwd.slab);
+  p.fwd_x = take(ways.copy_fwd ? (size_t)M * p.Kp * e : 0);
+  p.fwd_w = take(ways.copy_fwd ? (size_t)weights * p.Kp * e : 0);
   p.fwd_bytes = at;
   at = 0;
   p.dz_map = take(p.grouped ? p.dz_tiles * sizeof(int4) : 0);
@@ -547,19 +593,35 @@ static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, b
   p.dw_sums = take((size_t)p.dw.parts / 2 * sizeof(int4));
   p.dw_count = take(p.grouped ? 8 : 0);
   p.part = take((size_t)p.dz_tiles * n * 4);
-  p.dz = take((size_t)M * n * e);
+  p.dz = take((size_t)M * p.np * e);
   p.slab = take(std::max(p.dx.slab, p.dw.slab));
   p.db_slab = take((size_t)(p.grouped ? p.dw.parts : p.dw.splits > 1 ? p.dw.splits : 0) * n * 4);
+  p.bwd_x = take(ways.copy_bwd ? (size_t)M * p.Kp * e : 0);
+  p.bwd_w = take(ways.copy_bwd ? (size_t)weights * p.Kp * e : 0);
   p.bwd_bytes = at;
   return p;
+}
+
+template <typename T>
+static void pad_rows(const void* src, int64_t ld, int64_t group, int64_t per_group, int64_t rows, int64_t width, int64_t pitch, void* dst,
+                     hipStream_t s) {
+  const int pieces = (int)(pitch * sizeof(T) / 16);
+  pad_rows_kernel<T><<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows * pieces, 256), 8192)), 256, 0, s>>>(
+      (const T*)src, ld, group, per_group, rows, (int)width, pieces, (T*)dst);
+}
+
+static void pad_rows(int dtype, const void* src, int64_t ld, int64_t group, int64_t per_group, int64_t rows, int64_t width, int64_t pitch,
+                     void* dst, hipStream_t s) {
+  if (dtype_bytes(dtype) == 4)
+    pad_rows<uint32_t>(src, ld, group, per_group, rows, width, pitch, dst, s);
+  else
+    pad_rows<uint16_t>(src, ld, group, per_group, rows, width, pitch, dst, s);
 }
 
 // Every row of the operand starts on 16 bytes and its contiguous extent is whole pieces of them.
 static bool aligned(const void* p, int64_t ld, int64_t group, int64_t extent, int e) {
   return (((uint64_t)(uintptr_t)p | (uint64_t)(ld * e) | (uint64_t)(group * e) | (uint64_t)(extent * e)) & 15) == 0;
 }
-
-static bool wide(const void* p, int64_t ld, int e) { return p == nullptr || ((uintptr_t)p % 16 == 0 && ld * e % 16 == 0); }
 
 static int run_gemm(int kind, int dtype, const GemmPlan& p, bool direct, GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s) {
   a.row_tiles = (int)p.row_tiles;
@@ -584,16 +646,8 @@ static unsigned flat_grid(int64_t elems) { return (unsigned)std::max<int64_t>(1,
 template <typename T>
 static void launch_dz(const T* dy, int64_t lddy, const void* d, int64_t ldd, const int4* map, int64_t M, int n, int64_t tiles, T* dz,
                       int64_t lddz, T* dres, int64_t lddres, float* part, hipStream_t s) {
-  typedef typename Deriv<T>::type DT;
-  const DT* dd = (const DT*)d;
-  const int e = (int)sizeof(T), de = (int)sizeof(DT);
-  const bool vec = n % 8 == 0 && wide(dy, lddy, e) && wide(dz, lddz, e) && wide(dres, lddres, e) && wide(d, ldd, de);
-  if (vec)
-    dz_kernel<T, 8><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 256)), 256, 0, s>>>(dy, lddy, dd, ldd, map, M, n, dz, lddz, dres,
-                                                                                       lddres, part);
-  else
-    dz_kernel<T, 1><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 32)), 256, 0, s>>>(dy, lddy, dd, ldd, map, M, n, dz, lddz, dres,
-                                                                                      lddres, part);
+  dz_kernel<T><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 256)), 256, 0, s>>>(dy, lddy, (const typename Deriv<T>::type*)d, ldd, map, M, n,
+                                                                                 dz, lddz, dres, lddres, part);
 }
 
 template <typename T>
@@ -628,6 +682,16 @@ static bool pitch_fits(int64_t ld, int64_t width, int dtype) {
   return ld >= width && ld * dtype_bytes(dtype) <= kMaxPitchBytes;
 }
 
+static bool copies_fwd(int dtype, int64_t M, int64_t K, int64_t n, int G) {
+  const int per = 16 / dtype_bytes(dtype);
+  return copy_pays(2.0 * M * K * n, 0, 16 / per, M, (K + per - 1) / per * per, n * (G > 0 ? G : 1));
+}
+
+static bool copies_bwd(int dtype, int64_t M, int64_t K, int64_t n, int G) {
+  const int per = 16 / dtype_bytes(dtype);
+  return copy_pays(0, 4.0 * M * K * n, 16 / per, M, (K + n + 2 * per - 1) / per * per, n * (G > 0 ? G : 1));
+}
+
 }  // namespace bnpvi
 
 using namespace bnpvi;
@@ -638,9 +702,14 @@ int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G,
   if (dtype_bytes(dtype) == 0 || M < 0 || M > INT32_MAX || K < 1 || K > (1 << 20) || n < 1 || n > (1 << 20) || G < 0 ||
       G > kSortMaxLeaves)
     return -1;
-  // enough for either way of loading: which one it is goes by the addresses of the call
-  const DensePlan p = dense_plan(dtype, M, K, n, G, true), q = dense_plan(dtype, M, K, n, G, false);
-  return (int64_t)(backward ? std::max(p.bwd_bytes, q.bwd_bytes) : std::max(p.fwd_bytes, q.fwd_bytes));
+  // enough for every way of loading: which one it is goes by the addresses of the call
+  const bool cf = copies_fwd(dtype, M, K, n, G), cb = copies_bwd(dtype, M, K, n, G);
+  size_t most = 0;
+  for (int i = 0; i < 8; ++i) {
+    const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{(i & 1) != 0, (i & 2) != 0, (i & 4) != 0, cf, cb});
+    most = std::max(most, backward ? p.bwd_bytes : p.fwd_bytes);
+  }
+  return (int64_t)most;
 }
 
 int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const void* bias,
@@ -655,9 +724,10 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
                 (long long)n);
   if (M == 0) return BNPVI_OK;
   BNPVI_REQUIRE(x && w && y, "bnpvi_dense: NULL device pointer");
-  const int e = dtype_bytes(dtype), de = dtype == BNPVI_BF16 ? 2 : 4;
-  const bool direct = aligned(x, ldx, 0, K, e) && aligned(w, ldw, G > 1 ? w_group : 0, K, e);
-  const DensePlan p = dense_plan(dtype, M, K, n, G, direct);
+  const int e = dtype_bytes(dtype);
+  const bool x_lies = aligned(x, ldx, 0, K, e), w_lies = aligned(w, ldw, G > 1 ? w_group : 0, K, e);
+  const bool copy = !(x_lies && w_lies) && copies_fwd(dtype, M, K, n, G), direct = copy || (x_lies && w_lies);
+  const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{direct, true, true, copy, false});
   BNPVI_REQUIRE(work_bytes >= (int64_t)p.fwd_bytes && (p.fwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
                 "bnpvi_dense: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes, (long long)p.fwd_bytes);
   OnDevice on(ctx->device);
@@ -683,8 +753,6 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
   a.dact = dact;
   a.lddact = lddact;
   a.act = activation;
-  a.cvec = wide(y, ldy, e) && wide(residual, ldres, e) && wide(dact, lddact, de) && (dact == nullptr || de == 4 || lddact % 8 == 0) &&
-           (e == 4 || ldy % 8 == 0);
   if (G == 0 && M <= kGemvRows) {
     if (dtype == BNPVI_F32)
       gemv<float>(a, s);
@@ -709,6 +777,21 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
     a.map = (const int4*)(wk + p.fwd_map);
   }
   if (p.fwd.slab) a.slab = (float*)(wk + p.fwd_slab);
+  if (copy) {
+    const int64_t groups = G > 0 ? G : 1;
+    if (!x_lies) {
+      pad_rows(dtype, x, ldx, 0, M, M, K, p.Kp, wk + p.fwd_x, s);
+      a.R = wk + p.fwd_x;
+      a.ldr = p.Kp;
+    }
+    if (!w_lies) {
+      pad_rows(dtype, w, ldw, w_group, n, groups * n, K, p.Kp, wk + p.fwd_w, s);
+      a.S = wk + p.fwd_w;
+      a.lds = p.Kp;
+      a.s_group = G > 1 ? n * p.Kp : 0;
+    }
+    BNPVI_LAUNCH_CHECK();
+  }
   const int r = run_gemm(kFwd, dtype, p.fwd, direct, a, ctx, s);
   if (r) return r;
   if (p.fwd.slab) {
@@ -734,10 +817,12 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
                     (!dw || pitch_fits(ldx, K, dtype)) && (!dres || lddres >= n),
                 "bnpvi_dense_backward: a row pitch is below its width, or above 4 MiB");
   const int e = dtype_bytes(dtype);
-  // dz is dy, or lies in the workspace with rows of n
-  const bool direct = (dact ? n * e % 16 == 0 : aligned(dy, lddy, 0, n, e)) && (!dx || aligned(w, ldw, G > 1 ? w_group : 0, K, e)) &&
-                      (!dw || aligned(x, ldx, 0, K, e));
-  const DensePlan p = dense_plan(dtype, M, K, n, G, direct);
+  // dz is dy, or lies in the workspace in rows of whole 16 bytes
+  const bool dz_lies = dact != nullptr || aligned(dy, lddy, 0, n, e);
+  const bool w_lies = !dx || aligned(w, ldw, G > 1 ? w_group : 0, K, e), x_lies = !dw || aligned(x, ldx, 0, K, e);
+  const bool copy = M > 0 && (dx || dw) && !(dz_lies && w_lies && x_lies) && copies_bwd(dtype, M, K, n, G);
+  const Ways ways = {true, copy || (dz_lies && w_lies), copy || (dz_lies && x_lies), false, copy};
+  const DensePlan p = dense_plan(dtype, M, K, n, G, ways);
   BNPVI_REQUIRE(work_bytes >= (int64_t)p.bwd_bytes && (p.bwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
                 "bnpvi_dense_backward: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes,
                 (long long)p.bwd_bytes);
@@ -791,16 +876,16 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   if (need_dz && !none) {
     void* out = dact ? (void*)(wk + p.dz) : nullptr;
     if (dtype == BNPVI_F32)
-      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, n, (float*)dres, lddres, part, s);
+      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, p.np, (float*)dres, lddres, part, s);
     else if (dtype == BNPVI_BF16)
-      launch_dz<bf16_t>((const bf16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (bf16_t*)out, n, (bf16_t*)dres, lddres, part,
+      launch_dz<bf16_t>((const bf16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (bf16_t*)out, p.np, (bf16_t*)dres, lddres, part,
                         s);
     else
-      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, n, (f16_t*)dres, lddres, part, s);
+      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, p.np, (f16_t*)dres, lddres, part, s);
     BNPVI_LAUNCH_CHECK();
     if (dact) {
       dz = out;
-      lddz = n;
+      lddz = p.np;
     }
   }
   if (db && !db_in_dw) {
@@ -813,23 +898,44 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
       launch_db<f16_t>(part, first, tiles, (int)n, groups, db, s);
     BNPVI_LAUNCH_CHECK();
   }
+  const int64_t wg = G > 1 ? w_group : 0;
+  const void *xs = x, *ws = w;
+  int64_t ldxs = ldx, ldws = ldw, wgs = wg;
+  if (copy) {
+    if (!dz_lies) {
+      pad_rows(dtype, dy, lddy, 0, M, M, n, p.np, wk + p.dz, s);
+      dz = wk + p.dz;
+      lddz = p.np;
+    }
+    if (!w_lies) {
+      pad_rows(dtype, w, ldw, w_group, n, groups * n, K, p.Kp, wk + p.bwd_w, s);
+      ws = wk + p.bwd_w;
+      ldws = p.Kp;
+      wgs = G > 1 ? n * p.Kp : 0;
+    }
+    if (!x_lies) {
+      pad_rows(dtype, x, ldx, 0, M, M, K, p.Kp, wk + p.bwd_x, s);
+      xs = wk + p.bwd_x;
+      ldxs = p.Kp;
+    }
+    BNPVI_LAUNCH_CHECK();
+  }
   if (dx && !none) {
     GemmArgs a = {};
     a.R = dz;
     a.ldr = lddz;
-    a.S = w;
-    a.lds = ldw;
-    a.s_group = G > 1 ? w_group : 0;
+    a.S = ws;
+    a.lds = ldws;
+    a.s_group = wgs;
     a.rows = M;
     a.cols = K;
     a.K = n;
     a.G = G;
     a.C = dx;
     a.ldc = lddx;
-    a.cvec = wide(dx, lddx, e);
     if (G > 0) a.map = (const int4*)(wk + p.dx_map);
     if (p.dx.slab) a.slab = (float*)(wk + p.slab);
-    r = run_gemm(kDx, dtype, p.dx, direct, a, ctx, s);
+    r = run_gemm(kDx, dtype, p.dx, ways.dx, a, ctx, s);
     if (r) return r;
     if (p.dx.slab) {
       // no epilogue: a plain sum over the splits into rows of pitch lddx
@@ -849,8 +955,8 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     GemmArgs a = {};
     a.R = dz;
     a.ldr = lddz;
-    a.S = x;
-    a.lds = ldx;
+    a.S = xs;
+    a.lds = ldxs;
     a.rows = n;
     a.cols = K;
     a.K = M;
@@ -863,13 +969,12 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.C = dw;
     a.ldc = K;
     a.c_group = n * K;
-    a.cvec = wide(dw, K, e) && (groups == 1 || n * K * e % 16 == 0);
     if (p.dw.slab) a.slab = (float*)(wk + p.slab);
     if (db_in_dw) {
       a.db = db;
       if (p.dw.slab) a.db_slab = (float*)(wk + p.db_slab);
     }
-    r = run_gemm(kDw, dtype, p.dw, direct, a, ctx, s);
+    r = run_gemm(kDw, dtype, p.dw, ways.dw, a, ctx, s);
     if (r) return r;
     if (p.dw.slab) {
       const int4* sums = (const int4*)(wk + p.dw_sums);

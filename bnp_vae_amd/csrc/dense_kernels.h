@@ -56,7 +56,6 @@ struct GemmArgs {
   int entries;                 // at most
   int G, splits;
   int row_tiles, col_tiles;
-  int cvec;                    // C, residual and derivative take 16-byte accesses
   void* C;
   int64_t ldc;
   const void* bias;
@@ -633,15 +632,12 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
     const int c = lane % LPR, cl = wc + 8 * c;
     const int64_t col = t.col0 + cl;
     const int left = t.nc - cl < 8 ? t.nc - cl : 8;
-    const bool vec = a.cvec && left == 8;
     float b[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) b[e] = 0.f;
     if (KIND == kFwd && a.bias != nullptr && a.slab == nullptr && t.g >= 0) {
       const T* bp = reinterpret_cast<const T*>(a.bias) + t.g * a.bias_group + col;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) b[e] = (float)bp[e];
+      load_any<T, 8>(bp, left, b);
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wave is done reading the stages
 #pragma unroll
@@ -667,8 +663,8 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
             if (rl >= t.nr || left <= 0) continue;
             const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * (WC * 2) + ((c ^ (r & (WC / 8 - 1))) << 4));
             T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? t.g * a.c_group : 0) + (t.row0 + rl) * a.ldc + col;
-            if (vec) {
-              __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out));
+            if (left == 8) {
+              __builtin_nontemporal_store((u32x4_anywhere)v, reinterpret_cast<u32x4_anywhere*>(out));
             } else {
               union {
                 u32x4 u;
@@ -727,13 +723,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
           if (t.g >= 0) {
             if (a.res != nullptr) {
               const T* rp = reinterpret_cast<const T*>(a.res) + row * a.ldres + col;
-              if (vec) {
-                load_vec<T, 8>(rp, q);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (e < left) q[e] = (float)rp[e];
-              }
+              load_any<T, 8>(rp, left, q);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += b[e];
@@ -743,26 +733,14 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
           }
           if (a.dact != nullptr) {
             DT* dp = reinterpret_cast<DT*>(a.dact) + row * a.lddact + col;
-            if (vec) {
-              store_stream<DT, 8>(dp, d);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (e < left) dp[e] = (DT)d[e];
-            }
+            store_any<true, DT, 8>(dp, left, d);
           }
         }
-        if (vec) {
-          store_stream<T, 8>(out, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < left) out[e] = (T)v[e];
-        }
+        store_any<true, T, 8>(out, left, v);
       }
     }
     // a full tile in 16-byte pieces: the number of its stores is known
-    behind = a.cvec && a.slab == nullptr && t.nr == BR && t.nc == BC ? (KIND == kFwd && a.dact != nullptr ? 2 : 1) : 0;
+    behind = a.slab == nullptr && t.nr == BR && t.nc == BC ? (KIND == kFwd && a.dact != nullptr ? 2 : 1) : 0;
   }
   if constexpr (DIRECT) wait_loads<0>();         // the zeros behind the last tile: nothing may write into the next workgroup's LDS
 }

@@ -74,18 +74,46 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[E]) {
   *reinterpret_cast<vec*>(p) = q;
 }
 
-// the same past the caches' reuse order: results that are as large as the caches and written once
+// E elements anywhere in memory, the first `inside` of them (the others are 0, or not written).  Global loads and stores
+// of 16 bytes take any address.
 template <typename T, int E>
-__device__ __forceinline__ void store_stream(T* p, const float (&v)[E]) {
-  typedef T vec __attribute__((ext_vector_type(E)));
+__device__ __forceinline__ void load_any(const T* p, int inside, float (&v)[E]) {
   union {
-    vec t;
-    u32x4 u[sizeof(vec) / 16];
+    u32x4_anywhere u[E * sizeof(T) / 16];
+    T t[E];
+  } q;
+  if (inside >= E) {
+#pragma unroll
+    for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) q.u[i] = reinterpret_cast<const u32x4_anywhere*>(p)[i];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = (float)q.t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e < inside ? (float)p[e] : 0.f;
+  }
+}
+// STREAM: past the caches' reuse order, for results as large as the caches that are written once
+template <bool STREAM, typename T, int E>
+__device__ __forceinline__ void store_any(T* p, int inside, const float (&v)[E]) {
+  union {
+    u32x4_anywhere u[E * sizeof(T) / 16];
+    T t[E];
   } q;
 #pragma unroll
   for (int e = 0; e < E; ++e) q.t[e] = (T)v[e];
+  if (inside >= E) {
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(vec) / 16); ++i) __builtin_nontemporal_store(q.u[i], reinterpret_cast<u32x4*>(p) + i);
+    for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) {
+      if (STREAM)
+        __builtin_nontemporal_store(q.u[i], reinterpret_cast<u32x4_anywhere*>(p) + i);
+      else
+        reinterpret_cast<u32x4_anywhere*>(p)[i] = q.u[i];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e < inside) p[e] = q.t[e];
+  }
 }
 
 // The value another lane of the same 16 holds (data-parallel primitive `CTRL`); all lanes take part.
