@@ -404,6 +404,67 @@ def test_dense_shapes_around_a_row(layers):
     assert empty.shape == (0, 5, 16)
 
 
+@pytest.mark.parametrize("sizes", [None, [9, 0, 20]])
+@pytest.mark.parametrize("have", ["", "b", "r", "br"])
+def test_dense_gradients_of_some_inputs(layers, have, sizes):
+    """Each input alone, and asked for alone of a pass that could give all: the bits of the pass that gives all."""
+    M, K, n = 33, 40, 24
+    shape = (n,) if sizes is None else (3, n)
+    t = {"x": gpu(rand((M, K), torch.bfloat16, 1)), "w": gpu(rand(shape + (K,), torch.bfloat16, 2, 0.2))}
+    if "b" in have:
+        t["b"] = gpu(rand(shape, torch.bfloat16, 3))
+    if "r" in have:
+        t["r"] = gpu(rand((M, n), torch.bfloat16, 4))
+    off = None if sizes is None else torch.tensor([0, 9, 9, 29], dtype=torch.int32, device="cuda")
+    dy = gpu(rand((M, n), torch.bfloat16, 5))
+
+    def run(names):
+        leaves = {a: v.clone().requires_grad_(a in names) for a, v in t.items()}
+        return leaves, layers.dense(leaves["x"], leaves["w"], leaves.get("b"), "tanh", leaves.get("r"), off)
+    leaves, y = run(set(t))
+    want = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)))
+    for name in t:
+        got, = torch.autograd.grad(y, [leaves[name]], dy, retain_graph=True)
+        assert torch.equal(got, want[name]), name
+        alone, out = run({name})
+        got, = torch.autograd.grad(out, [alone[name]], dy)
+        assert torch.equal(got, want[name]) and torch.equal(out, y), name
+
+
+def test_combine_gradients_of_some_inputs(layers):
+    plan = layers.sort_by_leaf(torch.randint(-1, 5, (50, 2), device="cuda", generator=torch.Generator("cuda").manual_seed(1)), 5)
+    rows, w = gpu(rand((100, 36), torch.float32, 1)), gpu(rand((50, 2), torch.float32, 2))
+    dy = gpu(rand((50, 36), torch.float32, 3))
+    both = [rows.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+    want = torch.autograd.grad(layers.combine(both[0], plan, both[1]), both, dy)
+    a = rows.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(layers.combine(a, plan, w), [a], dy)[0], want[0])
+    b = w.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(layers.combine(rows, plan, b), [b], dy)[0], want[1])
+
+
+def test_a_second_differentiation_is_an_error(layers):
+    x = gpu(rand((6, 8), torch.float32, 1)).requires_grad_(True)
+    w = gpu(rand((5, 8), torch.float32, 2)).requires_grad_(True)
+    plan = layers.sort_by_leaf(torch.zeros(6, dtype=torch.int32, device="cuda"), 1)
+    phi = torch.rand((6, 4), device="cuda").requires_grad_(True)
+    passes = [(layers.dense(x, w, activation="tanh"), x), (layers.dispatch(x, plan), x), (layers.combine(x, plan), x),
+              (layers.combine(x, plan, torch.ones((6, 1), device="cuda")), x), (layers.top_leaves(phi, 2)[1], phi)]
+    for out, leaf in passes:
+        d, = torch.autograd.grad((out * out).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            torch.autograd.grad(d.sum() + leaf.sum(), leaf)
+
+
+def test_an_input_changed_before_the_backward_pass_is_an_error(layers):
+    x = gpu(rand((6, 8), torch.float32, 1))
+    w = gpu(rand((5, 8), torch.float32, 2)).requires_grad_(True)
+    y = layers.dense(x, w)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+
+
 @pytest.mark.parametrize("G", [0, 3])
 def test_dense_without_rows(layers, G):
     w = gpu(rand((G, 8, 16) if G else (8, 16), torch.float32, 1)).requires_grad_(True)

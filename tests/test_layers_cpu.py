@@ -98,3 +98,13 @@ def test_library_refuses_dense():
     _fails(backward(lddy=5), "pitch")
     _fails(backward(size=0), "workspace")
     _fails(backward(dy=None), "NULL")
+
+
+def test_views_whose_memory_is_not_their_value_are_refused():
+    negated = torch.zeros((4, 8), dtype=torch.complex64).conj().imag
+    assert negated.is_neg()
+    for t in (negated, torch.eye(4).to_sparse()):
+        with pytest.raises(TypeError, match="dense tensor"):
+            layers.top_leaves(t, 1)
+        with pytest.raises(TypeError, match="dense tensor"):
+            layers.dense(t, torch.zeros((3, 8)))
