@@ -479,12 +479,14 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
     tile_size(tile, br, bc);
     return (ceil_div(rows, br) + (by_rows ? G / 2 : 0)) * ceil_div(cols, bc);
   };
+  // whole turns of a full chip and one of what is left, which has the CUs to itself
   auto cost = [&](int tile, int64_t s) {
     const int r = row_of(tile);
-    const int64_t n = tiles_of(tile) * s;
-    const int each = (int)std::min<int64_t>(kPerCu[r], std::max<int64_t>(1, ceil_div(n, kNumCU)));
-    const double turns = (double)ceil_div(n, (int64_t)each * kNumCU), stage = (e == 4 ? k32 : k16)[r][each - 1] * (r == 2 ? 1.0 + 0.08 * kind : 1.0);
-    return turns * ((double)ceil_div(stages, s) * stage + kTileCost[r]) + (s > 1 ? 4.0 + 8.0 * s * rows * cols / 4.0e6 : 0.0);
+    const int64_t n = tiles_of(tile) * s, whole = n / (kPerCu[r] * kNumCU), rest = ceil_div(n % (kPerCu[r] * kNumCU), kNumCU);
+    auto turn = [&](int64_t each) {
+      return (double)ceil_div(stages, s) * (e == 4 ? k32 : k16)[r][each - 1] * (r == 2 ? 1.0 + 0.08 * kind : 1.0) + kTileCost[r];
+    };
+    return whole * turn(kPerCu[r]) + (rest ? turn(rest) : 0.0) + (s > 1 ? 4.0 + 8.0 * s * rows * cols / 4.0e6 : 0.0);
   };
   // groups of the sum, `len` stages a piece: the work, the pieces' first loads and epilogues, half a piece at the end, the
   // parts -- nearly all pieces where they are shorter than a leaf is on average, else those of the long leaves
