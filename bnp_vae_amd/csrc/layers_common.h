@@ -16,8 +16,8 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_anywhere __attribute__((ext_vector_type(4), aligned(2)));      // global loads take any address
+typedef uint32_t u32_anywhere __attribute__((aligned(2)));
 
 inline int dtype_bytes(int dtype) { return dtype == BNPVI_F32 ? 4 : dtype == BNPVI_BF16 || dtype == BNPVI_F16 ? 2 : 0; }
 
@@ -57,21 +57,34 @@ class LdsLimit {
   std::atomic<uint64_t> done_{0};
 };
 
-// E elements of T at an address that is a multiple of their size, as fp32; and back with one rounding to nearest even.
+// E elements of T -- 16 bytes at any address, or one element -- as fp32; and back with one rounding to nearest even.
 template <typename T, int E>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[E]) {
-  typedef T vec __attribute__((ext_vector_type(E)));
-  const vec q = *reinterpret_cast<const vec*>(p);
+__device__ __forceinline__ void load_piece(const T* p, float (&v)[E]) {
+  if constexpr (E == 1) {
+    v[0] = (float)*p;
+  } else {
+    union {
+      u32x4_anywhere u;
+      T t[E];
+    } q;
+    q.u = *reinterpret_cast<const u32x4_anywhere*>(p);
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = (float)q[e];
+    for (int e = 0; e < E; ++e) v[e] = (float)q.t[e];
+  }
 }
 template <typename T, int E>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[E]) {
-  typedef T vec __attribute__((ext_vector_type(E)));
-  vec q;
+__device__ __forceinline__ void store_piece(T* p, const float (&v)[E]) {
+  if constexpr (E == 1) {
+    *p = (T)v[0];
+  } else {
+    union {
+      u32x4_anywhere u;
+      T t[E];
+    } q;
 #pragma unroll
-  for (int e = 0; e < E; ++e) q[e] = (T)v[e];
-  *reinterpret_cast<vec*>(p) = q;
+    for (int e = 0; e < E; ++e) q.t[e] = (T)v[e];
+    *reinterpret_cast<u32x4_anywhere*>(p) = q.u;
+  }
 }
 
 // E elements anywhere in memory, the first `inside` of them (the others are 0, or not written).  Global loads and stores

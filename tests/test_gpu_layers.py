@@ -200,7 +200,8 @@ def exchange_reference(x, ys, leaf, w, L):
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("N,k,D,L", [(1, 1, 1, 1), (5, 2, 3, 4), (64, 1, 32, 25), (33, 3, 100, 7), (130, 2, 256, 64), (17, 4, 257, 5),
-                                     (9, 2, 1030, 3), (1000, 8, 6, 600), (0, 2, 8, 3)])
+                                     (9, 2, 1030, 3), (1000, 8, 6, 600), (0, 2, 8, 3),
+                                     (5000, 2, 37, 9), (4099, 3, 9, 40), (700, 2, 2, 3), (700, 2, 5, 3), (3000, 1, 7, 70), (2000, 5, 15, 7000)])
 def test_dispatch_and_combine(layers, dtype, N, k, D, L):
     T = TYPES[dtype]
     x, ys = rand((N, D), T, 1), rand((N * k, D), T, 2)
