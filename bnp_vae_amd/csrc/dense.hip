@@ -175,14 +175,15 @@ __global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
 
 // ---- dz, residual gradient, partial sums of the bias gradient --------------------------------------------------------
 // One workgroup: a row tile (of one group) x 256 columns.  dz = dy * d rounded once; the bias gradient adds the
-// unrounded products: per thread over its rows, then the eight row threads of a column in order.  dres (or nullptr):
-// dy, 0 in the rows of no group.
+// unrounded products: per thread over its rows, then the eight row threads of a column in order, into `part`, or into `db`
+// where one tile has all rows.  dres (or nullptr): dy, 0 in the rows of no group.
 constexpr int kDzRows = 128;
 
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64_t lddy, const typename Deriv<T>::type* __restrict__ d,
                                                  int64_t ldd, const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz,
-                                                 int64_t lddz, T* __restrict__ dres, int64_t lddres, float* __restrict__ part) {
+                                                 int64_t lddz, T* __restrict__ dres, int64_t lddres, float* __restrict__ part,
+                                                 T* __restrict__ db) {
   constexpr int CT = 32, E = 8;              // threads across, columns a thread
   __shared__ float sums[8][CT * E + 1];
   const int tx = threadIdx.x % CT, ty = threadIdx.x / CT;
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
       for (int e = 0; e < E; ++e) acc[e] += v[e];
     }
   }
-  if (part == nullptr) return;
+  if (part == nullptr && db == nullptr) return;
 #pragma unroll
   for (int e = 0; e < E; ++e) sums[ty][tx * E + e] = acc[e];
   __syncthreads();
@@ -231,7 +232,10 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += sums[k][i];
-      part[(int64_t)blockIdx.x * n + col] = s;
+      if (db != nullptr)
+        db[col] = (T)s;
+      else
+        part[(int64_t)blockIdx.x * n + col] = s;
     }
   }
 }
@@ -283,28 +287,38 @@ __global__ __launch_bounds__(1024) void db_kernel(const float* __restrict__ part
   }
 }
 
-// ---- sums over the splits of the reduce axis, in order -------------------------------------------------------------
+// ---- sums over the splits of the reduce axis, in order, of dW and behind it of db ---------------------------------------
+struct SumArgs {
+  const float* slab[2];
+  void* out[2];
+  int64_t elems[2];
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict__ slab, int splits, int64_t elems, T* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void split_sum_kernel(const SumArgs a, int splits) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.elems[0] + a.elems[1]; i += (int64_t)gridDim.x * 256) {
+    const bool two = i >= a.elems[0];
+    const int64_t elems = a.elems[two], e = two ? i - a.elems[0] : i;
+    const float* p = a.slab[two] + e;
     float s = 0.f;
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) s += slab[k * elems + i];
-    out[i] = (T)s;
+    for (int k = 0; k < splits; ++k) s += p[k * elems];
+    reinterpret_cast<T*>(a.out[two])[e] = (T)s;
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void piece_sum_kernel(const float* __restrict__ slab, const int4* __restrict__ sums,
-                                                        const int32_t* __restrict__ count, int64_t elems, T* __restrict__ out) {
-  for (int i = blockIdx.y; i < count[1]; i += gridDim.y) {
-    const int4 m = sums[i];
-    const float* p = slab + m.y * elems;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < elems; e += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void piece_sum_kernel(const SumArgs a, const int4* __restrict__ sums, const int32_t* __restrict__ count) {
+  for (int g = blockIdx.y; g < count[1]; g += gridDim.y) {
+    const int4 m = sums[g];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.elems[0] + a.elems[1]; i += (int64_t)gridDim.x * 256) {
+      const bool two = i >= a.elems[0];
+      const int64_t elems = a.elems[two], e = two ? i - a.elems[0] : i;
+      const float* p = a.slab[two] + m.y * elems + e;
       float s = 0.f;
 #pragma unroll 4
-      for (int k = 0; k < m.z; ++k) s += p[k * elems + e];
-      out[m.x * elems + e] = (T)s;
+      for (int k = 0; k < m.z; ++k) s += p[k * elems];
+      reinterpret_cast<T*>(a.out[two])[m.x * elems + e] = (T)s;
     }
   }
 }
@@ -647,9 +661,9 @@ static unsigned flat_grid(int64_t elems) { return (unsigned)std::max<int64_t>(1,
 
 template <typename T>
 static void launch_dz(const T* dy, int64_t lddy, const void* d, int64_t ldd, const int4* map, int64_t M, int n, int64_t tiles, T* dz,
-                      int64_t lddz, T* dres, int64_t lddres, float* part, hipStream_t s) {
+                      int64_t lddz, T* dres, int64_t lddres, float* part, void* db, hipStream_t s) {
   dz_kernel<T><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 256)), 256, 0, s>>>(dy, lddy, (const typename Deriv<T>::type*)d, ldd, map, M, n,
-                                                                                 dz, lddz, dres, lddres, part);
+                                                                                 dz, lddz, dres, lddres, part, (T*)db);
 }
 
 template <typename T>
@@ -658,14 +672,14 @@ static void launch_db(const float* part, const int32_t* first, int64_t tiles, in
 }
 
 template <typename T>
-static void launch_sums(const float* slab, const GemmPlan& p, bool grouped, const int4* sums, const int32_t* count, int64_t elems, void* out,
-                        hipStream_t s) {
+static void launch_sums(const SumArgs& a, const GemmPlan& p, bool grouped, const int4* sums, const int32_t* count, hipStream_t s) {
+  const int64_t elems = a.elems[0] + a.elems[1];
   if (grouped)
     piece_sum_kernel<T><<<dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(elems, 256), 1024)),
                                (unsigned)std::min<int64_t>(p.parts / 2, 64)),
-                          256, 0, s>>>(slab, sums, count, elems, (T*)out);
+                          256, 0, s>>>(a, sums, count);
   else
-    split_sum_kernel<T><<<flat_grid(elems), 256, 0, s>>>(slab, p.splits, elems, (T*)out);
+    split_sum_kernel<T><<<flat_grid(elems), 256, 0, s>>>(a, p.splits);
 }
 
 constexpr int64_t kMaxPitchBytes = int64_t(1) << 22;       // 256 rows of a tile stay below 2^31 bytes
@@ -838,9 +852,10 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   const int4* dz_map = nullptr;
   int32_t* first = nullptr;
   const bool none = M == 0;
-  // without an activation the products read dy itself and dW's kernel adds up its rows for the bias on the way
-  // (16385 x 64 -> 4096 fp32: 70 us of 450 were a pass over dy for that)
-  const bool db_in_dw = db && dw && !dact && p.dw.tile != kTile256;
+  // Without an activation the products read dy itself and dW's kernel adds up its rows for the bias on the way
+  // (16385 x 64 -> 4096 fp32: 70 us of 450 were a pass over dy for that).  With one, dz is rounded to 16 bits before dW's
+  // kernel sees it, so that there only fp32 does the same.
+  const bool db_in_dw = db && dw && (!dact || dtype == BNPVI_F32) && p.dw.tile != kTile256;
   const bool need_dz = (dact != nullptr && (dx || dw)) || (db && !db_in_dw) || dres;
   if (G > 0) {
     MapArgs m = {};
@@ -874,23 +889,25 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   }
   const void* dz = dy;
   int64_t lddz = lddy;
-  float* part = db && !db_in_dw ? (float*)(wk + p.part) : nullptr;
+  void* db_in_dz = db && !db_in_dw && G == 0 && p.dz_tiles == 1 && !none ? db : nullptr;          // a launch less
+  float* part = db && !db_in_dw && !db_in_dz ? (float*)(wk + p.part) : nullptr;
   if (need_dz && !none) {
     void* out = dact ? (void*)(wk + p.dz) : nullptr;
     if (dtype == BNPVI_F32)
-      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, p.np, (float*)dres, lddres, part, s);
+      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, p.np, (float*)dres, lddres, part, db_in_dz, s);
     else if (dtype == BNPVI_BF16)
       launch_dz<bf16_t>((const bf16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (bf16_t*)out, p.np, (bf16_t*)dres, lddres, part,
-                        s);
+                        db_in_dz, s);
     else
-      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, p.np, (f16_t*)dres, lddres, part, s);
+      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, p.np, (f16_t*)dres, lddres, part, db_in_dz,
+                       s);
     BNPVI_LAUNCH_CHECK();
     if (dact) {
       dz = out;
       lddz = p.np;
     }
   }
-  if (db && !db_in_dw) {
+  if (db && !db_in_dw && !db_in_dz) {
     const int64_t tiles = none ? 0 : p.dz_tiles;
     if (dtype == BNPVI_F32)
       launch_db<float>(part, first, tiles, (int)n, groups, db, s);
@@ -981,16 +998,13 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     if (p.dw.slab) {
       const int4* sums = (const int4*)(wk + p.dw_sums);
       const int32_t* count = (const int32_t*)(wk + p.dw_count);
-      auto add = [&](const float* slab, int64_t elems, void* out) {
-        if (dtype == BNPVI_F32)
-          launch_sums<float>(slab, p.dw, G > 0, sums, count, elems, out, s);
-        else if (dtype == BNPVI_BF16)
-          launch_sums<bf16_t>(slab, p.dw, G > 0, sums, count, elems, out, s);
-        else
-          launch_sums<f16_t>(slab, p.dw, G > 0, sums, count, elems, out, s);
-      };
-      add(a.slab, n * K, dw);
-      if (db_in_dw) add(a.db_slab, n, db);
+      const SumArgs b = {{a.slab, a.db_slab}, {dw, db}, {n * K, db_in_dw ? n : 0}};
+      if (dtype == BNPVI_F32)
+        launch_sums<float>(b, p.dw, G > 0, sums, count, s);
+      else if (dtype == BNPVI_BF16)
+        launch_sums<bf16_t>(b, p.dw, G > 0, sums, count, s);
+      else
+        launch_sums<f16_t>(b, p.dw, G > 0, sums, count, s);
       BNPVI_LAUNCH_CHECK();
     }
   }
