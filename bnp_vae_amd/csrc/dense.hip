@@ -84,60 +84,59 @@ __device__ void row_tiles(const int32_t* __restrict__ offsets, int G, int64_t M,
 // ---- pieces of the groups' sums (dW) ---------------------------------------------------------------------------------
 // Groups differ in length, and dW's tiles all have their group's: a group of more than `piece` frames is summed in pieces,
 // whose partial results lie in `part`s of their own and are added in order afterwards.  map[e] = {group, first frame, end
-// frame, part or -1}: the full pieces first, then the rest by quarters of a piece's length, so that the long ones start
-// first and every eighth entry -- one XCD's share -- is a like mixture.  sums[i] = {group, first part, parts} of the groups
-// in pieces; count = {entries, groups in pieces}.
+// frame, part or -1}, the longest first by 64ths of a piece, and every second eight of them backwards: every eighth entry --
+// one XCD's share -- is a like mixture.  (Entries of one 64th lie in any order; nothing is added in it.)  sums[i] = {group,
+// first part, parts} of the groups in pieces; count = {entries, groups in pieces}.
+constexpr int kLengths = 65;
+
 __device__ void sum_pieces(const int32_t* __restrict__ offsets, int G, int64_t M, int64_t piece, int entries, int most, int4* __restrict__ map,
-                           int4* __restrict__ sums, int32_t* __restrict__ count, int32_t* red) {
+                           int4* __restrict__ sums, int32_t* __restrict__ count, int32_t* at, int32_t* red) {
   const int t = threadIdx.x;
   const int per = (G + 1023) / 1024, g0 = min(G, t * per), g1 = min(G, g0 + per);
-  int32_t full = 0, parts = 0, split = 0, rest[4] = {0, 0, 0, 0};
-  auto look = [&](int g, int64_t& lo, int32_t& n, int64_t& left, int& quarter, bool& tail) {
+  int32_t parts = 0, split = 0;
+  auto look = [&](int g, int64_t& lo, int32_t& n, int64_t& left, int& shorter, bool& tail) {
     lo = clamp_row(offsets[g], 0, M);
     const int64_t len = clamp_row(offsets[g + 1], lo, M) - lo;
     n = (int32_t)(len / piece);
     left = len - n * piece;
     tail = left > 0 || len == 0;
-    quarter = 3 - (int)(4 * left / piece);
+    shorter = 64 - (int)(64 * left / piece);          // 0: a full piece
   };
   int64_t lo, left;
-  int32_t n;
-  int quarter;
+  int32_t n, used, all, unused;
+  int shorter;
   bool tail;
+  for (int i = t; i < kLengths; i += 1024) at[i] = 0;
+  __syncthreads();
   for (int g = g0; g < g1; ++g) {
-    look(g, lo, n, left, quarter, tail);
-    full += n;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) rest[q] += tail && quarter == q;
+    look(g, lo, n, left, shorter, tail);
+    if (n) atomicAdd(&at[0], n);
+    if (tail) atomicAdd(&at[shorter], 1);
     if (n + tail > 1) {
       parts += n + tail;
       ++split;
     }
   }
-  int32_t all, at_full = scan_threads(full, red, all), base = all, at_rest[4], unused;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    at_rest[q] = base + scan_threads(rest[q], red, all);
-    base += all;
-  }
+  __syncthreads();
+  const int32_t before = scan_threads(t < kLengths ? at[t] : 0, red, used);
+  if (t < kLengths) at[t] = before;
   int32_t at_part = scan_threads(parts, red, unused), at_split = scan_threads(split, red, all);
+  if ((uint32_t)used > (uint32_t)entries) used = entries;
   if (t == 0) {
-    count[0] = base < entries ? base : entries;
+    count[0] = used;
     count[1] = all < most ? all : most;
   }
+  auto put = [&](int32_t rank, const int4& m) {
+    const int32_t turn = rank >> 3, at_rank = (turn & 1) && 8 * turn + 8 <= used ? 8 * turn + 7 - (rank & 7) : rank;
+    if ((uint32_t)rank < (uint32_t)used) map[at_rank] = m;
+  };
   for (int g = g0; g < g1; ++g) {
-    look(g, lo, n, left, quarter, tail);
+    look(g, lo, n, left, shorter, tail);
     // the bounds hold wherever the offsets ascend; others are not followed out of the workspace
     const bool many = n + tail > 1 && (uint32_t)at_part < (uint32_t)(2 * most) && n + tail <= 2 * most - at_part;
-    for (int32_t i = 0; i < n; ++i, ++at_full)
-      if ((uint32_t)at_full < (uint32_t)entries) map[at_full] = int4{g, (int)(lo + i * piece), (int)(lo + (i + 1) * piece), many ? at_part + i : -1};
-    if (tail) {
-      int32_t at = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (quarter == q) at = at_rest[q]++;
-      if ((uint32_t)at < (uint32_t)entries) map[at] = int4{g, (int)(lo + n * piece), (int)(lo + n * piece + left), many ? at_part + n : -1};
-    }
+    int32_t rank = n ? atomicAdd(&at[0], n) : 0;
+    for (int32_t i = 0; i < n; ++i) put(rank + i, int4{g, (int)(lo + i * piece), (int)(lo + (i + 1) * piece), many ? at_part + i : -1});
+    if (tail) put(atomicAdd(&at[shorter], 1), int4{g, (int)(lo + n * piece), (int)(lo + n * piece + left), many ? at_part + n : -1});
     if (many) {
       if ((uint32_t)at_split < (uint32_t)most) sums[at_split] = int4{g, at_part, n + tail, 0};
       ++at_split;
@@ -163,13 +162,13 @@ struct MapArgs {
 };
 
 __global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
-  extern __shared__ int32_t start[];        // [G + 1] | [16]
-  int32_t* red = start + a.G + 1;
+  extern __shared__ int32_t start[];        // [G + 1 or kLengths] | [16]
+  int32_t* red = start + max(a.G + 1, kLengths);
   if (blockIdx.x < 2) {
     if (a.map[blockIdx.x] != nullptr)
       row_tiles(a.offsets, a.G, a.M, a.tile[blockIdx.x], a.ntiles[blockIdx.x], a.map[blockIdx.x], a.first[blockIdx.x], start, red);
   } else if (a.pieces != nullptr) {
-    sum_pieces(a.offsets, a.G, a.M, a.piece, a.entries, a.most, a.pieces, a.sums, a.count, red);
+    sum_pieces(a.offsets, a.G, a.M, a.piece, a.entries, a.most, a.pieces, a.sums, a.count, start, red);
   }
 }
 
@@ -541,6 +540,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
   p.tile = tile;
   if (const char* f = dev_getenv(kind == kFwd ? "BNPVI_TILE_FWD" : kind == kDx ? "BNPVI_TILE_DX" : "BNPVI_TILE_DW")) p.tile = atoi(f);
   if (const char* f = dev_getenv(kind == kFwd ? "BNPVI_SPLIT_FWD" : kind == kDx ? "BNPVI_SPLIT_DX" : "BNPVI_SPLIT_DW")) p.splits = atoi(f);
+  if (const char* f = dev_getenv("BNPVI_PIECE_DW"); f && by_sum) p.piece = atoi(f) * bk;
   int br, bc;
   tile_size(p.tile, br, bc);
   p.row_tiles = ceil_div(rows, br) + (by_rows ? G + 2 : 0);
@@ -650,7 +650,7 @@ static int run_gemm(int kind, int dtype, const GemmPlan& p, bool direct, GemmArg
 
 static int launch_maps(const MapArgs& a, int device, hipStream_t s) {
   static LdsLimit limit;
-  const size_t lds = (size_t)(a.G + 1 + 16) * 4;
+  const size_t lds = (size_t)(std::max(a.G + 1, kLengths) + 16) * 4;
   if (lds > 64 * 1024) BNPVI_HIP(limit.raise((const void*)maps_kernel, device));
   maps_kernel<<<a.pieces ? 3 : a.map[1] ? 2 : 1, 1024, lds, s>>>(a);
   BNPVI_LAUNCH_CHECK();

@@ -416,23 +416,26 @@ struct Stream {
   static constexpr int kBK = KB / (int)sizeof(T);
   typedef Source<T, kKM, ROWS ? BR : BC, THREADS, KB> Src;
   Src src;
-  uint32_t lin, last, step;
+  uint32_t lin, last, inc, twice;
   Share sh;
   int kt, nk;
 
-  __device__ __forceinline__ void begin(const GemmArgs& a, uint32_t first, uint32_t end, uint32_t every, const Share& of) {
+  __device__ __forceinline__ void begin(const GemmArgs& a, uint32_t first, uint32_t end, uint32_t ahead, uint32_t two_turns, const Share& of) {
     lin = first;
     sh = of;
     last = end;
-    step = every;
+    inc = ahead;
+    twice = two_turns;
     enter(a);
   }
   __device__ __forceinline__ void enter(const GemmArgs& a) {
     Tile t;
     kt = 0;
-    for (; lin < last; lin += step)
-      if (find_tile<KIND, BR, BC, kBK>(a, lin, sh, t)) {
-        lin += step;
+    while (lin < last) {
+      const bool found = find_tile<KIND, BR, BC, kBK>(a, lin, sh, t);
+      lin += inc;
+      inc = twice - inc;
+      if (found) {
         const int g = t.g < 0 ? 0 : t.g;
         if (ROWS)
           src.init(reinterpret_cast<const T*>(a.R) + (kKM ? t.row0 * a.ldr + t.k_lo : t.k_lo * a.ldr + t.row0), a.ldr, t.nr, t.kext);
@@ -443,6 +446,7 @@ struct Stream {
         nk = t.stages(kBK);
         return;
       }
+    }
     src.k = 0;                 // behind the last tile: zeros, so that the count of loads on their way stays the same
     nk = 0x7fffffff;
   }
@@ -481,12 +485,14 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
       last = used > xcd ? (used - xcd + 7) / 8 * per : 0;
     }
   }
-  uint32_t lin = first + (blockIdx.x >> 3);
+  // a grouped dW's tiles come longest first: odd turns go through the workgroups backwards, so that long meets short
+  const uint32_t wg = blockIdx.x >> 3, twice = 2 * step;
+  uint32_t lin = first + wg, inc = KIND == kDw && a.map != nullptr ? twice - 2 * wg - 1 : step;
   if (lin >= last) return;
   Stream<T, KIND, BR, BC, KB, THREADS, true> sr;
   Stream<T, KIND, BR, BC, KB, THREADS, false> ss;
-  sr.begin(a, lin, last, step, sh);
-  ss.begin(a, lin, last, step, sh);
+  sr.begin(a, lin, last, inc, twice, sh);
+  ss.begin(a, lin, last, inc, twice, sh);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave / (BC / WC) * WR, wc = wave % (BC / WC) * WC;
@@ -530,7 +536,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
   int behind = 0;
 
   Tile t;
-  for (; lin < last; lin += step) {
+  for (; lin < last; lin += inc, inc = twice - inc) {
     if (!find_tile<KIND, BR, BC, BK>(a, lin, sh, t)) continue;
     f32x16 acc[FR][FC];
 #pragma unroll
