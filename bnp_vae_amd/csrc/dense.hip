@@ -759,7 +759,6 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
   a.rows = M;
   a.cols = n;
   a.K = K;
-  a.G = G;
   a.C = y;
   a.ldc = ldy;
   a.bias = bias;
@@ -949,7 +948,6 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.rows = M;
     a.cols = K;
     a.K = n;
-    a.G = G;
     a.C = dx;
     a.ldc = lddx;
     if (G > 0) a.map = (const int4*)(wk + p.dx_map);
@@ -979,7 +977,6 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.rows = n;
     a.cols = K;
     a.K = M;
-    a.G = groups;
     if (G > 0) {
       a.map = (const int4*)(wk + p.dw_map);
       a.used = (const int32_t*)(wk + p.dw_count);

@@ -47,14 +47,13 @@ struct GemmArgs {
   const void* R;
   const void* S;
   int64_t ldr, lds;            // pitches in elements
-  int64_t rows, cols, K;       // rows of C (all groups), columns, reduce extent (kDw with groups: all frames)
+  int64_t rows, cols, K;       // rows of C (all groups), columns, reduce extent (kDw with groups: unused)
   int64_t s_group, c_group;    // elements between the groups' S (kFwd, kDx) or C (kDw)
-  const int32_t* offsets;      // groups' bounds (kDw) or nullptr
   const int4* map;             // with groups -- kFwd, kDx: row tiles {group, first row, end row}; kDw: pieces of the sum
                                // {group, first frame, end frame, part or -1}
   const int32_t* used;         // kDw with groups: entries of the map in use
   int entries;                 // at most
-  int G, splits;
+  int splits;
   int row_tiles, col_tiles;
   void* C;
   int64_t ldc;

@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256) void rows_from_leaves_kernel(const T* __restri
                                                                const float* __restrict__ weight, const int32_t* __restrict__ kept_at,
                                                                int64_t N, int k, int D, int tx, T* __restrict__ y, int64_t ldy, bool runs) {
   const int sub = threadIdx.x % tx, r = threadIdx.x / tx, rpb = 256 / tx;
-  const int32_t kept = *kept_at;
+  const int32_t kept = (int32_t)max((int64_t)0, min((int64_t)*kept_at, N * k));          // no read goes behind the rows
   const Frames f(N, rpb, runs);
   for (int64_t n = f.first + r; n < f.end; n += f.step) {
     for (int i = sub * E; i < D; i += tx * E) {

@@ -13,8 +13,11 @@ it in its encoder and decoder (/root/reference/src/model.py:70-94); the rest has
 
 Tensors are fp32, bf16 or fp16 on one GPU (responsibilities and weights of leaves fp32); everything is differentiable
 once through torch.autograd, runs on the tensors' device and its current stream, allocates through torch and waits for
-nothing, so it can be captured into a HIP graph (after one call outside a capture).  No CPU fallback.  A leaf number
-outside [0, L) -- `top_leaves` gives -1 -- means "no leaf": such a slot takes part in nothing."""
+nothing, so it can be captured into a HIP graph (after one call outside a capture).  A backward pass is captured with
+leaves of its own or after every result of an eager pass over the same leaves is gone: torch ties a leaf's gradient node to
+the stream of its first use.  No CPU fallback.
+
+A leaf number outside [0, L) -- `top_leaves` gives -1 -- means "no leaf": such a slot takes part in nothing."""
 from __future__ import annotations
 
 import ctypes as C
@@ -110,11 +113,18 @@ class LeafPlan(object):
 
     place   (N, k) int32  place of each slot in leaf order
     order   (N * k,) int32  slot at each place
-    offsets (L + 1,) int32  first place of each leaf; from offsets[L] on lie the slots without a leaf"""
+    offsets (L + 1,) int32  first place of each leaf; from offsets[L] on lie the slots without a leaf
+
+    sort_by_leaf makes it.  One put together by hand has to be such a sort: rows whose place lies outside are left out, and
+    places that repeat leave other rows unwritten."""
 
     __slots__ = ("place", "order", "offsets", "num_leaves")
 
     def __init__(self, place, order, offsets, num_leaves):
+        if place.dim() != 2 or place.dtype != torch.int32 or not place.is_contiguous():
+            raise ValueError("LeafPlan: place must be a contiguous (N, k) int32 tensor")
+        if tuple(offsets.shape) != (num_leaves + 1,) or offsets.dtype != torch.int32 or not offsets.is_contiguous():
+            raise ValueError("LeafPlan: offsets must be a contiguous (%d,) int32 tensor" % (num_leaves + 1))
         self.place, self.order, self.offsets, self.num_leaves = place, order, offsets, num_leaves
 
     @property

@@ -108,3 +108,14 @@ def test_views_whose_memory_is_not_their_value_are_refused():
             layers.top_leaves(t, 1)
         with pytest.raises(TypeError, match="dense tensor"):
             layers.dense(t, torch.zeros((3, 8)))
+
+
+def test_plans_of_other_shapes_and_types_are_refused():
+    i = dict(dtype=torch.int32)
+    place, order, offsets = torch.zeros((4, 2), **i), torch.zeros(8, **i), torch.zeros(4, **i)
+    plan = layers.LeafPlan(place, order, offsets, 3)
+    assert plan.num_frames == 4 and plan.choices == 2
+    for p, o, L in ((place.long(), offsets, 3), (place[0], offsets, 3), (place.t(), offsets, 3), (place, offsets, 4),
+                    (place, offsets.long(), 3), (place, torch.zeros(8, **i)[::2], 3)):
+        with pytest.raises(ValueError, match="LeafPlan"):
+            layers.LeafPlan(p, order, o, L)
