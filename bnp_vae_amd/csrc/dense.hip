@@ -340,30 +340,49 @@ __global__ __launch_bounds__(256) void split_epilogue_kernel(const float* __rest
   }
 }
 
-// ---- one to four rows: a product with a vector -----------------------------------------------------------------------
-// Bound by the weight's bytes (one frame: by the wait for them): WPC waves share a column, 16 bytes a lane of its row of
-// W, all of a part's loads under way at once; their sums meet in LDS.
-constexpr int kGemvRows = 4;
+// ---- up to eight rows: products with vectors ---------------------------------------------------------------------------
+// Bound by the weight's bytes (one frame: by the wait for them): a wave a column, 16 bytes a lane of its row of W, or four
+// waves where rows are long and columns too few for all CUs, whose sums meet in LDS (8 x 4096 -> 1024 bf16: 6.5 us, one
+// wave 7.4; 4 x 4096 -> 4096: 12.6, one wave 8.8; fp32 4 x 4096 -> 4096: 17.1 and 16.7, one row 11.9 and 13.1).
+// The matrix kernel takes 32 rows whatever their number and parts of the sum to fill the chip (8 x 4096 -> 32: 14.7 us in
+// bf16 and 22.5 in fp32, here 6.8 and 6.2), but reads x once a tile, where every column here reads all of it: 8 x 4096 ->
+// 4096 in fp32 takes 23.5 us there and would take 34.4 here, six rows 23.3 and 23.5.
+static bool as_vectors(int64_t M, int64_t K, int64_t n, int G) { return G == 0 && (M <= 4 || (M <= 8 && (double)M * K * n <= 1.0e8)); }
 
 template <typename T>
 struct Piece {
   static constexpr int kPer = 16 / (int)sizeof(T);
-  float v[kPer];
+  union {
+    u32x4_anywhere u;
+    T t[kPer];
+  } v;
   __device__ __forceinline__ void load(const T* p, int inside) {
     if (inside >= kPer) {
-      union {
-        u32x4_anywhere u;
-        T t[kPer];
-      } q;
-      q.u = *reinterpret_cast<const u32x4_anywhere*>(p);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) v[e] = (float)q.t[e];
+      v.u = *reinterpret_cast<const u32x4_anywhere*>(p);
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) v[e] = e < inside ? (float)p[e] : 0.f;
+      for (int e = 0; e < kPer; ++e) v.t[e] = e < inside ? p[e] : (T)0.f;
     }
   }
 };
+// acc + <a, b>, for 16 bits by the instruction that adds two products of a pair to an fp32 sum
+template <typename T>
+__device__ __forceinline__ float dot(const Piece<T>& a, const Piece<T>& b, float acc) {
+#pragma unroll
+  for (int e = 0; e < Piece<T>::kPer; e += sizeof(T) == 4 ? 1 : 2) {
+    if constexpr (sizeof(T) == 4) {
+      acc = fmaf(a.v.t[e], b.v.t[e], acc);
+    } else {
+      typedef T two __attribute__((ext_vector_type(2)));
+      const two p = {a.v.t[e], a.v.t[e + 1]}, q = {b.v.t[e], b.v.t[e + 1]};
+      if constexpr (std::is_same<T, bf16_t>::value)
+        acc = __builtin_amdgcn_fdot2_f32_bf16(p, q, acc, false);
+      else
+        acc = __builtin_amdgcn_fdot2(p, q, acc, false);
+    }
+  }
+  return acc;
+}
 
 template <typename T, int M, int WPC>
 __global__ __launch_bounds__(256) void gemv_kernel(const GemmArgs a) {
@@ -385,8 +404,7 @@ __global__ __launch_bounds__(256) void gemv_kernel(const GemmArgs a) {
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         px.load(x + m * a.ldr + k, inside);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) acc[m] = fmaf(px.v[e], pw.v[e], acc[m]);
+        acc[m] = dot(px, pw, acc[m]);
       }
     }
   }
@@ -413,7 +431,7 @@ __global__ __launch_bounds__(256) void gemv_kernel(const GemmArgs a) {
 
 template <typename T, int M>
 static void launch_gemv(const GemmArgs& a, hipStream_t s) {
-  if (a.K * (int64_t)sizeof(T) > 2048)
+  if (a.K * (int64_t)sizeof(T) > 2048 && (sizeof(T) == 4 || a.cols < 2048))
     gemv_kernel<T, M, 4><<<(unsigned)a.cols, 256, 0, s>>>(a);
   else
     gemv_kernel<T, M, 1><<<(unsigned)ceil_div(a.cols, 4), 256, 0, s>>>(a);
@@ -428,8 +446,16 @@ static void gemv(const GemmArgs& a, hipStream_t s) {
       return launch_gemv<T, 2>(a, s);
     case 3:
       return launch_gemv<T, 3>(a, s);
-    default:
+    case 4:
       return launch_gemv<T, 4>(a, s);
+    case 5:
+      return launch_gemv<T, 5>(a, s);
+    case 6:
+      return launch_gemv<T, 6>(a, s);
+    case 7:
+      return launch_gemv<T, 7>(a, s);
+    default:
+      return launch_gemv<T, 8>(a, s);
   }
 }
 
@@ -589,7 +615,7 @@ static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, c
   p.dx = gemm_plan(kDx, dtype, M, K, n, p.grouped, G, ways.dx);
   p.dw = gemm_plan(kDw, dtype, n, K, M, p.grouped, G, ways.dw);
   p.dz_tiles = ceil_div(M, kDzRows) + (p.grouped ? G + 2 : 0);
-  const bool vector = !p.grouped && M <= kGemvRows;
+  const bool vector = as_vectors(M, K, n, G);
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t o = at;
@@ -768,7 +794,7 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
   a.dact = dact;
   a.lddact = lddact;
   a.act = activation;
-  if (G == 0 && M <= kGemvRows) {
+  if (as_vectors(M, K, n, G)) {
     if (dtype == BNPVI_F32)
       gemv<float>(a, s);
     else if (dtype == BNPVI_BF16)

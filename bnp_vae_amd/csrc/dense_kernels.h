@@ -15,6 +15,17 @@
 // Products: v_mfma_f32_32x32x16 (bf16, f16) and v_mfma_f32_32x32x2_f32, fp32 accumulation.  S is the first operand of
 // the instruction, so a lane ends with four consecutive columns of one row; the accumulators pass through LDS once
 // more so that the epilogue reads and writes whole 16-byte pieces of rows, eight lanes and more a row.
+//
+// What bounds it.  A wave tile of 128 x 64 needs 6 KB of fragments for 8 instructions: of the LDS's 128 bytes a cycle the
+// fragments take three quarters and the arriving stages the rest, so that matrix pipe and LDS are full at the same time,
+// and 8192^3 in bf16 runs at 1170 / 1065 / 1050 TFLOP/s (forward, dx, dW; the library 1430; without the loads 1460).  Where
+// the sum is short the epilogue counts: dx of 65536 x 256 -> 4096 takes 200 us, 95 of them its 537 MB of stores alone, 60
+// the products, and a tile's stores and the next one's products share the time only as far as its loads reach ahead.
+// 65536 x 4096 -> 256 forward reads 537 MB in 150 us (3.6 TB/s, a copy 4.7).  fp32 is bound by its matrix rate: 135 of 157
+// TFLOP/s at K = 2048, and by stores where K is short (16384 x 64 -> 4096: 61 us of products, 68 of stores).
+// Tried without gain: four waves of 128 x 128 (8192^3 1100 TFLOP/s; dx spills), stages of 64 bytes, a fourth stage in the
+// ring, loads spread over the steps of a stage (dx 1035 -> 1125 us), the epilogue unrolled (it spills: 160 -> 300 us) or
+// from registers (32 bytes a row and store: dx 200 -> 280 us), 128 x 256 tiles two a CU, co-resident workgroups out of phase.
 #pragma once
 
 #include <type_traits>
@@ -151,7 +162,8 @@ __device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t r, char* l,
 // the 128 that one cycle of the LDS serves
 template <int KB>
 __device__ __forceinline__ int swizzle(int r) {
-  return KB == 128 ? r & 7 : (r >> 1) & 3;
+  static_assert(KB == 128, "eight pieces a row");
+  return r & 7;
 }
 
 // Where the 16-byte pieces of one operand stage (KB bytes of k) come from.  B rows (KM) or columns (MM), P pieces a lane.

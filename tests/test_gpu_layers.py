@@ -362,7 +362,8 @@ def test_dense_activations(layers, dtype, act):
 
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
-@pytest.mark.parametrize("M,K,n", [(1, 4096, 32), (8, 4096, 256), (40, 2048, 48), (500, 1000, 64), (2500, 64, 512), (4000, 160, 264)])
+@pytest.mark.parametrize("M,K,n", [(1, 4096, 32), (8, 4096, 256), (40, 2048, 48), (500, 1000, 64), (2500, 64, 512), (4000, 160, 264),
+                                   (3, 1000, 2050), (4, 1031, 9), (5, 700, 2500), (6, 33, 5), (7, 4096, 40), (8, 2050, 70), (8, 4096, 4100), (9, 1000, 40)])
 def test_dense_long_sums_and_many_tiles(layers, dtype, M, K, n):
     check_dense(layers, M, K, n, TYPES[dtype], "gelu", True, True, seed=M)
 
