@@ -656,6 +656,35 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
       const T* bp = reinterpret_cast<const T*>(a.bias) + t.g * a.bias_group + col;
       load_any<T, 8>(bp, left, b);
     }
+    // This lane's first row; the others are uniform distances away.  The residual's pieces of 32 rows are under way together
+    // and used in order without an index (one after the other the residual block of 32768 x 1024 takes 328 us, so 317; the
+    // registers that this costs make 65536 x 4096 -> 256 without a residual 1 % slower).
+    const int64_t row0 = t.row0 + wr + lane / LPR;
+    T* const out0 = reinterpret_cast<T*>(a.C) + (KIND == kDw ? t.g * a.c_group : 0) + row0 * a.ldc + col;
+    constexpr int IT = 32 / RPI, RP = 8 * (int)sizeof(T) / 16;
+    const bool with_res = KIND == kFwd && a.res != nullptr && a.slab == nullptr && t.g >= 0;
+    u32x4 ahead[KIND == kFwd ? IT * RP : 1];
+    const T* const res0 = reinterpret_cast<const T*>(a.res) + row0 * a.ldres + col;
+    auto fetch = [&](int i) {
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        if (wr + 32 * i + it * RPI + lane / LPR >= t.nr || left <= 0) continue;
+        const T* rp = res0 + (int64_t)(32 * i + it * RPI) * a.ldres;
+        if (left == 8) {
+#pragma unroll
+          for (int q = 0; q < RP; ++q) ahead[it * RP + q] = reinterpret_cast<const u32x4_anywhere*>(rp)[q];
+        } else {
+          union {
+            u32x4 u[RP];
+            T t[8];
+          } x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x.t[e] = e < left ? rp[e] : (T)0.f;
+#pragma unroll
+          for (int q = 0; q < RP; ++q) ahead[it * RP + q] = x.u[q];
+        }
+      }
+    };
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wave is done reading the stages
 #pragma unroll
     for (int i = 0; i < FR; ++i) {
@@ -675,11 +704,11 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
             }
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 1
-          for (int it = 0; it < 32 / RPI; ++it) {
+          for (int it = 0; it < IT; ++it) {
             const int r = it * RPI + lane / LPR, rl = wr + 32 * i + r;
             if (rl >= t.nr || left <= 0) continue;
             const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * (WC * 2) + ((c ^ (r & (WC / 8 - 1))) << 4));
-            T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? t.g * a.c_group : 0) + (t.row0 + rl) * a.ldc + col;
+            T* out = out0 + (int64_t)(32 * i + it * RPI) * a.ldc;
             if (left == 8) {
               __builtin_nontemporal_store((u32x4_anywhere)v, reinterpret_cast<u32x4_anywhere*>(out));
             } else {
@@ -706,15 +735,15 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
               f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the wave reads only what it wrote itself
+      if (with_res) fetch(i);
 #pragma unroll 1
-      for (int it = 0; it < 32 / RPI; ++it) {
+      for (int it = 0; it < IT; ++it) {
         const int r = it * RPI + lane / LPR, rl = wr + 32 * i + r;
         if (rl >= t.nr || left <= 0) continue;
-        const int64_t row = t.row0 + rl;
         const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + r * (WC * 4) + (((2 * c) ^ (r & (SLOTS - 1))) << 4));
         const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + r * (WC * 4) + (((2 * c + 1) ^ (r & (SLOTS - 1))) << 4));
         if (a.slab != nullptr && t.z >= 0) {
-          float* out = a.slab + ((int64_t)t.z * a.rows + row) * a.cols + col;
+          float* out = a.slab + ((int64_t)t.z * a.rows + row0 + 32 * i + it * RPI) * a.cols + col;
           if (left == 8 && a.cols % 4 == 0) {
             *reinterpret_cast<f32x4*>(out) = v0;
             *reinterpret_cast<f32x4*>(out + 4) = v1;
@@ -731,16 +760,22 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
           v[e] = v0[e];
           v[e + 4] = v1[e];
         }
-        T* out = reinterpret_cast<T*>(a.C) + (KIND == kDw ? t.g * a.c_group : 0) + row * a.ldc + col;
+        T* out = out0 + (int64_t)(32 * i + it * RPI) * a.ldc;
         if (KIND == kFwd) {
           typedef typename Deriv<T>::type DT;
           float d[8], q[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) q[e] = d[e] = 0.f;
           if (t.g >= 0) {
-            if (a.res != nullptr) {
-              const T* rp = reinterpret_cast<const T*>(a.res) + row * a.ldres + col;
-              load_any<T, 8>(rp, left, q);
+            if (with_res) {
+              union {
+                u32x4 u[RP];
+                T t[8];
+              } x;
+#pragma unroll
+              for (int p = 0; p < RP; ++p) x.u[p] = ahead[p];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) q[e] = (float)x.t[e];
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += b[e];
@@ -749,11 +784,15 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
             for (int e = 0; e < 8; ++e) v[e] += q[e];
           }
           if (a.dact != nullptr) {
-            DT* dp = reinterpret_cast<DT*>(a.dact) + row * a.lddact + col;
+            DT* dp = reinterpret_cast<DT*>(a.dact) + row0 * a.lddact + col + (int64_t)(32 * i + it * RPI) * a.lddact;
             store_any<true, DT, 8>(dp, left, d);
           }
         }
         store_any<true, T, 8>(out, left, v);
+        if constexpr (KIND == kFwd) {
+#pragma unroll
+          for (int p = 0; p + RP < IT * RP; ++p) ahead[p] = ahead[p + RP];
+        }
       }
     }
     // a full tile in 16-byte pieces: the number of its stores is known
