@@ -61,14 +61,17 @@ def _latents(z, encoder, device):
     return out
 
 
-def _rows_by_leaf(assign, L):
-    """Row indices in the order of their leaves, rows ascending within a leaf."""
+def _by_leaf(assign, L, *tables):
+    """Row indices in the order of their leaves, rows ascending within a leaf, and the tables' rows in that order."""
     import torch
     from . import layers
     from ._lib import lib
     if L <= lib.bnpvi_leaf_sort_max_leaves() and assign.shape[0] < 1 << 31:
-        return layers.sort_by_leaf(assign, L).order.to(torch.int64)
-    return torch.sort(assign.to(torch.int64), stable=True).indices
+        plan = layers.sort_by_leaf(assign, L)              # every row has a leaf
+        moved = [layers.dispatch(t.view(torch.float32), plan).view(t.dtype) for t in tables]      # bytes, whatever they mean
+        return [plan.order.to(torch.int64)] + moved
+    rows = torch.sort(assign.to(torch.int64), stable=True).indices
+    return [rows] + [t[rows] for t in tables]
 
 
 def closest_frames(nodes_list, z, K, device=None, encoder=None):
@@ -98,9 +101,9 @@ def closest_frames(nodes_list, z, K, device=None, encoder=None):
         node, dist = dev.path_distances(assign)
         depth = node.shape[1]
         # candidates in the reference's order: leaves depth-first, rows ascending within a leaf
-        rows = _rows_by_leaf(assign, dev.tree.L)
-        cand_node = node[rows].reshape(-1).to(torch.int64)
-        cand_dist = dist[rows].reshape(-1)
+        rows, node, dist = _by_leaf(assign, dev.tree.L, node, dist)
+        cand_node = node.reshape(-1).to(torch.int64)
+        cand_dist = dist.reshape(-1)
         cand_row = rows.repeat_interleave(depth)
         keep = cand_node >= 0
         cand_node, cand_dist, cand_row = cand_node[keep], cand_dist[keep], cand_row[keep]
