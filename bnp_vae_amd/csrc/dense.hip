@@ -485,8 +485,13 @@ static void tile_size(int tile, int& br, int& bc) {
 // workgroup the microseconds below, by how many of them share a CU (8192^3 in 16 bits: 64 / 128 / 256 wide tiles make 384 /
 // 560 / 760 outputs a nanosecond and stage, so the large tile wins wherever it fills the chip; fp32 is bound by its matrix
 // rate), and a tile its first load and its epilogue.  65536 x 4096 -> 256: 207 us in tiles of 128, 173 in tiles of 256;
-// 16384 x 512 -> 512: 15 us in tiles of 128, 22 in tiles of 256.  Splitting the sum costs a launch and two passes over the
-// parts.  Transposing reads cost the large tile's stages a tenth more (8192^3: 938 / 1035 / 1100 us forward, dx, dW).
+// 16384 x 512 -> 512: 15 us in tiles of 128, 22 in tiles of 256; 256 leaves of 200 rows, 512 -> 512: 80 and 102.
+// Splitting the sum costs a launch and two passes over the parts.  Transposing reads cost the large tile's stages a tenth
+// more (8192^3: 938 / 1035 / 1100 us forward, dx, dW).
+//
+// Narrow results take the tall tile (50000 x 1024 -> 32: 19 us in bf16 and 55 in fp32, tiles of 64: 22 and 81), few rows the
+// flat one, and so do small leaves, whose last tile is half empty on average (256 leaves of 40 / 96 / 128 rows, 512 -> 512 in
+// bf16: 39 / 52 / 67 us, tiles of 64 or 128: 41 / 57 / 62; fp32, of 40 / 200 rows: 122 / 332 us and 144 / 342).
 //
 // dW with groups: leaves are unequal, and a launch waits for its longest tile.  A leaf longer than `piece` frames is summed
 // in pieces; the shorter they are the evener the end (half a piece is idle on average), the more partial results pass
@@ -501,7 +506,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
   p.splits = 1;
   if (cols <= 32 && per_group > 32) {
     p.tile = kTileTall;
-  } else if (per_group <= 32) {
+  } else if (per_group <= (by_rows ? (e == 4 ? 256 : 96) : 32)) {
     p.tile = kTileFlat;
   } else {
     p.tile = kTile64;
@@ -509,7 +514,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
   // kTile128, kTile64 (also for the narrow ones), kTile256; up to four workgroups a CU
   static const double k16[3][4] = {{0.9, 1.3, 1.3, 1.3}, {0.5, 0.6, 0.72, 0.84}, {1.83, 1.83, 1.83, 1.83}};
   static const double k32[3][4] = {{1.8, 3.5, 3.5, 3.5}, {0.6, 1.0, 1.5, 1.92}, {0, 0, 0, 0}};
-  static const double kTileCost[] = {5.0, 3.5, 8.0};
+  const double tile_cost[] = {5.0, 3.5, kind == kFwd ? 12.0 : kind == kDx ? 9.0 : 8.0};
   static const int kPerCu[] = {2, 4, 1};
   auto row_of = [](int tile) { return tile == kTile128 ? 0 : tile == kTile256 ? 2 : 1; };
   const int64_t stages = std::max<int64_t>(1, ceil_div(K, bk));
@@ -523,7 +528,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
     const int r = row_of(tile);
     const int64_t n = tiles_of(tile) * s, whole = n / (kPerCu[r] * kNumCU), rest = ceil_div(n % (kPerCu[r] * kNumCU), kNumCU);
     auto turn = [&](int64_t each) {
-      return (double)ceil_div(stages, s) * (e == 4 ? k32 : k16)[r][each - 1] * (r == 2 ? 1.0 + 0.08 * kind : 1.0) + kTileCost[r];
+      return (double)ceil_div(stages, s) * (e == 4 ? k32 : k16)[r][each - 1] * (r == 2 ? 1.0 + 0.08 * kind : 1.0) + tile_cost[r];
     };
     return whole * turn(kPerCu[r]) + (rest ? turn(rest) : 0.0) + (s > 1 ? 4.0 + 8.0 * s * rows * cols / 4.0e6 : 0.0);
   };
@@ -534,7 +539,7 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
     const double slots = (double)kPerCu[r] * kNumCU, tiles = (double)tiles_of(tile), work = tiles * (double)(stages + G / 2) / slots;
     const double full = (double)stages / (double)len, stage = (e == 4 ? k32 : k16)[r][kPerCu[r] - 1] * (r == 2 ? 1.16 : 1.0);
     const double parts = stages >= len * G ? full + G / 2 : 0.3 * full;
-    return work * stage + (full + G) * tiles / slots * kTileCost[r] + 0.5 * len * stage + 4.0 + 8.0 * parts * rows * cols / 4.0e6;
+    return work * stage + (full + G) * tiles / slots * tile_cost[r] + 0.5 * len * stage + 4.0 + 8.0 * parts * rows * cols / 4.0e6;
   };
   const int64_t most = grouped ? 1 : std::min<int64_t>(64, std::max<int64_t>(1, stages / 2));
   const int tried[] = {p.tile, kTile128, kTile256};

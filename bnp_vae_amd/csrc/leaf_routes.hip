@@ -569,8 +569,10 @@ static SortPlan sort_plan(int64_t M, int L) {
   p.bits = 1;
   while ((int64_t(1) << p.bits) < B) ++p.bits;
   if (M <= 8192 && (size_t)17 * B * 4 + 64 <= (size_t)kMaxLdsBytes) {
-    p.nb = 1;                                // a minibatch: one workgroup, one launch
-    p.waves = M <= 1024 ? 4 : 16;
+    // a minibatch: one workgroup, one launch (8192 slots, 512 leaves: 13.6 us, three launches 17.8; 16000: 22 and 17.9), of 16
+    // waves but for the smallest (1000 slots, 512 leaves: 6.1 us, four waves 8.2; 256 slots, 25 leaves: 4.7 and 3.9)
+    p.nb = 1;
+    p.waves = M <= 512 && L <= 256 ? 4 : 16;
     p.threads = p.waves * 64;
     p.chunk = M < 1 ? 1 : M;
     p.lds = ((size_t)(p.waves + 1) * B + 16) * 4;
