@@ -125,6 +125,8 @@ class LeafPlan(object):
             raise ValueError("LeafPlan: place must be a contiguous (N, k) int32 tensor")
         if tuple(offsets.shape) != (num_leaves + 1,) or offsets.dtype != torch.int32 or not offsets.is_contiguous():
             raise ValueError("LeafPlan: offsets must be a contiguous (%d,) int32 tensor" % (num_leaves + 1))
+        if place.device != offsets.device:
+            raise ValueError("LeafPlan: place is on %s, offsets on %s" % (place.device, offsets.device))
         self.place, self.order, self.offsets, self.num_leaves = place, order, offsets, num_leaves
 
     @property
@@ -160,7 +162,10 @@ def sort_by_leaf(leaf, num_leaves):
 def _check_plan(what, plan, **tensors):
     if not isinstance(plan, LeafPlan):
         raise TypeError("%s: plan must be a LeafPlan (sort_by_leaf), not %s" % (what, type(plan).__name__))
-    return _on_gpu(what, **dict(tensors, place=plan.place, offsets=plan.offsets))
+    device = _on_gpu(what, **tensors)
+    if plan.place.device != device:
+        raise ValueError("%s: the plan is on %s, other tensors on %s" % (what, plan.place.device, device))
+    return device
 
 
 def dispatch(x, plan):
