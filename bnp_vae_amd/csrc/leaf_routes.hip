@@ -563,6 +563,7 @@ int bnpvi_top_leaves_backward(bnpvi_ctx* ctx, const int32_t* leaf, const float* 
 
 // ---- sort: sizes of one call ---------------------------------------------------------------------------------------
 struct SortPlan {
+  bool single;                 // one workgroup, one launch, no workspace: its LDS holds the firsts of all bins too
   int waves, threads, bits, nb;
   int64_t chunk;
   size_t lds;
@@ -570,12 +571,14 @@ struct SortPlan {
 
 static SortPlan sort_plan(int64_t M, int L) {
   SortPlan p;
+  p.single = false;
   const int B = L + 1, nsum = (B + 63) / 64;
   p.bits = 1;
   while ((int64_t(1) << p.bits) < B) ++p.bits;
   if (M <= 8192 && (size_t)17 * B * 4 + 64 <= (size_t)kMaxLdsBytes) {
     // a minibatch: one workgroup, one launch (8192 slots, 512 leaves: 13.6 us, three launches 17.8; 16000: 22 and 17.9), of 16
     // waves but for the smallest (1000 slots, 512 leaves: 6.1 us, four waves 8.2; 256 slots, 25 leaves: 4.7 and 3.9)
+    p.single = true;
     p.nb = 1;
     p.waves = M <= 512 && L <= 256 ? 4 : 16;
     p.threads = p.waves * 64;
@@ -597,14 +600,12 @@ static SortPlan sort_plan(int64_t M, int L) {
   return p;
 }
 
-static bool one_launch(const SortPlan& p, int64_t M) { return p.nb == 1 && p.chunk == (M < 1 ? 1 : M); }
-
 int bnpvi_leaf_sort_max_leaves(void) { return kSortMaxLeaves; }
 
 int64_t bnpvi_leaf_sort_workspace(int64_t M, int L) {
   if (M < 0 || M > INT32_MAX || L < 1 || L > kSortMaxLeaves) return -1;
   const SortPlan p = sort_plan(M, L);
-  return M <= 8192 && one_launch(p, M) ? 0 : ((int64_t)(p.nb + 1) * (L + 1) + (L + 64) / 64) * 4;
+  return p.single ? 0 : ((int64_t)(p.nb + 1) * (L + 1) + (L + 64) / 64) * 4;
 }
 
 int bnpvi_leaf_sort(bnpvi_ctx* ctx, const int32_t* leaf, int64_t M, int L, int32_t* place, int32_t* order, int32_t* offsets,
@@ -623,7 +624,7 @@ int bnpvi_leaf_sort(bnpvi_ctx* ctx, const int32_t* leaf, int64_t M, int L, int32
   const int B = L + 1;
   static LdsLimit place_limit, count_limit;
   BNPVI_HIP(place_limit.raise((const void*)leaf_place_kernel, ctx->device));
-  if (need == 0) {
+  if (p.single) {
     leaf_place_kernel<<<1, p.threads, p.lds, s>>>(leaf, M, L, p.chunk, p.bits, p.waves, nullptr, nullptr, nullptr, place, order, offsets);
   } else {
     BNPVI_HIP(count_limit.raise((const void*)leaf_count_kernel, ctx->device));

@@ -878,3 +878,42 @@ def test_hierarchy_from_features(layers, dtype, monkeypatch):
     assert np.array_equal(p[0], q[0]) and np.array_equal(p[1], q[1])
     with pytest.raises(ValueError, match="encoder"):
         hierarchy.nearest_leaf(nodes, x, encoder=[])
+
+
+# ------------------------------------------------------------------------------------------------ sorts of one chunk over many leaves
+@pytest.mark.parametrize("M", [2047, 2048, 2049])
+@pytest.mark.parametrize("L", [2407, 2408, 7776, 16384])
+def test_sort_of_a_chunk_over_many_leaves(layers, M, L):
+    """As many slots as a chunk holds, where the counters of a single workgroup just fit the LDS and where they do not."""
+    leaf = torch.randint(-1, L, (M,), generator=torch.Generator().manual_seed(M + L), dtype=torch.int32)
+    leaf[5], leaf[-1] = L, L - 1
+    plan = layers.sort_by_leaf(gpu(leaf), L)
+    place, order, offsets = sort_reference(leaf, L)
+    assert torch.equal(plan.offsets.cpu().long(), offsets)
+    assert torch.equal(plan.order.cpu().long(), order)
+    assert torch.equal(plan.place.cpu().long().reshape(-1), place)
+
+
+@pytest.mark.parametrize("N,k", [(2048, 1), (1024, 2), (512, 4), (256, 8)])
+def test_exchange_of_2048_slots_over_the_largest_tree(layers, N, k):
+    L = 7776
+    leaf = torch.randint(-1, L, (N, k), generator=torch.Generator().manual_seed(N), dtype=torch.int32)
+    x = rand((N, 12), torch.float32, 1)
+    plan = layers.sort_by_leaf(gpu(leaf), L)
+    xs = layers.dispatch(gpu(x), plan)
+    ys = rand((N * k, 12), torch.float32, 2)
+    want_xs, want_y, rows, _wk, _place, _order, _kept = exchange_reference(x, ys, leaf, None, L)
+    assert torch.equal(xs.cpu().double(), want_xs)
+    within(layers.combine(gpu(ys), plan), want_y, 2.0 ** -24 * want_y.abs() + (k + 16) * 2.0 ** -23 * rows.abs().sum(1))
+
+
+def test_closest_frames_of_2048_frames_below_a_wide_tree(layers):
+    """Frames are brought into leaf order with the framework's own sort: on 2048 frames over 2500 leaves they lie as
+    torch.sort puts them."""
+    from bnp_vae_amd import hierarchy
+    assign = torch.randint(0, 2500, (2048,), device="cuda", generator=torch.Generator("cuda").manual_seed(3), dtype=torch.int32)
+    node = torch.randint(-1, 3000, (2048, 3), device="cuda", generator=torch.Generator("cuda").manual_seed(4), dtype=torch.int32)
+    dist = torch.rand((2048, 3), device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    rows, node_s, dist_s = hierarchy._by_leaf(assign, 2500, node, dist)
+    want = torch.sort(assign.long(), stable=True).indices
+    assert torch.equal(rows, want) and torch.equal(node_s, node[want]) and torch.equal(dist_s, dist[want])

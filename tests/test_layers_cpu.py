@@ -119,3 +119,16 @@ def test_plans_of_other_shapes_and_types_are_refused():
                     (place, offsets.long(), 3), (place, torch.zeros(8, **i)[::2], 3)):
         with pytest.raises(ValueError, match="LeafPlan"):
             layers.LeafPlan(p, order, o, L)
+
+
+@pytest.mark.parametrize("L", [1, 64, 2407, 2408, 7776, 16384])
+@pytest.mark.parametrize("M", [0, 1, 2047, 2048, 2049, 4096, 8191, 8192, 8193])
+def test_a_sort_without_workspace_has_its_counters_in_the_lds(M, L):
+    """One workgroup sorts alone where 16 waves' counters of L + 1 bins, the bins' firsts and 16 sums fit 160 KB; everywhere
+    else the call needs a workspace for the chunks' counters, however many slots there are."""
+    alone = M <= 8192 and 4 * (17 * (L + 1) + 16) <= 160 * 1024
+    need = _lib.lib.bnpvi_leaf_sort_workspace(M, L)
+    assert need == 0 if alone else need >= 8 * (L + 1)
+    if not alone:
+        c, one = _Ctx(), C.c_void_p(256)
+        _fails(_lib.lib.bnpvi_leaf_sort(c.p, one, M, L, one, one, one, None, 0, None), "workspace")
