@@ -180,8 +180,8 @@ __global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
 constexpr int kDzRows = 128;
 
 template <typename T>
-__global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64_t lddy, const typename Deriv<T>::type* __restrict__ d,
-                                                 int64_t ldd, const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz,
+__global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64_t lddy, const float* __restrict__ d, int64_t ldd,
+                                                 const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz,
                                                  int64_t lddz, T* __restrict__ dres, int64_t lddres, float* __restrict__ part,
                                                  T* __restrict__ db) {
   constexpr int CT = 32, E = 8;              // threads across, columns a thread
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
       load_any<T, E>(dy + r * lddy + c, inside, v);
       if (dres != nullptr) store_any<false, T, E>(dres + r * lddres + c, inside, v);
       if (d != nullptr) {
-        load_any<typename Deriv<T>::type, E>(d + r * ldd + c, inside, o);
+        load_any<float, E>(d + r * ldd + c, inside, o);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] *= o[e];
         // rows of dz end on 16 bytes, with zeros behind column n
@@ -325,7 +325,6 @@ __global__ __launch_bounds__(256) void piece_sum_kernel(const SumArgs a, const i
 
 template <typename T>
 __global__ __launch_bounds__(256) void split_epilogue_kernel(const float* __restrict__ slab, int splits, const GemmArgs a) {
-  typedef typename Deriv<T>::type DT;
   const int64_t elems = a.rows * a.cols;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / a.cols, col = i % a.cols;
@@ -336,7 +335,7 @@ __global__ __launch_bounds__(256) void split_epilogue_kernel(const float* __rest
     activate<sizeof(T) == 2, 1>(a.act, v, d);
     float y = v[0];
     if (a.res != nullptr) y += (float)reinterpret_cast<const T*>(a.res)[row * a.ldres + col];
-    if (a.dact != nullptr) reinterpret_cast<DT*>(a.dact)[row * a.lddact + col] = (DT)d[0];
+    if (a.dact != nullptr) a.dact[row * a.lddact + col] = d[0];
     reinterpret_cast<T*>(a.C)[row * a.ldc + col] = (T)y;
   }
 }
@@ -419,14 +418,13 @@ __global__ __launch_bounds__(256) void gemv_kernel(const GemmArgs a) {
   __syncthreads();
   const int m = lane;
   if (part != 0 || m >= M || col >= a.cols) return;
-  typedef typename Deriv<T>::type DT;
   float z[1] = {0.f}, d[1];
 #pragma unroll
   for (int p = 0; p < WPC; ++p) z[0] += sums[wave + p][m];
   if (a.bias != nullptr) z[0] += (float)reinterpret_cast<const T*>(a.bias)[col];
   activate<sizeof(T) == 2, 1>(a.act, z, d);
   if (a.res != nullptr) z[0] += (float)reinterpret_cast<const T*>(a.res)[m * a.ldres + col];
-  if (a.dact != nullptr) reinterpret_cast<DT*>(a.dact)[m * a.lddact + col] = (DT)d[0];
+  if (a.dact != nullptr) a.dact[m * a.lddact + col] = d[0];
   reinterpret_cast<T*>(a.C)[m * a.ldc + col] = (T)z[0];
 }
 
@@ -694,7 +692,7 @@ static unsigned flat_grid(int64_t elems) { return (unsigned)std::max<int64_t>(1,
 template <typename T>
 static void launch_dz(const T* dy, int64_t lddy, const void* d, int64_t ldd, const int4* map, int64_t M, int n, int64_t tiles, T* dz,
                       int64_t lddz, T* dres, int64_t lddres, float* part, void* db, hipStream_t s) {
-  dz_kernel<T><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 256)), 256, 0, s>>>(dy, lddy, (const typename Deriv<T>::type*)d, ldd, map, M, n,
+  dz_kernel<T><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 256)), 256, 0, s>>>(dy, lddy, (const float*)d, ldd, map, M, n,
                                                                                  dz, lddz, dres, lddres, part, (T*)db);
 }
 
@@ -797,7 +795,7 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
   a.bias_group = G > 1 ? bias_group : 0;
   a.res = residual;
   a.ldres = ldres;
-  a.dact = dact;
+  a.dact = (float*)dact;
   a.lddact = lddact;
   a.act = activation;
   if (as_vectors(M, K, n, G)) {

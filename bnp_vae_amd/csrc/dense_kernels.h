@@ -40,17 +40,6 @@ typedef bf16_t bf16x4 __attribute__((ext_vector_type(4)));
 typedef f16_t f16x8v __attribute__((ext_vector_type(8)));
 typedef __fp16 f16x4s __attribute__((ext_vector_type(4)));
 
-// The derivative of the activation is kept for the backward pass in a type that does not add to the error of the
-// 16-bit gradients: fp16 (half a step 2^-12, 2^-25 absolute below 2^-14) beside bf16's 2^-9, fp32 beside fp16 and fp32.
-template <typename T>
-struct Deriv {
-  typedef float type;
-};
-template <>
-struct Deriv<bf16_t> {
-  typedef f16_t type;
-};
-
 enum { kFwd = 0, kDx = 1, kDw = 2 };
 enum { kTile128 = 0, kTile64 = 1, kTileFlat = 2, kTileTall = 3, kTile256 = 4 };      // 128x128, 64x64, 32x128, 128x32, 256x256
 
@@ -72,7 +61,7 @@ struct GemmArgs {
   int64_t bias_group;
   const void* res;
   int64_t ldres;
-  void* dact;
+  float* dact;                 // act'(z) in 32 bits beside every type: its far ends (softsign' 1e-8 at 1e4) pass fp16's range
   int64_t lddact;
   int act;
   float* slab;                 // [group x split][rows][cols] partial sums, or nullptr
@@ -543,7 +532,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
   // vector stores of a full tile's epilogue that a wave issues behind its loads (0: unknown, wait for all of them)
   constexpr int LPR = WC / 8, RPI = 64 / LPR, SLOTS = WC / 4;
   constexpr int Y_OPS = FR * (32 / RPI) * (int)sizeof(T) / 2;
-  constexpr int D_OPS = FR * (32 / RPI) * (int)sizeof(typename Deriv<T>::type) / 2;
+  constexpr int D_OPS = FR * (32 / RPI) * 2;
   int behind = 0;
 
   Tile t;
@@ -762,7 +751,6 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
         }
         T* out = out0 + (int64_t)(32 * i + it * RPI) * a.ldc;
         if (KIND == kFwd) {
-          typedef typename Deriv<T>::type DT;
           float d[8], q[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) q[e] = d[e] = 0.f;
@@ -784,8 +772,8 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
             for (int e = 0; e < 8; ++e) v[e] += q[e];
           }
           if (a.dact != nullptr) {
-            DT* dp = reinterpret_cast<DT*>(a.dact) + row0 * a.lddact + col + (int64_t)(32 * i + it * RPI) * a.lddact;
-            store_any<true, DT, 8>(dp, left, d);
+            float* dp = a.dact + row0 * a.lddact + col + (int64_t)(32 * i + it * RPI) * a.lddact;
+            store_any<true, float, 8>(dp, left, d);
           }
         }
         store_any<true, T, 8>(out, left, v);

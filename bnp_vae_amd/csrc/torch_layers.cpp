@@ -293,7 +293,7 @@ std::tuple<Tensor, Tensor> dense_forward(const Tensor& x_in, const Tensor& w_in,
   const int64_t M = x.size(0), K = x.size(1), n = w.t.size(-2), G = w.t.dim() == 3 ? w.t.size(0) : 0;
   const int type = type_of(x);
   Tensor y = at::empty({M, n}, x.options()), dact, work;
-  if (want_dact && act != BNPVI_ACT_NONE) dact = at::empty({M, n}, x.options().dtype(type == BNPVI_BF16 ? at::kHalf : at::kFloat));
+  if (want_dact && act != BNPVI_ACT_NONE) dact = at::empty({M, n}, x.options().dtype(at::kFloat));
   const int64_t need = dense_workspace(type, M, K, n, G, 0);
   if (need > 0) work = at::empty({need}, x.options().dtype(at::kByte));
   check(lib.dense(ctx_of(ctx), type, ptr(x), pitch(x), ptr(w.t), w.row, w.group, ptr(bias), G > 1 ? n : 0, act, ptr(res),

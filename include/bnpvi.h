@@ -359,8 +359,8 @@ int bnpvi_rows_from_leaves_backward(bnpvi_ctx* ctx, int dtype, const void* dy_de
  * x [M][ldx] (K wide), W [n][ldw], bias [n] or NULL, residual [M][ldres] or NULL (n wide), y [M][ldy].
  * G = 0, offsets NULL: one weight for all rows.  G >= 1 and offsets int32 [G + 1], ascending: rows offsets[g] ..
  * offsets[g + 1] - 1 use W + g w_group and bias + g bias_group (elements); rows of no group get y = 0, and what their
- * x, residual and dy hold is not looked at.  dact NULL, or [M][lddact]: act'(z) for the backward call, in fp16 where
- * dtype is BNPVI_BF16 and in fp32 otherwise.  fp32 accumulation; fp32 inputs are multiplied in fp32.
+ * x, residual and dy hold is not looked at.  dact NULL, or [M][lddact]: act'(z) for the backward call, in fp32 for
+ * every dtype.  fp32 accumulation; fp32 inputs are multiplied in fp32.
  * backward, with dz = dy dact (dact NULL: dz = dy, the case of BNPVI_ACT_NONE), rounded to dtype once:
  *     dx = dz W [M][lddx],  dw[g] = dz_g^T x_g [groups][n][K],  db[g] = sum of dz_g (unrounded) [groups][n],
  *     dres = dy with zeros in the rows of no group [M][lddres]
