@@ -173,16 +173,26 @@ __global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
 }
 
 // ---- dz, residual gradient, partial sums of the bias gradient --------------------------------------------------------
-// One workgroup: a row tile (of one group) x 256 columns.  dz = dy * d rounded once; the bias gradient adds the
-// unrounded products: per thread over its rows, then the eight row threads of a column in order, into `part`, or into `db`
-// where one tile has all rows.  dres (or nullptr): dy, 0 in the rows of no group.  Bound by memory: 131072 x 512 in bf16
-// takes 85 us for 403 MB (4.7 TB/s).
+// One workgroup: a row tile (of one group) x 256 columns.  dz = dy * d, in fp32 rounded once, in 16 bits in two parts
+// hi + lo (dense_kernels.h): |dz - hi - lo| is at most 2^-16 of |dz| in bf16, 2^-22 in fp16 (where lo's smallest step adds
+// 2^-25, half of dy's own).  hi stays finite where dz is -- a dz behind fp16's largest value, which is up to 1.13 dy, is 65504
+// and the rest of it.  The bias gradient adds the unrounded products: per thread over its rows, then the eight row threads
+// of a column in order, into `part`, or into `db` where one tile has all rows.  dres (or nullptr): dy, 0 in the rows of no
+// group.  Bound by memory: 131072 x 512 in bf16 takes 130 us for 671 MB (5.1 TB/s).
+template <typename T>
+__device__ __forceinline__ void two_parts(float v, T& hi, T& lo) {
+  constexpr float most = std::is_same<T, bf16_t>::value ? 3.3895313892515355e38f : 65504.f;
+  const bool finite = fabsf(v) < __builtin_inff();
+  hi = (T)(finite ? fminf(fmaxf(v, -most), most) : v);
+  lo = (T)(finite ? v - (float)hi : 0.f);
+}
+
 constexpr int kDzRows = 128;
 
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64_t lddy, const float* __restrict__ d, int64_t ldd,
-                                                 const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz,
-                                                 int64_t lddz, T* __restrict__ dres, int64_t lddres, float* __restrict__ part,
+                                                 const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz, int64_t lddz,
+                                                 T* __restrict__ dres, int64_t lddres, float* __restrict__ part,
                                                  T* __restrict__ db) {
   constexpr int CT = 32, E = 8;              // threads across, columns a thread
   __shared__ float sums[8][CT * E + 1];
@@ -199,7 +209,8 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (inside > 0) {
+  constexpr bool PAIR = sizeof(T) == 2;
+  if (inside > 0 || (PAIR && dz != nullptr && 2 * c < lddz)) {
 #pragma unroll 2
     for (int64_t r = r0 + ty; r < r1; r += 8) {
       float v[E], o[E];
@@ -215,8 +226,21 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
         load_any<float, E>(d + r * ldd + c, inside, o);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] *= o[e];
-        // rows of dz end on 16 bytes, with zeros behind column n
-        if (dz != nullptr) store_any<false, T, E>(dz + r * lddz + c, (int)(lddz - c), v);
+        if (dz != nullptr) {
+          if constexpr (PAIR) {          // zeros behind column n up to the end of its 32
+            union {
+              u32x4 u;
+              T t[E];
+            } hi, lo;
+#pragma unroll
+            for (int e = 0; e < E; ++e) two_parts<T>(v[e], hi.t[e], lo.t[e]);
+            T* at = dz + r * lddz + (c / 32) * 64 + c % 32;
+            *reinterpret_cast<u32x4*>(at) = hi.u;
+            *reinterpret_cast<u32x4*>(at + 32) = lo.u;
+          } else {                       // zeros behind column n up to a whole 16 bytes
+            store_any<false, T, E>(dz + r * lddz + c, (int)(lddz - c), v);
+          }
+        }
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] += v[e];
@@ -478,7 +502,7 @@ static void tile_size(int tile, int& br, int& bc) {
 }
 
 // rows x cols of output, `K` summed; grouped: G groups along the rows (kFwd, kDx) or along the sum (kDw); direct: all
-// operands' rows start on 16 bytes.
+// operands' rows start on 16 bytes; pair: R in two parts, 32 k's a stage.
 //
 // The tile and the number of parts of the sum are the cheapest by what was measured.  A stage of 128 bytes of k takes a
 // workgroup the microseconds below, by how many of them share a CU (8192^3 in 16 bits: 64 / 128 / 256 wide tiles make 384 /
@@ -495,15 +519,15 @@ static void tile_size(int tile, int& br, int& bc) {
 // dW with groups: leaves are unequal, and a launch waits for its longest tile.  A leaf longer than `piece` frames is summed
 // in pieces; the shorter they are the evener the end (half a piece is idle on average), the more partial results pass
 // through memory.
-static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64_t K, bool grouped, int G, bool direct) {
+static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64_t K, bool grouped, int G, bool direct, bool pair = false) {
   GemmPlan p;
-  const int e = dtype_bytes(dtype), bk = 128 / e;
+  const int e = dtype_bytes(dtype), bk = pair ? 32 : 128 / e;
   const bool by_rows = grouped && kind != kDw;
   const bool by_sum = grouped && kind == kDw;
   const int64_t per_group = by_rows ? ceil_div(rows, G) : rows;
   p.piece = p.entries = p.parts = 0;
   p.splits = 1;
-  if (cols <= 32 && per_group > 32) {
+  if (cols <= 32 && per_group > 32 && !pair) {
     p.tile = kTileTall;
   } else if (per_group <= (by_rows ? (e == 4 ? 256 : 96) : 32)) {
     p.tile = kTileFlat;
@@ -590,12 +614,14 @@ static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 struct Ways {
   bool fwd, dx, dw;            // the products may load straight into LDS
   bool copy_fwd, copy_bwd;     // operands that do not lie so are copied first
+  bool pair;                   // dz in two 16-bit parts
 };
 
 struct DensePlan {
   GemmPlan fwd, dx, dw;
   bool grouped;
   int64_t dz_tiles, Kp, np;    // pitches of whole 16 bytes
+  int64_t dz_pitch;            // of dz, or of the copy of dy in its place
   // byte offsets of the workspace's parts
   size_t fwd_map, fwd_slab, fwd_x, fwd_w, fwd_bytes, bwd_x, bwd_w;
   size_t dz_map, dz_first, dx_map, dw_map, dw_sums, dw_count, part, dz, slab, db_slab, bwd_bytes;
@@ -609,6 +635,7 @@ static bool copy_pays(double flops_fwd, double flops_bwd, int e, int64_t M, int6
 }
 
 static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, const Ways& ways) {
+  const bool pair = ways.pair;
   DensePlan p;
   const int e = dtype_bytes(dtype), per = 16 / e;
   const int64_t weights = n * (G > 0 ? G : 1);
@@ -616,8 +643,8 @@ static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, c
   p.Kp = (K + per - 1) / per * per;
   p.np = (n + per - 1) / per * per;
   p.fwd = gemm_plan(kFwd, dtype, M, n, K, p.grouped, G, ways.fwd);
-  p.dx = gemm_plan(kDx, dtype, M, K, n, p.grouped, G, ways.dx);
-  p.dw = gemm_plan(kDw, dtype, n, K, M, p.grouped, G, ways.dw);
+  p.dx = gemm_plan(kDx, dtype, M, K, n, p.grouped, G, ways.dx, pair);
+  p.dw = gemm_plan(kDw, dtype, n, K, M, p.grouped, G, ways.dw, pair);
   p.dz_tiles = ceil_div(M, kDzRows) + (p.grouped ? G + 2 : 0);
   const bool vector = as_vectors(M, K, n, G);
   size_t at = 0;
@@ -639,7 +666,8 @@ static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, c
   p.dw_sums = take((size_t)p.dw.parts / 2 * sizeof(int4));
   p.dw_count = take(p.grouped ? 8 : 0);
   p.part = take((size_t)p.dz_tiles * n * 4);
-  p.dz = take((size_t)M * p.np * e);
+  p.dz_pitch = pair ? (n + 31) / 32 * 64 : p.np;
+  p.dz = take((size_t)M * p.dz_pitch * e);
   p.slab = take(std::max(p.dx.slab, p.dw.slab));
   p.db_slab = take((size_t)(p.grouped ? p.dw.parts : p.dw.splits > 1 ? p.dw.splits : 0) * n * 4);
   p.bwd_x = take(ways.copy_bwd ? (size_t)M * p.Kp * e : 0);
@@ -669,13 +697,13 @@ static bool aligned(const void* p, int64_t ld, int64_t group, int64_t extent, in
   return (((uint64_t)(uintptr_t)p | (uint64_t)(ld * e) | (uint64_t)(group * e) | (uint64_t)(extent * e)) & 15) == 0;
 }
 
-static int run_gemm(int kind, int dtype, const GemmPlan& p, bool direct, GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s) {
+static int run_gemm(int kind, int dtype, const GemmPlan& p, bool direct, bool pair, GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s) {
   a.row_tiles = (int)p.row_tiles;
   a.col_tiles = p.col_tiles;
   a.splits = p.splits;
-  return dtype == BNPVI_F32    ? launch_gemm_f32(kind, p.tile, direct, a, ctx, s)
-         : dtype == BNPVI_BF16 ? launch_gemm_bf16(kind, p.tile, direct, a, ctx, s)
-                               : launch_gemm_f16(kind, p.tile, direct, a, ctx, s);
+  return dtype == BNPVI_F32    ? launch_gemm_f32(kind, p.tile, direct, pair, a, ctx, s)
+         : dtype == BNPVI_BF16 ? launch_gemm_bf16(kind, p.tile, direct, pair, a, ctx, s)
+                               : launch_gemm_f16(kind, p.tile, direct, pair, a, ctx, s);
 }
 
 static int launch_maps(const MapArgs& a, int device, hipStream_t s) {
@@ -751,8 +779,8 @@ int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G,
   // enough for every way of loading: which one it is goes by the addresses of the call
   const bool cf = copies_fwd(dtype, M, K, n, G), cb = copies_bwd(dtype, M, K, n, G);
   size_t most = 0;
-  for (int i = 0; i < 8; ++i) {
-    const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{(i & 1) != 0, (i & 2) != 0, (i & 4) != 0, cf, cb});
+  for (int i = 0; i < (backward && dtype_bytes(dtype) == 2 ? 16 : 8); ++i) {
+    const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{(i & 1) != 0, (i & 2) != 0, (i & 4) != 0, cf, cb, (i & 8) != 0});
     most = std::max(most, backward ? p.bwd_bytes : p.fwd_bytes);
   }
   return (int64_t)most;
@@ -773,7 +801,7 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
   const int e = dtype_bytes(dtype);
   const bool x_lies = aligned(x, ldx, 0, K, e), w_lies = aligned(w, ldw, G > 1 ? w_group : 0, K, e);
   const bool copy = !(x_lies && w_lies) && copies_fwd(dtype, M, K, n, G), direct = copy || (x_lies && w_lies);
-  const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{direct, true, true, copy, false});
+  const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{direct, true, true, copy, false, false});
   BNPVI_REQUIRE(work_bytes >= (int64_t)p.fwd_bytes && (p.fwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
                 "bnpvi_dense: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes, (long long)p.fwd_bytes);
   OnDevice on(ctx->device);
@@ -837,7 +865,7 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
     }
     BNPVI_LAUNCH_CHECK();
   }
-  const int r = run_gemm(kFwd, dtype, p.fwd, direct, a, ctx, s);
+  const int r = run_gemm(kFwd, dtype, p.fwd, direct, false, a, ctx, s);
   if (r) return r;
   if (p.fwd.slab) {
     const unsigned g = flat_grid(M * n);
@@ -862,11 +890,11 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
                     (!dw || pitch_fits(ldx, K, dtype)) && (!dres || lddres >= n),
                 "bnpvi_dense_backward: a row pitch is below its width, or above 4 MiB");
   const int e = dtype_bytes(dtype);
-  // dz is dy, or lies in the workspace in rows of whole 16 bytes
+  // dz is dy, or lies in the workspace in rows of whole 16 bytes, in 16 bits in two parts
   const bool dz_lies = dact != nullptr || aligned(dy, lddy, 0, n, e);
   const bool w_lies = !dx || aligned(w, ldw, G > 1 ? w_group : 0, K, e), x_lies = !dw || aligned(x, ldx, 0, K, e);
   const bool copy = M > 0 && (dx || dw) && !(dz_lies && w_lies && x_lies) && copies_bwd(dtype, M, K, n, G);
-  const Ways ways = {true, copy || (dz_lies && w_lies), copy || (dz_lies && x_lies), false, copy};
+  const Ways ways = {true, copy || (dz_lies && w_lies), copy || (dz_lies && x_lies), false, copy, dact != nullptr && e == 2};
   const DensePlan p = dense_plan(dtype, M, K, n, G, ways);
   BNPVI_REQUIRE(work_bytes >= (int64_t)p.bwd_bytes && (p.bwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
                 "bnpvi_dense_backward: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes,
@@ -882,8 +910,8 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   int32_t* first = nullptr;
   const bool none = M == 0;
   // Without an activation the products read dy itself and dW's kernel adds up its rows for the bias on the way
-  // (16385 x 64 -> 4096 fp32: 70 us of 450 were a pass over dy for that).  With one, dz is rounded to 16 bits before dW's
-  // kernel sees it, so that there only fp32 does the same.
+  // (16385 x 64 -> 4096 fp32: 70 us of 450 were a pass over dy for that).  With one, dW's kernel sees 16 bits of dz in
+  // two parts, so that there only fp32 does the same.
   const bool db_in_dw = db && dw && (!dact || dtype == BNPVI_F32) && p.dw.tile != kTile256;
   const bool need_dz = (dact != nullptr && (dx || dw)) || (db && !db_in_dw) || dres;
   if (G > 0) {
@@ -923,17 +951,17 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   if (need_dz && !none) {
     void* out = dact ? (void*)(wk + p.dz) : nullptr;
     if (dtype == BNPVI_F32)
-      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, p.np, (float*)dres, lddres, part, db_in_dz, s);
+      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, p.dz_pitch, (float*)dres, lddres, part, db_in_dz, s);
     else if (dtype == BNPVI_BF16)
-      launch_dz<bf16_t>((const bf16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (bf16_t*)out, p.np, (bf16_t*)dres, lddres, part,
+      launch_dz<bf16_t>((const bf16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (bf16_t*)out, p.dz_pitch, (bf16_t*)dres, lddres, part,
                         db_in_dz, s);
     else
-      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, p.np, (f16_t*)dres, lddres, part, db_in_dz,
+      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, p.dz_pitch, (f16_t*)dres, lddres, part, db_in_dz,
                        s);
     BNPVI_LAUNCH_CHECK();
     if (dact) {
       dz = out;
-      lddz = p.np;
+      lddz = p.dz_pitch;
     }
   }
   if (db && !db_in_dw && !db_in_dz) {
@@ -982,7 +1010,7 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.ldc = lddx;
     if (G > 0) a.map = (const int4*)(wk + p.dx_map);
     if (p.dx.slab) a.slab = (float*)(wk + p.slab);
-    r = run_gemm(kDx, dtype, p.dx, ways.dx, a, ctx, s);
+    r = run_gemm(kDx, dtype, p.dx, ways.dx, ways.pair, a, ctx, s);
     if (r) return r;
     if (p.dx.slab) {
       // no epilogue: a plain sum over the splits into rows of pitch lddx
@@ -1020,7 +1048,7 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
       a.db = db;
       if (p.dw.slab) a.db_slab = (float*)(wk + p.db_slab);
     }
-    r = run_gemm(kDw, dtype, p.dw, ways.dw, a, ctx, s);
+    r = run_gemm(kDw, dtype, p.dw, ways.dw, ways.pair, a, ctx, s);
     if (r) return r;
     if (p.dw.slab) {
       const int4* sums = (const int4*)(wk + p.dw_sums);

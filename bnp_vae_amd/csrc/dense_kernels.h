@@ -173,7 +173,7 @@ struct Source {
   static __device__ __forceinline__ int row(int q) { return (q * THREADS + (int)threadIdx.x) / kRow; }
   static __device__ __forceinline__ int piece(int q) {
     const int r = row(q), c = (q * THREADS + (int)threadIdx.x) % kRow;
-    if (KM) return c ^ swizzle<KB>(r);
+    if constexpr (KM) return c ^ swizzle<KB>(r);
     if (sizeof(T) == 2) return (((c >> 1) ^ (r & (kUnits - 1))) << 1) | (c & 1);
     return c;
   }
@@ -296,17 +296,34 @@ template <typename T, bool KM, int B, int KB>
 struct Reader {
   int off[4];      // KM: byte offset of each k-step's piece; 16-bit MM: of each pair (first / second four k's)
   int lane;
+  int at;          // 16-bit MM: of the first pair of fragment 0 at k-step 0; the others differ in bits of the unit and in rows
   __device__ __forceinline__ void init(int row0) {
     lane = threadIdx.x & 63;
     const int i = lane & 31, h = lane >> 5;
-    if (KM) {
+    if constexpr (KM) {
 #pragma unroll
       for (int s = 0; s < KB / 32; ++s) off[s] = (row0 + i) * KB + (((2 * s + h) ^ swizzle<KB>(i)) << 4);
     } else if (sizeof(T) == 2) {
       off[0] = (h * 8 + ((lane & 15) >> 2)) * (B * 2) + (lane & 3) * 8;     // the unit is added per fragment
       off[1] = row0 / 16 + ((lane >> 4) & 1);
+      at = off[0] + ((off[1] ^ ((h * 8 + ((lane & 15) >> 2)) & (B / 16 - 1))) << 5);
     } else {
       off[0] = h * 4 * (B * 4) + (row0 + i) * 4;
+    }
+  }
+  // The same fragment by one exclusive-or and one addition, made anew in every stage: kept in registers the addresses of all
+  // fragments spill (dz in two parts, 256 x 256: 31 registers, dW of 65536 x 4096 -> 256 309 us,
+  // so 300).
+  __device__ __forceinline__ void anew() {
+    if constexpr (!KM && sizeof(T) == 2) asm volatile("" : "+v"(at));
+  }
+  __device__ __forceinline__ typename Frag<T>::type get_anew(const char* lds, int f, int s) const {
+    if constexpr (!KM && sizeof(T) == 2) {
+      constexpr int U = B / 16, W = B * 2;
+      const int u = (2 * f) ^ (16 * s & (U - 1));
+      return Frag<T>::transposed(lds + ((at ^ (u << 5)) + s * 16 * W), lds + ((at ^ ((u ^ (4 & (U - 1))) << 5)) + (s * 16 + 4) * W));
+    } else {
+      return get(lds, f, s);
     }
   }
   __device__ __forceinline__ typename Frag<T>::type get(const char* lds, int f, int s) const {
@@ -338,17 +355,37 @@ __device__ __forceinline__ void wait_loads() {
 // Workgroup tile BR x BC, wave tile WR x WC, stages of KB bytes of k.  The operand that comes from far (x or dz in the
 // forward and dx products, x in the dW product) has a ring of three stages in LDS, the other one of two; through
 // registers both have two.  One barrier a stage.
-template <int BR, int BC, int KB, int KIND, bool DIRECT>
+//
+// PAIR: R is dz in two 16-bit parts, hi + lo, since dx and dW of one 16-bit part are 1.4 times as far from the exact ones as
+// a single rounding of the results (0.0024 against 0.0017 relative in bf16).  A row of it holds 32 columns of hi, 32 of lo,
+// and so on, so that a stage is as many bytes as ever, of half as many k's (dx) or of both parts of its columns (dW); S's
+// stages are half as long, and each of its fragments is multiplied with both parts.  That is twice the
+// instructions: 65536 x 4096 -> 256 in bf16 takes 282 / 300 us for dx / dW, from one part 200 / 175; 32768 x 1024 -> 1024 takes
+// 135 / 148, from one part 82 / 92 (920 to 1020 TFLOP/s of the doubled products).
+template <int KIND, bool PAIR, int BR, int BC, int KB>
+struct Stages {
+  static constexpr bool kRKM = KIND != kDw, kSKM = KIND == kFwd;
+  static constexpr int kRRows = PAIR && !kRKM ? 2 * BR : BR, kRBytes = PAIR && !kRKM ? KB / 2 : KB;      // rows and k bytes of R's stage
+  static constexpr int kSBytes = PAIR ? KB / 2 : KB;
+};
+template <int BR, int BC, int WR, int WC, int KB, int KIND, bool DIRECT, bool PAIR>
 struct Rings {
   static constexpr int kR = DIRECT && KIND != kDw ? 3 : 2, kS = DIRECT && KIND == kDw ? 3 : 2;
-  static constexpr int kBytes = (kR * BR + kS * BC) * KB;
+  static constexpr int kRStage = BR * KB, kSStage = BC * Stages<KIND, PAIR, BR, BC, KB>::kSBytes;
+  // the epilogue takes 32 rows of every wave at once: as many waves as fit in a stage of R, then of S, the others behind
+  static constexpr int kEp = 32 * WC * 4, kWaves = (BR / WR) * (BC / WC);
+  static constexpr int kRWaves = kRStage / kEp < kWaves ? kRStage / kEp : kWaves;
+  static constexpr int kSWaves = kSStage / kEp < kWaves - kRWaves ? kSStage / kEp : kWaves - kRWaves;
+  static constexpr int kBehind = kR * kRStage + kS * kSStage;
+  static constexpr int kBytes = kBehind + (kWaves - kRWaves - kSWaves) * kEp;
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
-// the dW kernel can add up the rows of R for the bias, but not where its accumulators already fill the registers
-template <int KIND, int BR>
-constexpr bool kRowSums = KIND == kDw && BR < 256;
+// the dW kernel can add up the rows of R for the bias, but not where its accumulators already fill the registers; with an
+// activation in 16 bits the pass that makes dz's two parts does that
+template <int KIND, int BR, bool PAIR>
+constexpr bool kRowSums = KIND == kDw && BR < 256 && !PAIR;
 
 // One output tile: its place in C, its group, its part of the sum.
 struct Tile {
@@ -410,11 +447,12 @@ __device__ __forceinline__ bool find_tile(const GemmArgs& a, uint32_t lin, const
 }
 
 // The stages of one operand, tile after tile of this workgroup, in the order in which they are multiplied.
-template <typename T, int KIND, int BR, int BC, int KB, int THREADS, bool ROWS>
+template <typename T, int KIND, bool PAIR, int BR, int BC, int KB, int THREADS, bool ROWS>
 struct Stream {
-  static constexpr bool kKM = ROWS ? KIND != kDw : KIND == kFwd;
-  static constexpr int kBK = KB / (int)sizeof(T);
-  typedef Source<T, kKM, ROWS ? BR : BC, THREADS, KB> Src;
+  typedef Stages<KIND, PAIR, BR, BC, KB> St;
+  static constexpr bool kKM = ROWS ? St::kRKM : St::kSKM;
+  static constexpr int kBK = St::kSBytes / (int)sizeof(T);
+  typedef Source<T, kKM, ROWS ? St::kRRows : BC, THREADS, ROWS ? St::kRBytes : St::kSBytes> Src;
   Src src;
   uint32_t lin, last, inc, twice;
   Share sh;
@@ -437,7 +475,10 @@ struct Stream {
       inc = twice - inc;
       if (found) {
         const int g = t.g < 0 ? 0 : t.g;
-        if (ROWS)
+        if (ROWS && PAIR)          // both parts of whole 32s of columns
+          src.init(reinterpret_cast<const T*>(a.R) + (kKM ? t.row0 * a.ldr + 2 * t.k_lo : t.k_lo * a.ldr + 2 * t.row0), a.ldr,
+                   kKM ? t.nr : 2 * ((t.nr + 31) & ~31), kKM ? 2 * ((t.kext + 31) & ~31) : t.kext);
+        else if (ROWS)
           src.init(reinterpret_cast<const T*>(a.R) + (kKM ? t.row0 * a.ldr + t.k_lo : t.k_lo * a.ldr + t.row0), a.ldr, t.nr, t.kext);
         else
           src.init(reinterpret_cast<const T*>(a.S) + (KIND == kDw ? 0 : g * a.s_group) +
@@ -459,15 +500,16 @@ struct Stream {
 // XCDs in turn; every XCD owns a contiguous run of tiles, columns first, which its workgroups walk side by side, so that
 // the tiles that share rows of R share an L2.  The operands' stages follow each other across tiles, so the next tile
 // arrives while the last stages of this one are multiplied and while its epilogue runs.
-template <typename T, int KIND, int BR, int BC, int WR, int WC, int KB, bool DIRECT>
+template <typename T, int KIND, int BR, int BC, int WR, int WC, int KB, bool DIRECT, bool PAIR>
 __global__ __launch_bounds__((BR / WR) * (BC / WC) * 64) __attribute__((amdgpu_waves_per_eu(BR * BC >= 128 * 128 ? 2 : 4)))
 void gemm_kernel(const GemmArgs a, uint32_t tiles) {
   constexpr int THREADS = (BR / WR) * (BC / WC) * 64, WAVES = THREADS / 64;
-  constexpr bool RKM = KIND != kDw, SKM = KIND == kFwd;
-  constexpr int FR = WR / 32, FC = WC / 32, BK = KB / (int)sizeof(T);
-  typedef Rings<BR, BC, KB, KIND, DIRECT> Ring;
+  static_assert(!PAIR || (sizeof(T) == 2 && KIND != kFwd), "dz of 16 bits in two parts");
+  typedef Stages<KIND, PAIR, BR, BC, KB> St;
+  constexpr int FR = WR / 32, FC = WC / 32, BK = St::kSBytes / (int)sizeof(T);
+  typedef Rings<BR, BC, WR, WC, KB, KIND, DIRECT, PAIR> Ring;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  char* const ring_s = lds + Ring::kR * BR * KB;
+  char* const ring_s = lds + Ring::kR * Ring::kRStage;
 
   const uint32_t xcd = blockIdx.x & 7, q8 = tiles >> 3, rem = tiles & 7;
   const uint32_t step = (gridDim.x + 7 - xcd) >> 3;
@@ -489,23 +531,29 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
   const uint32_t wg = blockIdx.x >> 3, twice = 2 * step;
   uint32_t lin = first + wg, inc = KIND == kDw && a.map != nullptr ? twice - 2 * wg - 1 : step;
   if (lin >= last) return;
-  Stream<T, KIND, BR, BC, KB, THREADS, true> sr;
-  Stream<T, KIND, BR, BC, KB, THREADS, false> ss;
+  Stream<T, KIND, PAIR, BR, BC, KB, THREADS, true> sr;
+  Stream<T, KIND, PAIR, BR, BC, KB, THREADS, false> ss;
   sr.begin(a, lin, last, inc, twice, sh);
   ss.begin(a, lin, last, inc, twice, sh);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave / (BC / WC) * WR, wc = wave % (BC / WC) * WC;
-  Reader<T, RKM, BR, KB> rr;
-  Reader<T, SKM, BC, KB> rs;
-  rr.init(wr);
+  Reader<T, St::kRKM, St::kRRows, St::kRBytes> rr;
+  Reader<T, St::kSKM, BC, St::kSBytes> rs;
+  rr.init(PAIR && !St::kRKM ? 2 * wr : wr);
   rs.init(wc);
+  // step s of a stage: a k-step, or with two parts hi and then lo of k-step s / 2
+  auto get_r = [&](const char* at, int i, int s) {
+    return !PAIR ? rr.get(at, i, s) : St::kRKM ? rr.get(at, i, s / 2 + 2 * (s & 1)) : rr.get_anew(at, 2 * i + (s & 1), s / 2);
+  };
+  auto get_s = [&](const char* at, int j, int s) { return PAIR ? rs.get_anew(at, j, s / 2) : rs.get(at, j, s); };
+  auto slot_s = [](int s) { return PAIR ? (s / 2) & 1 : s & 1; };
 
   u32x4 hr[DIRECT ? 1 : decltype(sr.src)::kP], hs[DIRECT ? 1 : decltype(ss.src)::kP];
   int fill_r = 0, fill_s = 0, use_r = 0, use_s = 0;          // ring positions
   auto load_r = [&] {
     if constexpr (DIRECT) {
-      sr.src.to_lds(sr.kt, lds + fill_r * (BR * KB));
+      sr.src.to_lds(sr.kt, lds + fill_r * Ring::kRStage);
       fill_r = fill_r == Ring::kR - 1 ? 0 : fill_r + 1;
     } else {
       sr.src.fetch(sr.kt, hr);
@@ -514,7 +562,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
   };
   auto load_s = [&] {
     if constexpr (DIRECT) {
-      ss.src.to_lds(ss.kt, ring_s + fill_s * (BC * KB));
+      ss.src.to_lds(ss.kt, ring_s + fill_s * Ring::kSStage);
       fill_s = fill_s == Ring::kS - 1 ? 0 : fill_s + 1;
     } else {
       ss.src.fetch(ss.kt, hs);
@@ -546,15 +594,15 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     // the bias gradient where dz is dy: row sums of R, by the waves that hold the first columns
-    const bool row_sums = kRowSums<KIND, BR> && (a.db != nullptr || a.db_slab != nullptr) && t.col0 == 0 && wc == 0;
+    const bool row_sums = kRowSums<KIND, BR, PAIR> && (a.db != nullptr || a.db_slab != nullptr) && t.col0 == 0 && wc == 0;
     float rsum[FR];
 #pragma unroll
     for (int i = 0; i < FR; ++i) rsum[i] = 0.f;
     const int nk = t.stages(BK);
     auto add_up = [&](auto with_sums) {
     for (int kt = 0; kt < nk; ++kt) {
-      char* const at_r = lds + use_r * (BR * KB);
-      char* const at_s = ring_s + use_s * (BC * KB);
+      char* const at_r = lds + use_r * Ring::kRStage;
+      char* const at_s = ring_s + use_s * Ring::kSStage;
       if constexpr (!DIRECT) {
         sr.src.put(at_r, hr);
         ss.src.put(at_s, hs);
@@ -569,11 +617,15 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
         behind = 0;
       }
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // ... and all waves are done with the one before
+      if constexpr (PAIR) {
+        rr.anew();
+        rs.anew();
+      }
       typename Frag<T>::type fr[2][FR], fc[2][FC];
 #pragma unroll
-      for (int i = 0; i < FR; ++i) fr[0][i] = rr.get(at_r, i, 0);
+      for (int i = 0; i < FR; ++i) fr[0][i] = get_r(at_r, i, 0);
 #pragma unroll
-      for (int j = 0; j < FC; ++j) fc[0][j] = rs.get(at_s, j, 0);
+      for (int j = 0; j < FC; ++j) fc[0][j] = get_s(at_s, j, 0);
       if (DEEP_S) {
         load_r();
         load_s();
@@ -585,9 +637,11 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
       for (int s = 0; s < KB / 32; ++s) {       // the next k-step's fragments are read while this one's are multiplied
         if (s + 1 < KB / 32) {
 #pragma unroll
-          for (int i = 0; i < FR; ++i) fr[(s + 1) & 1][i] = rr.get(at_r, i, s + 1);
+          for (int i = 0; i < FR; ++i) fr[(s + 1) & 1][i] = get_r(at_r, i, s + 1);
+          if (!PAIR || (s & 1)) {
 #pragma unroll
-          for (int j = 0; j < FC; ++j) fc[(s + 1) & 1][j] = rs.get(at_s, j, s + 1);
+            for (int j = 0; j < FC; ++j) fc[slot_s(s + 1)][j] = get_s(at_s, j, s + 1);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -595,7 +649,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
 #pragma unroll
           for (int i = 0; i < FR; ++i)
 #pragma unroll
-            for (int j = 0; j < FC; ++j) Frag<T>::mma(fc[s & 1][j], fr[s & 1][i], acc[i][j], u);
+            for (int j = 0; j < FC; ++j) Frag<T>::mma(fc[slot_s(s)][j], fr[s & 1][i], acc[i][j], u);
         if constexpr (decltype(with_sums)::value) {
 #pragma unroll
           for (int i = 0; i < FR; ++i) rsum[i] = Frag<T>::sum(fr[s & 1][i], rsum[i]);
@@ -606,7 +660,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
       use_s = use_s == Ring::kS - 1 ? 0 : use_s + 1;
     }
     };
-    if constexpr (kRowSums<KIND, BR>) {
+    if constexpr (kRowSums<KIND, BR, PAIR>) {
       if (row_sums)
         add_up(std::true_type());
       else
@@ -614,7 +668,7 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
     } else {
       add_up(std::false_type());
     }
-    if (kRowSums<KIND, BR> && row_sums) {
+    if (kRowSums<KIND, BR, PAIR> && row_sums) {
 #pragma unroll
       for (int i = 0; i < FR; ++i) {
         const float sum = rsum[i] + __shfl_xor(rsum[i], 32);
@@ -629,12 +683,12 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
     }
 
     // ---- epilogue, 32 rows of the wave's tile at a time through the stages just multiplied, which nothing fills before
-    // the next barrier.  A lane holds four consecutive columns of one row; 16-byte slot s of row r lies at
+    // the next barrier (and the LDS behind the rings, where those are short).  A lane holds four consecutive columns of one row; 16-byte slot s of row r lies at
     // s ^ (r mod slots), so that eight rows written at the same column fall on different banks.
-    constexpr int EP = 32 * WC * 4, R_WAVES = BR * KB / EP < WAVES ? BR * KB / EP : WAVES;
-    static_assert(R_WAVES + BC * KB / EP >= WAVES, "the epilogue fits the two stages");
-    char* const mine = wave < R_WAVES ? lds + (use_r == 0 ? Ring::kR - 1 : use_r - 1) * (BR * KB) + wave * EP
-                                      : ring_s + (use_s == 0 ? Ring::kS - 1 : use_s - 1) * (BC * KB) + (wave - R_WAVES) * EP;
+    char* const mine = wave < Ring::kRWaves ? lds + (use_r == 0 ? Ring::kR - 1 : use_r - 1) * Ring::kRStage + wave * Ring::kEp
+                       : wave < Ring::kRWaves + Ring::kSWaves
+                           ? ring_s + (use_s == 0 ? Ring::kS - 1 : use_s - 1) * Ring::kSStage + (wave - Ring::kRWaves) * Ring::kEp
+                           : lds + Ring::kBehind + (wave - Ring::kRWaves - Ring::kSWaves) * Ring::kEp;
     const int c = lane % LPR, cl = wc + 8 * c;
     const int64_t col = t.col0 + cl;
     const int left = t.nc - cl < 8 ? t.nc - cl : 8;
@@ -789,8 +843,8 @@ void gemm_kernel(const GemmArgs a, uint32_t tiles) {
   if constexpr (DIRECT) wait_loads<0>();         // the zeros behind the last tile: nothing may write into the next workgroup's LDS
 }
 
-int launch_gemm_f32(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
-int launch_gemm_bf16(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
-int launch_gemm_f16(int kind, int tile, bool direct, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
+int launch_gemm_f32(int kind, int tile, bool direct, bool pair, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
+int launch_gemm_bf16(int kind, int tile, bool direct, bool pair, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
+int launch_gemm_f16(int kind, int tile, bool direct, bool pair, const GemmArgs& a, const bnpvi_ctx* ctx, hipStream_t s);
 
 }  // namespace bnpvi

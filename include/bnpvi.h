@@ -361,7 +361,8 @@ int bnpvi_rows_from_leaves_backward(bnpvi_ctx* ctx, int dtype, const void* dy_de
  * offsets[g + 1] - 1 use W + g w_group and bias + g bias_group (elements); rows of no group get y = 0, and what their
  * x, residual and dy hold is not looked at.  dact NULL, or [M][lddact]: act'(z) for the backward call, in fp32 for
  * every dtype.  fp32 accumulation; fp32 inputs are multiplied in fp32.
- * backward, with dz = dy dact (dact NULL: dz = dy, the case of BNPVI_ACT_NONE), rounded to dtype once:
+ * backward, with dz = dy dact (dact NULL: dz = dy, the case of BNPVI_ACT_NONE), in fp32 and in 16 bits in two parts of
+ * dtype, so that each result below is rounded to 16 bits once:
  *     dx = dz W [M][lddx],  dw[g] = dz_g^T x_g [groups][n][K],  db[g] = sum of dz_g (unrounded) [groups][n],
  *     dres = dy with zeros in the rows of no group [M][lddres]
  * each NULL where it is not wanted; a group without rows gets zeros, and so does dx in the rows of no group.
