@@ -13,6 +13,10 @@ from test_gpu_layers import HALF, TINY, TYPES, act64, gpu, rand, within
 
 pytestmark = pytest.mark.gpu
 
+# dz = dy act'(z) is held in two 16-bit parts: off by 2^-16 of itself in bf16 and 2^-22 in fp16, and where the second part
+# is as small as the type's smallest step by half of that.
+PARTS = {torch.bfloat16: (2.0 ** -16, 2.0 ** -134), torch.float16: (2.0 ** -22, 2.0 ** -25)}
+
 
 @pytest.fixture(scope="module")
 def layers():
@@ -44,10 +48,29 @@ def test_small_derivatives_keep_their_bits(layers, act, most, M):
     within(dx[:, 0], want, (2 * 2.0 ** -8 + 2.0 ** -14) * want.abs() + TINY[T])
 
 
+@pytest.mark.parametrize("dtype,most", [("bf16", 13.0), ("f16", 5.5)])
+@pytest.mark.parametrize("M", [8, 160])
+def test_the_tail_of_gelu(layers, dtype, most, M):
+    """gelu(z) and its derivative for negative z, relative to themselves: one rounding, and 2^-14 for the distribution
+    function (2^-20) and exp2 (2^-15).  A result below the type's normal range is off by half of
+    its smallest step."""
+    T = TYPES[dtype]
+    z = -torch.linspace(0.25, most, M).to(T)
+    x, w = torch.zeros((M, 16), dtype=T), torch.zeros((8, 16), dtype=T)
+    x[:, 0], w[0, 0] = z, 1
+    X = gpu(x).requires_grad_(True)
+    y = layers.dense(X, gpu(w), activation="gelu")
+    dy = torch.zeros((M, 8), dtype=T)
+    dy[:, 0] = 1
+    dx, = torch.autograd.grad(y, X, gpu(dy))
+    value, slope = act64("gelu", z.double())
+    within(y[:, 0], value, (HALF[T] + 2.0 ** -14) * value.abs() + TINY[T] / 2, "y")
+    # the slope passes 0 at z = -0.75: relative to its two terms there
+    terms = 0.5 * torch.erfc(-z.double() / math.sqrt(2)) + z.double().abs() * torch.exp(-z.double() ** 2 / 2) / math.sqrt(2 * math.pi)
+    within(dx[:, 0], slope, HALF[T] * slope.abs() + 2.0 ** -14 * terms + PARTS[T][0] * slope.abs() + TINY[T] / 2, "dx")
+
+
 # ------------------------------------------------------------------------------------------------ dz in 16 bits
-# dz = dy act'(z) is held in two 16-bit parts: off by 2^-16 of itself in bf16 and 2^-22 in fp16, and where the second part
-# is as small as the type's smallest step by half of that.
-PARTS = {torch.bfloat16: (2.0 ** -16, 2.0 ** -134), torch.float16: (2.0 ** -22, 2.0 ** -25)}
 
 
 def quarters(shape, seed):
