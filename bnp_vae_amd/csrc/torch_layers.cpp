@@ -113,6 +113,13 @@ variable_list once(variable_list grads, const variable_list& given, const variab
   return all;
 }
 
+// A tangent of forward-mode differentiation would be dropped without a word: the results here carry none.
+void no_tangents(std::initializer_list<const Tensor*> list) {
+  for (const Tensor* t : list)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw Failure("the layer operators have no forward-mode derivative (an input is a dual tensor)");
+}
+
 bool needs(const Tensor& t) { return t.defined() && t.requires_grad(); }
 std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
@@ -153,6 +160,7 @@ struct TopLeaves : Function<TopLeaves> {
 };
 
 std::tuple<Tensor, Tensor> top_leaves(const Tensor& phi, int64_t L, int64_t k, bool renorm, int64_t ctx) {
+  no_tangents({&phi});
   if (at::GradMode::is_enabled() && phi.requires_grad()) {
     auto out = TopLeaves::apply(phi, L, k, renorm, ctx);
     return {out[0], out[1]};
@@ -239,12 +247,14 @@ struct Combine : Function<Combine> {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets, int64_t ctx) {
+  no_tangents({&x});
   if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, place, offsets, ctx);
   return to_leaves(x, place, offsets, ctx);
 }
 
 Tensor combine(const Tensor& ys, const Tensor& place, const Tensor& offsets, const std::optional<Tensor>& weight, int64_t ctx) {
   const Tensor w = weight ? weight->contiguous() : Tensor();
+  no_tangents({&ys, &w});
   if (at::GradMode::is_enabled() && (ys.requires_grad() || needs(w)))
     return Combine::apply(ys, maybe(w), place, offsets, ctx);
   return from_leaves(ys, place, offsets, w, ctx);
@@ -341,6 +351,7 @@ struct Dense : Function<Dense> {
 Tensor dense(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& res,
              const std::optional<Tensor>& offsets, int64_t act, int64_t ctx) {
   const Tensor b = bias.value_or(Tensor()), r = res.value_or(Tensor()), o = offsets ? offsets->contiguous() : Tensor();
+  no_tangents({&x, &w, &b, &r});
   if (at::GradMode::is_enabled()) {
     const bool inner = x.requires_grad() || w.requires_grad() || needs(b);
     if (inner || needs(r)) return Dense::apply(x, w, maybe(b), maybe(r), maybe(o), act, ctx, inner);

@@ -12,7 +12,7 @@
 it in its encoder and decoder (/root/reference/src/model.py:70-94); the rest has no counterpart there.
 
 Tensors are fp32, bf16 or fp16 on one GPU (responsibilities and weights of leaves fp32); everything is differentiable
-once through torch.autograd, runs on the tensors' device and its current stream, allocates through torch and waits for
+once through torch.autograd (backward; forward-mode tangents are refused), runs on the tensors' device and its current stream, allocates through torch and waits for
 nothing, so it can be captured into a HIP graph (after one call outside a capture).  A backward pass is captured with
 leaves of its own or after every result of an eager pass over the same leaves is gone: torch ties a leaf's gradient node to
 the stream of its first use.  No CPU fallback.

@@ -917,3 +917,23 @@ def test_closest_frames_of_2048_frames_below_a_wide_tree(layers):
     rows, node_s, dist_s = hierarchy._by_leaf(assign, 2500, node, dist)
     want = torch.sort(assign.long(), stable=True).indices
     assert torch.equal(rows, want) and torch.equal(node_s, node[want]) and torch.equal(dist_s, dist[want])
+
+
+# ------------------------------------------------------------------------------------------------ other ways to differentiate or record
+def test_forward_mode_is_an_error(layers):
+    import torch.autograd.forward_ad as fwd
+    x, w, phi = gpu(rand((6, 8), torch.float32, 1)), gpu(rand((5, 8), torch.float32, 2)), torch.rand((6, 4), device="cuda")
+    b, r, one = gpu(rand((5,), torch.float32, 3)), gpu(rand((6, 5), torch.float32, 4)), torch.ones((6, 1), device="cuda")
+    plan = layers.sort_by_leaf(torch.zeros(6, dtype=torch.int32, device="cuda"), 1)
+    calls = [(lambda t: layers.dense(t, w), x), (lambda t: layers.dense(x, t), w), (lambda t: layers.dense(x, w, t), b),
+             (lambda t: layers.dense(x, w, None, "tanh", t), r), (lambda t: layers.dispatch(t, plan), x),
+             (lambda t: layers.combine(t, plan), x), (lambda t: layers.combine(x, plan, t), one), (lambda t: layers.top_leaves(t, 2), phi)]
+    for call, t in calls:
+        for leaf in (t, t.clone().requires_grad_(True)):
+            with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(fwd.make_dual(leaf, torch.ones_like(leaf)))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+    with fwd.dual_level():                            # beside dual tensors the plain ones go their way
+        fwd.make_dual(x.clone(), x)
+        assert torch.equal(layers.dense(x, w), layers.dense(x.clone(), w))

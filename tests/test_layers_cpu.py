@@ -132,3 +132,24 @@ def test_a_sort_without_workspace_has_its_counters_in_the_lds(M, L):
     if not alone:
         c, one = _Ctx(), C.c_void_p(256)
         _fails(_lib.lib.bnpvi_leaf_sort(c.p, one, M, L, one, one, one, None, 0, None), "workspace")
+
+
+def test_dual_tensors_are_refused():
+    """Forward-mode differentiation: a result without its tangent would be a wrong derivative (here below the checks that
+    refuse CPU tensors)."""
+    import torch.autograd.forward_ad as fwd
+    t, plain = torch.rand((4, 8)), torch.rand((4, 8))
+    place, offsets = torch.zeros((4, 1), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    with fwd.dual_level():
+        dual = fwd.make_dual(t, torch.ones_like(t))
+        one = fwd.make_dual(torch.ones(4, 1), torch.ones(4, 1))
+        for call in (lambda: layers._ext.top_leaves(dual, 8, 2, True, 0),
+                     lambda: layers._ext.dispatch(dual, place, offsets, 0),
+                     lambda: layers._ext.combine(dual, place, offsets, None, 0),
+                     lambda: layers._ext.combine(plain, place, offsets, one, 0),
+                     lambda: layers._ext.dense(dual, plain, None, None, None, 0, 0),
+                     lambda: layers._ext.dense(plain, dual, None, None, None, 0, 0),
+                     lambda: layers._ext.dense(plain, plain, one[:, 0], None, None, 0, 0),
+                     lambda: layers._ext.dense(plain, plain[:, :], None, dual[:, :4], None, 0, 0)):
+            with pytest.raises(_lib.BnpviError, match="forward-mode"):
+                call()
