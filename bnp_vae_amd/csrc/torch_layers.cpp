@@ -7,8 +7,10 @@
 #include <mutex>
 #include <unordered_map>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/bnpvi.h"
@@ -120,6 +122,13 @@ void no_tangents(std::initializer_list<const Tensor*> list) {
       throw Failure("the layer operators have no forward-mode derivative (an input is a dual tensor)");
 }
 
+// Recorders of torch calls (torch.jit.trace, make_fx) see the allocation of a result and not the kernel that fills it: the
+// recorded program would give unwritten memory.
+void not_recorded() {
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+    throw Failure("the layer operators cannot be traced: a recorder of torch calls does not see their kernels");
+}
+
 bool needs(const Tensor& t) { return t.defined() && t.requires_grad(); }
 std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
@@ -160,6 +169,7 @@ struct TopLeaves : Function<TopLeaves> {
 };
 
 std::tuple<Tensor, Tensor> top_leaves(const Tensor& phi, int64_t L, int64_t k, bool renorm, int64_t ctx) {
+  not_recorded();
   no_tangents({&phi});
   if (at::GradMode::is_enabled() && phi.requires_grad()) {
     auto out = TopLeaves::apply(phi, L, k, renorm, ctx);
@@ -171,6 +181,7 @@ std::tuple<Tensor, Tensor> top_leaves(const Tensor& phi, int64_t L, int64_t k, b
 
 // ---- sort, dispatch, combine ----------------------------------------------------------------------------------------
 std::tuple<Tensor, Tensor, Tensor> sort_by_leaf(const Tensor& leaf_in, int64_t L, int64_t ctx) {
+  not_recorded();
   const Tensor leaf = leaf_in.contiguous();
   const int64_t N = leaf.size(0), k = leaf.size(1), M = N * k;
   Tensor place = at::empty({N, k}, leaf.options()), order = at::empty({M}, leaf.options()), offsets = at::empty({L + 1}, leaf.options()), work;
@@ -247,12 +258,14 @@ struct Combine : Function<Combine> {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets, int64_t ctx) {
+  not_recorded();
   no_tangents({&x});
   if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, place, offsets, ctx);
   return to_leaves(x, place, offsets, ctx);
 }
 
 Tensor combine(const Tensor& ys, const Tensor& place, const Tensor& offsets, const std::optional<Tensor>& weight, int64_t ctx) {
+  not_recorded();
   const Tensor w = weight ? weight->contiguous() : Tensor();
   no_tangents({&ys, &w});
   if (at::GradMode::is_enabled() && (ys.requires_grad() || needs(w)))
@@ -350,6 +363,7 @@ struct Dense : Function<Dense> {
 
 Tensor dense(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& res,
              const std::optional<Tensor>& offsets, int64_t act, int64_t ctx) {
+  not_recorded();
   const Tensor b = bias.value_or(Tensor()), r = res.value_or(Tensor()), o = offsets ? offsets->contiguous() : Tensor();
   no_tangents({&x, &w, &b, &r});
   if (at::GradMode::is_enabled()) {

@@ -12,10 +12,11 @@
 it in its encoder and decoder (/root/reference/src/model.py:70-94); the rest has no counterpart there.
 
 Tensors are fp32, bf16 or fp16 on one GPU (responsibilities and weights of leaves fp32); everything is differentiable
-once through torch.autograd (backward; forward-mode tangents are refused), runs on the tensors' device and its current stream, allocates through torch and waits for
-nothing, so it can be captured into a HIP graph (after one call outside a capture).  A backward pass is captured with
-leaves of its own or after every result of an eager pass over the same leaves is gone: torch ties a leaf's gradient node to
-the stream of its first use.  No CPU fallback.
+once through torch.autograd (backward: forward-mode tangents are refused, and so are recorders of torch calls such as
+torch.jit.trace), runs on the tensors' device and its current stream, allocates through torch and waits for nothing, so it
+can be captured into a HIP graph (after one call outside a capture).  A backward pass is captured with leaves of its own or
+after every result of an eager pass over the same leaves is gone: torch ties a leaf's gradient node to the stream of its
+first use.  No CPU fallback.
 
 A leaf number outside [0, L) -- `top_leaves` gives -1 -- means "no leaf": such a slot takes part in nothing."""
 from __future__ import annotations

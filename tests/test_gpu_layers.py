@@ -937,3 +937,28 @@ def test_forward_mode_is_an_error(layers):
     with fwd.dual_level():                            # beside dual tensors the plain ones go their way
         fwd.make_dual(x.clone(), x)
         assert torch.equal(layers.dense(x, w), layers.dense(x.clone(), w))
+
+
+def test_tracing_is_an_error(layers):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, phi = gpu(rand((6, 8), torch.float32, 1)), gpu(rand((5, 8), torch.float32, 2)), torch.rand((6, 4), device="cuda")
+    leaf = torch.zeros(6, dtype=torch.int32, device="cuda")
+    plan = layers.sort_by_leaf(leaf, 1)
+    for call, t in ((lambda t: layers.dense(t, w, activation="gelu"), x), (lambda t: layers.dispatch(t, plan), x),
+                    (lambda t: layers.combine(t, plan), x), (lambda t: layers.top_leaves(t, 2)[1], phi),
+                    (lambda t: layers.sort_by_leaf(t, 1).place, leaf)):
+        want = call(t)
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (t,))
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(call)(t)
+        assert torch.equal(call(t), want)
+
+
+def test_functional_transforms_are_errors(layers):
+    x, w = gpu(rand((3, 6, 8), torch.float32, 1)), gpu(rand((5, 8), torch.float32, 2))
+    for call in (lambda: torch.func.vmap(lambda t: layers.dense(t, w))(x),
+                 lambda: torch.func.grad(lambda t: layers.dense(t, w).sum())(x),
+                 lambda: torch.func.vmap(lambda t: layers.top_leaves(t, 2)[1])(x)):
+        with pytest.raises(RuntimeError):
+            call()

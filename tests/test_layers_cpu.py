@@ -153,3 +153,18 @@ def test_dual_tensors_are_refused():
                      lambda: layers._ext.dense(plain, plain[:, :], None, dual[:, :4], None, 0, 0)):
             with pytest.raises(_lib.BnpviError, match="forward-mode"):
                 call()
+
+
+def test_recorders_of_torch_calls_are_refused():
+    """torch.jit.trace and make_fx would record the allocation of the result without its kernel (here below the checks
+    that refuse CPU tensors)."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    t, leaf = torch.rand((4, 8)), torch.zeros((4, 1), dtype=torch.int32)
+    offsets = torch.zeros(4, dtype=torch.int32)
+    for call in (lambda x: layers._ext.top_leaves(x, 8, 2, True, 0)[1], lambda x: layers._ext.dispatch(x, leaf, offsets, 0),
+                 lambda x: layers._ext.combine(x, leaf, offsets, None, 0), lambda x: layers._ext.dense(x, x, None, None, None, 0, 0),
+                 lambda x: layers._ext.sort_by_leaf(leaf, 3, 0)[0] + x[0, 0]):
+        with pytest.raises(_lib.BnpviError, match="traced"):
+            torch.jit.trace(call, (t,))
+        with pytest.raises(_lib.BnpviError, match="traced"):
+            make_fx(call)(t)
