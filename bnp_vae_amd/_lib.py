@@ -85,6 +85,7 @@ EXPORTS = {
     "bnpvi_rows_from_leaves": (_i, [_p, _i, _p, _i64, _p, _p, _p, _i, _i64, _i, _i, _p, _i64, _p]),
     "bnpvi_rows_from_leaves_backward": (_i, [_p, _i, _p, _i64, _p, _i64, _p, _p, _p, _i, _i64, _i, _i, _p, _i64, _p, _p]),
     "bnpvi_dense_workspace": (_i64, [_i, _i64, _i64, _i64, _i, _i]),
+    "bnpvi_dense_workspace_for": (_i64, [_i, _i64, _i64, _i64, _i, _i]),
     "bnpvi_dense": (_i, [_p, _i, _p, _i64, _p, _i64, _i64, _p, _i64, _i, _p, _i64, _p, _i, _i64, _i64, _i64, _p, _i64,
                          _p, _i64, _p, _i64, _p]),
     "bnpvi_dense_backward": (_i, [_p, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i, _i64, _i64, _i64, _p,

@@ -610,22 +610,38 @@ static GemmPlan gemm_plan(int kind, int dtype, int64_t rows, int64_t cols, int64
 
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Which operands lie on 16 bytes, or will after they are copied there
-struct Ways {
-  bool fwd, dx, dw;            // the products may load straight into LDS
-  bool copy_fwd, copy_bwd;     // operands that do not lie so are copied first
-  bool pair;                   // dz in two 16-bit parts
+// What a call's work and workspace go by: sizes, which operands lie on 16 bytes (`aligned`), and for a backward pass what it is
+// given and asked for.
+struct Call {
+  int dtype;
+  int64_t M, K, n;
+  int G;
+  bool x_lies, w_lies, dy_lies;
+  bool dact, dx, dw, db, dres;
 };
 
-struct DensePlan {
-  GemmPlan fwd, dx, dw;
-  bool grouped;
-  int64_t dz_tiles, Kp, np;    // pitches of whole 16 bytes
-  int64_t dz_pitch;            // of dz, or of the copy of dy in its place
-  // byte offsets of the workspace's parts
-  size_t fwd_map, fwd_slab, fwd_x, fwd_w, fwd_bytes, bwd_x, bwd_w;
-  size_t dz_map, dz_first, dx_map, dw_map, dw_sums, dw_count, part, dz, slab, db_slab, bwd_bytes;
+struct ForwardPlan {
+  GemmPlan gemm;
+  bool direct, copy;           // the product loads straight into LDS; operands that do not lie are copied first
+  int64_t Kp;                  // pitch of the copies, whole 16 bytes
+  size_t map, slab, x, w, bytes;      // byte offsets of the workspace's parts, 0 bytes each where the call has no use for them
 };
+
+struct BackwardPlan {
+  GemmPlan dx, dw;
+  bool dx_direct, dw_direct, copy;
+  bool pair;                   // dz in two 16-bit parts
+  bool write_dz, dz_pass;      // dz is not dy; a pass over dy is needed
+  bool db_in_dw, db_in_dz;
+  int64_t dz_tiles, Kp, dz_pitch;     // pitches: of copies of x and W, of dz or of the copy of dy in its place
+  size_t dz_map, dz_first, dx_map, dw_map, dw_sums, dw_count, part, dz, slab, db_slab, x, w, bytes;
+};
+
+static size_t take(size_t& at, size_t bytes) {
+  const size_t o = at;
+  at += up256(bytes);
+  return o;
+}
 
 // Copying pays where the products are large: through registers they run at 0.3 PFLOP/s where straight loads reach 0.65
 // (dW: 0.17 against 0.75; 32768 x 1023 -> 1021 in bf16: 225 / 267 / 399 us forward, dx, dW through registers, 107 / 90 / 90
@@ -634,45 +650,64 @@ static bool copy_pays(double flops_fwd, double flops_bwd, int e, int64_t M, int6
   return flops_fwd * 1.7e-9 + flops_bwd * 3.1e-9 > 10.0 + 2.0 * e * ((double)M * Kp + (double)weights * Kp) / 4.7e6;
 }
 
-static DensePlan dense_plan(int dtype, int64_t M, int64_t K, int64_t n, int G, const Ways& ways) {
-  const bool pair = ways.pair;
-  DensePlan p;
-  const int e = dtype_bytes(dtype), per = 16 / e;
-  const int64_t weights = n * (G > 0 ? G : 1);
-  p.grouped = G > 0;
-  p.Kp = (K + per - 1) / per * per;
-  p.np = (n + per - 1) / per * per;
-  p.fwd = gemm_plan(kFwd, dtype, M, n, K, p.grouped, G, ways.fwd);
-  p.dx = gemm_plan(kDx, dtype, M, K, n, p.grouped, G, ways.dx, pair);
-  p.dw = gemm_plan(kDw, dtype, n, K, M, p.grouped, G, ways.dw, pair);
-  p.dz_tiles = ceil_div(M, kDzRows) + (p.grouped ? G + 2 : 0);
-  const bool vector = as_vectors(M, K, n, G);
+static int64_t whole_pieces(int64_t width, int e) { return (width * e + 15) / 16 * 16 / e; }
+
+static ForwardPlan forward_plan(const Call& c) {
+  ForwardPlan p;
+  const int e = dtype_bytes(c.dtype);
+  const int64_t weights = c.n * (c.G > 0 ? c.G : 1);
+  const bool lie = c.x_lies && c.w_lies, vector = as_vectors(c.M, c.K, c.n, c.G);
+  p.Kp = whole_pieces(c.K, e);
+  p.copy = !lie && !vector && copy_pays(2.0 * c.M * c.K * c.n, 0, e, c.M, p.Kp, weights);
+  p.direct = lie || p.copy;
+  p.gemm = gemm_plan(kFwd, c.dtype, c.M, c.n, c.K, c.G > 0, c.G, p.direct);
   size_t at = 0;
-  auto take = [&at](size_t bytes) {
-    const size_t o = at;
-    at += up256(bytes);
-    return o;
-  };
-  p.fwd_map = take(p.grouped ? p.fwd.row_tiles * sizeof(int4) : 0);
-  p.fwd_slab = take(vector ? 0 : p.fwd.slab);
-  p.fwd_x = take(ways.copy_fwd ? (size_t)M * p.Kp * e : 0);
-  p.fwd_w = take(ways.copy_fwd ? (size_t)weights * p.Kp * e : 0);
-  p.fwd_bytes = at;
-  at = 0;
-  p.dz_map = take(p.grouped ? p.dz_tiles * sizeof(int4) : 0);
-  p.dz_first = take(p.grouped ? (size_t)(G + 1) * 4 : 0);
-  p.dx_map = take(p.grouped ? p.dx.row_tiles * sizeof(int4) : 0);
-  p.dw_map = take((size_t)p.dw.entries * sizeof(int4));
-  p.dw_sums = take((size_t)p.dw.parts / 2 * sizeof(int4));
-  p.dw_count = take(p.grouped ? 8 : 0);
-  p.part = take((size_t)p.dz_tiles * n * 4);
-  p.dz_pitch = pair ? (n + 31) / 32 * 64 : p.np;
-  p.dz = take((size_t)M * p.dz_pitch * e);
-  p.slab = take(std::max(p.dx.slab, p.dw.slab));
-  p.db_slab = take((size_t)(p.grouped ? p.dw.parts : p.dw.splits > 1 ? p.dw.splits : 0) * n * 4);
-  p.bwd_x = take(ways.copy_bwd ? (size_t)M * p.Kp * e : 0);
-  p.bwd_w = take(ways.copy_bwd ? (size_t)weights * p.Kp * e : 0);
-  p.bwd_bytes = at;
+  p.map = take(at, c.G > 0 ? p.gemm.row_tiles * sizeof(int4) : 0);
+  p.slab = take(at, vector ? 0 : p.gemm.slab);
+  p.x = take(at, p.copy && !c.x_lies ? (size_t)c.M * p.Kp * e : 0);
+  p.w = take(at, p.copy && !c.w_lies ? (size_t)weights * p.Kp * e : 0);
+  p.bytes = at;
+  return p;
+}
+
+static BackwardPlan backward_plan(const Call& c) {
+  BackwardPlan p = {};
+  const int e = dtype_bytes(c.dtype);
+  const int64_t weights = c.n * (c.G > 0 ? c.G : 1);
+  const bool grouped = c.G > 0, products = c.dx || c.dw;
+  p.pair = c.dact && e == 2;
+  p.write_dz = c.dact && products;
+  // dz is dy, or lies in the workspace
+  const bool dz_lies = p.write_dz || c.dy_lies, w_lies = !c.dx || c.w_lies, x_lies = !c.dw || c.x_lies;
+  p.Kp = whole_pieces(c.K, e);
+  p.copy = c.M > 0 && products && !(dz_lies && w_lies && x_lies) &&
+           copy_pays(0, 4.0 * c.M * c.K * c.n, e, c.M, whole_pieces(c.K + c.n + 16 / e, e), weights);
+  p.dx_direct = p.copy || (dz_lies && w_lies);
+  p.dw_direct = p.copy || (dz_lies && x_lies);
+  if (c.dx) p.dx = gemm_plan(kDx, c.dtype, c.M, c.K, c.n, grouped, c.G, p.dx_direct, p.pair);
+  if (c.dw) p.dw = gemm_plan(kDw, c.dtype, c.n, c.K, c.M, grouped, c.G, p.dw_direct, p.pair);
+  // Without an activation the products read dy itself and dW's kernel adds up its rows for the bias on the way
+  // (16385 x 64 -> 4096 fp32: 70 us of 450 were a pass over dy for that).  With one, dW's kernel sees 16 bits of dz in
+  // two parts, so that there only fp32 does the same.
+  p.db_in_dw = c.db && c.dw && (!c.dact || c.dtype == BNPVI_F32) && p.dw.tile != kTile256;
+  p.dz_pass = p.write_dz || (c.db && !p.db_in_dw) || c.dres;
+  p.dz_tiles = ceil_div(c.M, kDzRows) + (grouped ? c.G + 2 : 0);
+  p.db_in_dz = c.db && !p.db_in_dw && !grouped && p.dz_tiles == 1 && c.M > 0;          // a launch less
+  p.dz_pitch = p.pair ? (c.n + 31) / 32 * 64 : whole_pieces(c.n, e);
+  size_t at = 0;
+  p.dz_map = take(at, grouped && p.dz_pass ? p.dz_tiles * sizeof(int4) : 0);
+  p.dz_first = take(at, grouped && p.dz_pass ? (size_t)(c.G + 1) * 4 : 0);
+  p.dx_map = take(at, grouped && c.dx ? p.dx.row_tiles * sizeof(int4) : 0);
+  p.dw_map = take(at, (size_t)p.dw.entries * sizeof(int4));
+  p.dw_sums = take(at, (size_t)p.dw.parts / 2 * sizeof(int4));
+  p.dw_count = take(at, grouped || c.M > 0 ? 8 : 0);          // also where it is not used: no call with rows goes without a workspace
+  p.part = take(at, c.db && !p.db_in_dw && !p.db_in_dz ? (size_t)p.dz_tiles * c.n * 4 : 0);
+  p.dz = take(at, p.write_dz || (p.copy && !dz_lies) ? (size_t)c.M * p.dz_pitch * e : 0);
+  p.slab = take(at, std::max(p.dx.slab, p.dw.slab));
+  p.db_slab = take(at, p.db_in_dw ? (size_t)(grouped ? p.dw.parts : p.dw.splits > 1 ? p.dw.splits : 0) * c.n * 4 : 0);
+  p.x = take(at, p.copy && !x_lies ? (size_t)c.M * p.Kp * e : 0);
+  p.w = take(at, p.copy && !w_lies ? (size_t)weights * p.Kp * e : 0);
+  p.bytes = at;
   return p;
 }
 
@@ -756,14 +791,8 @@ static bool pitch_fits(int64_t ld, int64_t width, int dtype) {
   return ld >= width && ld * dtype_bytes(dtype) <= kMaxPitchBytes;
 }
 
-static bool copies_fwd(int dtype, int64_t M, int64_t K, int64_t n, int G) {
-  const int per = 16 / dtype_bytes(dtype);
-  return copy_pays(2.0 * M * K * n, 0, 16 / per, M, (K + per - 1) / per * per, n * (G > 0 ? G : 1));
-}
-
-static bool copies_bwd(int dtype, int64_t M, int64_t K, int64_t n, int G) {
-  const int per = 16 / dtype_bytes(dtype);
-  return copy_pays(0, 4.0 * M * K * n, 16 / per, M, (K + n + 2 * per - 1) / per * per, n * (G > 0 ? G : 1));
+static bool sizes_fit(int dtype, int64_t M, int64_t K, int64_t n, int G) {
+  return dtype_bytes(dtype) > 0 && M >= 0 && M <= INT32_MAX && K >= 1 && K <= (1 << 20) && n >= 1 && n <= (1 << 20) && G >= 0 && G <= kSortMaxLeaves;
 }
 
 }  // namespace bnpvi
@@ -772,18 +801,27 @@ using namespace bnpvi;
 
 extern "C" {
 
+int64_t bnpvi_dense_workspace_for(int dtype, int64_t M, int64_t K, int64_t n, int G, int call) {
+  if (!sizes_fit(dtype, M, K, n, G)) return -1;
+  auto has = [call](int bit) { return (call & bit) != 0; };
+  const Call c = {dtype, M, K, n, G, !has(BNPVI_DENSE_X_OFF), !has(BNPVI_DENSE_W_OFF), !has(BNPVI_DENSE_DY_OFF), has(BNPVI_DENSE_DACT),
+                  has(BNPVI_DENSE_DX), has(BNPVI_DENSE_DW), has(BNPVI_DENSE_DB), has(BNPVI_DENSE_DRES)};
+  return (int64_t)(has(BNPVI_DENSE_BACKWARD) ? backward_plan(c).bytes : forward_plan(c).bytes);
+}
+
 int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G, int backward) {
-  if (dtype_bytes(dtype) == 0 || M < 0 || M > INT32_MAX || K < 1 || K > (1 << 20) || n < 1 || n > (1 << 20) || G < 0 ||
-      G > kSortMaxLeaves)
-    return -1;
-  // enough for every way of loading: which one it is goes by the addresses of the call
-  const bool cf = copies_fwd(dtype, M, K, n, G), cb = copies_bwd(dtype, M, K, n, G);
-  size_t most = 0;
-  for (int i = 0; i < (backward && dtype_bytes(dtype) == 2 ? 16 : 8); ++i) {
-    const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{(i & 1) != 0, (i & 2) != 0, (i & 4) != 0, cf, cb, (i & 8) != 0});
-    most = std::max(most, backward ? p.bwd_bytes : p.fwd_bytes);
-  }
-  return (int64_t)most;
+  if (!sizes_fit(dtype, M, K, n, G)) return -1;
+  // enough for every call of these sizes: wherever its operands lie, with and without an activation, with db in dW's pass or
+  // not (a call that asks for less needs no more)
+  int64_t most = 0;
+  for (int off = 0; off < 8; ++off)
+    for (int given = 0; given < (backward ? 4 : 1); ++given) {
+      const int call = (off & 1 ? BNPVI_DENSE_X_OFF : 0) | (off & 2 ? BNPVI_DENSE_W_OFF : 0) | (off & 4 ? BNPVI_DENSE_DY_OFF : 0);
+      const int asked = BNPVI_DENSE_BACKWARD | BNPVI_DENSE_DX | BNPVI_DENSE_DB | BNPVI_DENSE_DRES | (given & 1 ? BNPVI_DENSE_DACT : 0) |
+                        (given & 2 ? 0 : BNPVI_DENSE_DW);
+      most = std::max(most, bnpvi_dense_workspace_for(dtype, M, K, n, G, backward ? call | asked : call));
+    }
+  return most;
 }
 
 int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const void* bias,
@@ -799,11 +837,12 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
   if (M == 0) return BNPVI_OK;
   BNPVI_REQUIRE(x && w && y, "bnpvi_dense: NULL device pointer");
   const int e = dtype_bytes(dtype);
-  const bool x_lies = aligned(x, ldx, 0, K, e), w_lies = aligned(w, ldw, G > 1 ? w_group : 0, K, e);
-  const bool copy = !(x_lies && w_lies) && copies_fwd(dtype, M, K, n, G), direct = copy || (x_lies && w_lies);
-  const DensePlan p = dense_plan(dtype, M, K, n, G, Ways{direct, true, true, copy, false, false});
-  BNPVI_REQUIRE(work_bytes >= (int64_t)p.fwd_bytes && (p.fwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
-                "bnpvi_dense: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes, (long long)p.fwd_bytes);
+  Call c = {dtype, M, K, n, G};
+  c.x_lies = aligned(x, ldx, 0, K, e);
+  c.w_lies = aligned(w, ldw, G > 1 ? w_group : 0, K, e);
+  const ForwardPlan p = forward_plan(c);
+  BNPVI_REQUIRE(work_bytes >= (int64_t)p.bytes && (p.bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
+                "bnpvi_dense: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes, (long long)p.bytes);
   OnDevice on(ctx->device);
   BNPVI_HIP(on.status());
   hipStream_t s = (hipStream_t)stream;
@@ -842,39 +881,39 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
     m.offsets = offsets;
     m.G = G;
     m.M = M;
-    tile_size(p.fwd.tile, m.tile[0], bc);
-    m.ntiles[0] = p.fwd.row_tiles;
-    m.map[0] = (int4*)(wk + p.fwd_map);
+    tile_size(p.gemm.tile, m.tile[0], bc);
+    m.ntiles[0] = p.gemm.row_tiles;
+    m.map[0] = (int4*)(wk + p.map);
     const int r = launch_maps(m, ctx->device, s);
     if (r) return r;
-    a.map = (const int4*)(wk + p.fwd_map);
+    a.map = (const int4*)(wk + p.map);
   }
-  if (p.fwd.slab) a.slab = (float*)(wk + p.fwd_slab);
-  if (copy) {
+  if (p.gemm.slab) a.slab = (float*)(wk + p.slab);
+  if (p.copy) {
     const int64_t groups = G > 0 ? G : 1;
-    if (!x_lies) {
-      pad_rows(dtype, x, ldx, 0, M, M, K, p.Kp, wk + p.fwd_x, s);
-      a.R = wk + p.fwd_x;
+    if (!c.x_lies) {
+      pad_rows(dtype, x, ldx, 0, M, M, K, p.Kp, wk + p.x, s);
+      a.R = wk + p.x;
       a.ldr = p.Kp;
     }
-    if (!w_lies) {
-      pad_rows(dtype, w, ldw, w_group, n, groups * n, K, p.Kp, wk + p.fwd_w, s);
-      a.S = wk + p.fwd_w;
+    if (!c.w_lies) {
+      pad_rows(dtype, w, ldw, w_group, n, groups * n, K, p.Kp, wk + p.w, s);
+      a.S = wk + p.w;
       a.lds = p.Kp;
       a.s_group = G > 1 ? n * p.Kp : 0;
     }
     BNPVI_LAUNCH_CHECK();
   }
-  const int r = run_gemm(kFwd, dtype, p.fwd, direct, false, a, ctx, s);
+  const int r = run_gemm(kFwd, dtype, p.gemm, p.direct, false, a, ctx, s);
   if (r) return r;
-  if (p.fwd.slab) {
+  if (p.gemm.slab) {
     const unsigned g = flat_grid(M * n);
     if (dtype == BNPVI_F32)
-      split_epilogue_kernel<float><<<g, 256, 0, s>>>(a.slab, p.fwd.splits, a);
+      split_epilogue_kernel<float><<<g, 256, 0, s>>>(a.slab, p.gemm.splits, a);
     else if (dtype == BNPVI_BF16)
-      split_epilogue_kernel<bf16_t><<<g, 256, 0, s>>>(a.slab, p.fwd.splits, a);
+      split_epilogue_kernel<bf16_t><<<g, 256, 0, s>>>(a.slab, p.gemm.splits, a);
     else
-      split_epilogue_kernel<f16_t><<<g, 256, 0, s>>>(a.slab, p.fwd.splits, a);
+      split_epilogue_kernel<f16_t><<<g, 256, 0, s>>>(a.slab, p.gemm.splits, a);
     BNPVI_LAUNCH_CHECK();
   }
   return BNPVI_OK;
@@ -890,15 +929,18 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
                     (!dw || pitch_fits(ldx, K, dtype)) && (!dres || lddres >= n),
                 "bnpvi_dense_backward: a row pitch is below its width, or above 4 MiB");
   const int e = dtype_bytes(dtype);
-  // dz is dy, or lies in the workspace in rows of whole 16 bytes, in 16 bits in two parts
-  const bool dz_lies = dact != nullptr || aligned(dy, lddy, 0, n, e);
-  const bool w_lies = !dx || aligned(w, ldw, G > 1 ? w_group : 0, K, e), x_lies = !dw || aligned(x, ldx, 0, K, e);
-  const bool copy = M > 0 && (dx || dw) && !(dz_lies && w_lies && x_lies) && copies_bwd(dtype, M, K, n, G);
-  const Ways ways = {true, copy || (dz_lies && w_lies), copy || (dz_lies && x_lies), false, copy, dact != nullptr && e == 2};
-  const DensePlan p = dense_plan(dtype, M, K, n, G, ways);
-  BNPVI_REQUIRE(work_bytes >= (int64_t)p.bwd_bytes && (p.bwd_bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
-                "bnpvi_dense_backward: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes,
-                (long long)p.bwd_bytes);
+  Call c = {dtype, M, K, n, G};
+  c.x_lies = aligned(x, ldx, 0, K, e);
+  c.w_lies = aligned(w, ldw, G > 1 ? w_group : 0, K, e);
+  c.dy_lies = aligned(dy, lddy, 0, n, e);
+  c.dact = dact != nullptr;
+  c.dx = dx != nullptr;
+  c.dw = dw != nullptr;
+  c.db = db != nullptr;
+  c.dres = dres != nullptr;
+  const BackwardPlan p = backward_plan(c);
+  BNPVI_REQUIRE(work_bytes >= (int64_t)p.bytes && (p.bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
+                "bnpvi_dense_backward: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes, (long long)p.bytes);
   BNPVI_REQUIRE(M == 0 || (dy && (!dx || w) && (!dw || x)), "bnpvi_dense_backward: NULL device pointer");
   OnDevice on(ctx->device);
   BNPVI_HIP(on.status());
@@ -909,18 +951,13 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   const int4* dz_map = nullptr;
   int32_t* first = nullptr;
   const bool none = M == 0;
-  // Without an activation the products read dy itself and dW's kernel adds up its rows for the bias on the way
-  // (16385 x 64 -> 4096 fp32: 70 us of 450 were a pass over dy for that).  With one, dW's kernel sees 16 bits of dz in
-  // two parts, so that there only fp32 does the same.
-  const bool db_in_dw = db && dw && (!dact || dtype == BNPVI_F32) && p.dw.tile != kTile256;
-  const bool need_dz = (dact != nullptr && (dx || dw)) || (db && !db_in_dw) || dres;
   if (G > 0) {
     MapArgs m = {};
     int bc;
     m.offsets = offsets;
     m.G = G;
     m.M = M;
-    if (need_dz) {
+    if (p.dz_pass) {
       first = (int32_t*)(wk + p.dz_first);
       dz_map = (const int4*)(wk + p.dz_map);
       m.tile[0] = kDzRows;
@@ -946,10 +983,10 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   }
   const void* dz = dy;
   int64_t lddz = lddy;
-  void* db_in_dz = db && !db_in_dw && G == 0 && p.dz_tiles == 1 && !none ? db : nullptr;          // a launch less
-  float* part = db && !db_in_dw && !db_in_dz ? (float*)(wk + p.part) : nullptr;
-  if (need_dz && !none) {
-    void* out = dact ? (void*)(wk + p.dz) : nullptr;
+  void* db_in_dz = p.db_in_dz ? db : nullptr;
+  float* part = db && !p.db_in_dw && !p.db_in_dz ? (float*)(wk + p.part) : nullptr;
+  if (p.dz_pass && !none) {
+    void* out = p.write_dz ? (void*)(wk + p.dz) : nullptr;
     if (dtype == BNPVI_F32)
       launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, p.dz_pitch, (float*)dres, lddres, part, db_in_dz, s);
     else if (dtype == BNPVI_BF16)
@@ -959,12 +996,12 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
       launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, p.dz_pitch, (f16_t*)dres, lddres, part, db_in_dz,
                        s);
     BNPVI_LAUNCH_CHECK();
-    if (dact) {
+    if (p.write_dz) {
       dz = out;
       lddz = p.dz_pitch;
     }
   }
-  if (db && !db_in_dw && !db_in_dz) {
+  if (db && !p.db_in_dw && !p.db_in_dz) {
     const int64_t tiles = none ? 0 : p.dz_tiles;
     if (dtype == BNPVI_F32)
       launch_db<float>(part, first, tiles, (int)n, groups, db, s);
@@ -977,21 +1014,21 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   const int64_t wg = G > 1 ? w_group : 0;
   const void *xs = x, *ws = w;
   int64_t ldxs = ldx, ldws = ldw, wgs = wg;
-  if (copy) {
-    if (!dz_lies) {
-      pad_rows(dtype, dy, lddy, 0, M, M, n, p.np, wk + p.dz, s);
+  if (p.copy) {
+    if (!p.write_dz && !c.dy_lies) {
+      pad_rows(dtype, dy, lddy, 0, M, M, n, p.dz_pitch, wk + p.dz, s);
       dz = wk + p.dz;
-      lddz = p.np;
+      lddz = p.dz_pitch;
     }
-    if (!w_lies) {
-      pad_rows(dtype, w, ldw, w_group, n, groups * n, K, p.Kp, wk + p.bwd_w, s);
-      ws = wk + p.bwd_w;
+    if (dx && !c.w_lies) {
+      pad_rows(dtype, w, ldw, w_group, n, groups * n, K, p.Kp, wk + p.w, s);
+      ws = wk + p.w;
       ldws = p.Kp;
       wgs = G > 1 ? n * p.Kp : 0;
     }
-    if (!x_lies) {
-      pad_rows(dtype, x, ldx, 0, M, M, K, p.Kp, wk + p.bwd_x, s);
-      xs = wk + p.bwd_x;
+    if (dw && !c.x_lies) {
+      pad_rows(dtype, x, ldx, 0, M, M, K, p.Kp, wk + p.x, s);
+      xs = wk + p.x;
       ldxs = p.Kp;
     }
     BNPVI_LAUNCH_CHECK();
@@ -1010,7 +1047,7 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.ldc = lddx;
     if (G > 0) a.map = (const int4*)(wk + p.dx_map);
     if (p.dx.slab) a.slab = (float*)(wk + p.slab);
-    r = run_gemm(kDx, dtype, p.dx, ways.dx, ways.pair, a, ctx, s);
+    r = run_gemm(kDx, dtype, p.dx, p.dx_direct, p.pair, a, ctx, s);
     if (r) return r;
     if (p.dx.slab) {
       // no epilogue: a plain sum over the splits into rows of pitch lddx
@@ -1044,16 +1081,16 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     a.ldc = K;
     a.c_group = n * K;
     if (p.dw.slab) a.slab = (float*)(wk + p.slab);
-    if (db_in_dw) {
+    if (p.db_in_dw) {
       a.db = db;
       if (p.dw.slab) a.db_slab = (float*)(wk + p.db_slab);
     }
-    r = run_gemm(kDw, dtype, p.dw, ways.dw, ways.pair, a, ctx, s);
+    r = run_gemm(kDw, dtype, p.dw, p.dw_direct, p.pair, a, ctx, s);
     if (r) return r;
     if (p.dw.slab) {
       const int4* sums = (const int4*)(wk + p.dw_sums);
       const int32_t* count = (const int32_t*)(wk + p.dw_count);
-      const SumArgs b = {{a.slab, a.db_slab}, {dw, db}, {n * K, db_in_dw ? n : 0}};
+      const SumArgs b = {{a.slab, a.db_slab}, {dw, db}, {n * K, p.db_in_dw ? n : 0}};
       if (dtype == BNPVI_F32)
         launch_sums<float>(b, p.dw, G > 0, sums, count, s);
       else if (dtype == BNPVI_BF16)

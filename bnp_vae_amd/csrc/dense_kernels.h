@@ -505,7 +505,7 @@ struct Stream {
 template <typename T, int KIND, int BR, int BC, int WR, int WC, int KB, bool DIRECT, bool PAIR>
 __global__ __launch_bounds__((BR / WR) * (BC / WC) * 64) __attribute__((amdgpu_waves_per_eu(BR * BC >= 128 * 128 ? 2 : 4)))
 void gemm_kernel(const GemmArgs a, uint32_t tiles) {
-  constexpr int THREADS = (BR / WR) * (BC / WC) * 64, WAVES = THREADS / 64;
+  constexpr int THREADS = (BR / WR) * (BC / WC) * 64;
   static_assert(!PAIR || (sizeof(T) == 2 && KIND != kFwd), "dz of 16 bits in two parts");
   typedef Stages<KIND, PAIR, BR, BC, KB> St;
   constexpr int FR = WR / 32, FC = WC / 32, BK = St::kSBytes / (int)sizeof(T);

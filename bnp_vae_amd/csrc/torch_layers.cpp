@@ -36,7 +36,7 @@ struct Library {
   decltype(&bnpvi_rows_to_leaves) rows_to_leaves;
   decltype(&bnpvi_rows_from_leaves) rows_from_leaves;
   decltype(&bnpvi_rows_from_leaves_backward) rows_from_leaves_backward;
-  decltype(&bnpvi_dense_workspace) dense_workspace;
+  decltype(&bnpvi_dense_workspace_for) dense_workspace;
   decltype(&bnpvi_dense) dense;
   decltype(&bnpvi_dense_backward) dense_backward;
 } lib;
@@ -58,7 +58,7 @@ void bind(const std::string& path) {
   find(h, "bnpvi_rows_to_leaves", lib.rows_to_leaves);
   find(h, "bnpvi_rows_from_leaves", lib.rows_from_leaves);
   find(h, "bnpvi_rows_from_leaves_backward", lib.rows_from_leaves_backward);
-  find(h, "bnpvi_dense_workspace", lib.dense_workspace);
+  find(h, "bnpvi_dense_workspace_for", lib.dense_workspace);
   find(h, "bnpvi_dense", lib.dense);
   find(h, "bnpvi_dense_backward", lib.dense_backward);
 }
@@ -274,8 +274,8 @@ Tensor combine(const Tensor& ys, const Tensor& place, const Tensor& offsets, con
 }
 
 // ---- dense -----------------------------------------------------------------------------------------------------------
-// The workspace of a call goes by its sizes alone; a program has few of them.
-int64_t dense_workspace(int type, int64_t M, int64_t K, int64_t n, int64_t G, int backward) {
+// The workspace of a call goes by its sizes and the bits of `call`; a program has few of them.
+int64_t dense_workspace(int type, int64_t M, int64_t K, int64_t n, int64_t G, int call) {
   struct Key {
     int64_t v[6];
     bool operator==(const Key& o) const { return std::equal(v, v + 6, o.v); }
@@ -289,12 +289,12 @@ int64_t dense_workspace(int type, int64_t M, int64_t K, int64_t n, int64_t G, in
   };
   static std::mutex mutex;
   static std::unordered_map<Key, int64_t, Hash> known;
-  const Key key{{type, M, K, n, G, backward}};
+  const Key key{{type, M, K, n, G, call}};
   std::lock_guard<std::mutex> hold(mutex);
   const auto it = known.find(key);
   if (it != known.end()) return it->second;
   if (known.size() >= 4096) known.clear();
-  return known[key] = lib.dense_workspace(type, M, K, n, static_cast<int>(G), backward);
+  return known[key] = lib.dense_workspace(type, M, K, n, static_cast<int>(G), call);
 }
 
 // A weight (n, K) or (G, n, K) with contiguous rows, and its pitches.
@@ -309,6 +309,12 @@ Weights weights(const Tensor& w) {
   return {t, n > 1 ? t.stride(-2) : K, t.dim() == 3 && t.size(0) > 1 ? t.stride(0) : 0};
 }
 
+// `bit` where the operand is off 16 bytes.
+int off16(const Tensor& t, int64_t pitch, int64_t group, int64_t width, int bit) {
+  const uint64_t all = reinterpret_cast<uint64_t>(ptr(t)) | static_cast<uint64_t>((pitch | group | width) * t.element_size());
+  return all & 15 ? bit : 0;
+}
+
 std::tuple<Tensor, Tensor> dense_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& bias_in, const Tensor& res_in,
                                          const Tensor& offsets, int64_t act, int64_t ctx, bool want_dact) {
   const Tensor x = rows(x_in), bias = bias_in.defined() ? bias_in.contiguous() : bias_in, res = res_in.defined() ? rows(res_in) : res_in;
@@ -317,7 +323,8 @@ std::tuple<Tensor, Tensor> dense_forward(const Tensor& x_in, const Tensor& w_in,
   const int type = type_of(x);
   Tensor y = at::empty({M, n}, x.options()), dact, work;
   if (want_dact && act != BNPVI_ACT_NONE) dact = at::empty({M, n}, x.options().dtype(at::kFloat));
-  const int64_t need = dense_workspace(type, M, K, n, G, 0);
+  const int64_t need = dense_workspace(type, M, K, n, G, off16(x, pitch(x), 0, K, BNPVI_DENSE_X_OFF) |
+                                                             off16(w.t, w.row, w.group, K, BNPVI_DENSE_W_OFF));
   if (need > 0) work = at::empty({need}, x.options().dtype(at::kByte));
   check(lib.dense(ctx_of(ctx), type, ptr(x), pitch(x), ptr(w.t), w.row, w.group, ptr(bias), G > 1 ? n : 0, act, ptr(res),
                   res.defined() ? pitch(res) : 0, ptr<int32_t>(offsets), G, M, K, n, ptr(y), n, ptr(dact), n, ptr(work), need, stream_of(x)),
@@ -350,7 +357,10 @@ struct Dense : Function<Dense> {
     const bool need_res = (has & 2) && c->needs_input_grad(2 + (has & 1));
     if (need_res && G) dres = at::empty({M, n}, x.options());
     if (dx.defined() || dw.defined() || db.defined() || dres.defined()) {
-      const int64_t need = dense_workspace(type, M, K, n, G, 1);
+      const int call = BNPVI_DENSE_BACKWARD | off16(x, pitch(x), 0, K, BNPVI_DENSE_X_OFF) | off16(w.t, w.row, w.group, K, BNPVI_DENSE_W_OFF) |
+                       off16(dy, pitch(dy), 0, n, BNPVI_DENSE_DY_OFF) | (ptr(dact) ? BNPVI_DENSE_DACT : 0) | (ptr(dx) ? BNPVI_DENSE_DX : 0) |
+                       (dw.defined() ? BNPVI_DENSE_DW : 0) | (db.defined() ? BNPVI_DENSE_DB : 0) | (ptr(dres) ? BNPVI_DENSE_DRES : 0);
+      const int64_t need = dense_workspace(type, M, K, n, G, call);
       if (need > 0) work = at::empty({need}, x.options().dtype(at::kByte));
       check(lib.dense_backward(ctx_of(ctx), type, ptr(dy), pitch(dy), ptr(dact), n, ptr(x), pitch(x), ptr(w.t), w.row, w.group,
                                ptr<int32_t>(offsets), G, M, K, n, ptr(dx), K, ptr(dw), ptr(db), ptr(dres), n, ptr(work), need, stream_of(x)),

@@ -367,8 +367,23 @@ int bnpvi_rows_from_leaves_backward(bnpvi_ctx* ctx, int dtype, const void* dy_de
  *     dres = dy with zeros in the rows of no group [M][lddres]
  * each NULL where it is not wanted; a group without rows gets zeros, and so does dx in the rows of no group.
  * 1 <= K, n <= 2^20, M < 2^31, G <= bnpvi_leaf_sort_max_leaves(), pitches of what is multiplied at most 4 MiB.
- * Workspace: bnpvi_dense_workspace(dtype, M, K, n, G, backward) bytes, aligned to 256. */
+ * Workspace, aligned to 256: bnpvi_dense_workspace(dtype, M, K, n, G, backward) bytes are enough for every call of these
+ * sizes; bnpvi_dense_workspace_for says what one call needs, by the bits below that are true of it (its operands' copies
+ * and dz can be much of the former).  An operand is "off 16 bytes" where its address, its row pitch, its width or (W with
+ * G > 1) w_group is no multiple of 16 bytes.  A backward call of rows always needs some. */
+enum {
+  BNPVI_DENSE_BACKWARD = 1,
+  BNPVI_DENSE_X_OFF = 2,    /* x, W, dy are off 16 bytes */
+  BNPVI_DENSE_W_OFF = 4,
+  BNPVI_DENSE_DY_OFF = 8,
+  BNPVI_DENSE_DACT = 16,    /* of a backward call: dact is given, */
+  BNPVI_DENSE_DX = 32,      /* dx, dw, db, dres are asked for */
+  BNPVI_DENSE_DW = 64,
+  BNPVI_DENSE_DB = 128,
+  BNPVI_DENSE_DRES = 256
+};
 int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G, int backward);
+int64_t bnpvi_dense_workspace_for(int dtype, int64_t M, int64_t K, int64_t n, int G, int call);
 int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int64_t w_group,
                 const void* bias_dev, int64_t bias_group, int activation, const void* residual_dev, int64_t ldres,
                 const int32_t* offsets_dev, int G, int64_t M, int64_t K, int64_t n, void* y_dev, int64_t ldy, void* dact_dev,

@@ -962,3 +962,30 @@ def test_functional_transforms_are_errors(layers):
                  lambda: torch.func.vmap(lambda t: layers.top_leaves(t, 2)[1])(x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+# ------------------------------------------------------------------------------------------------ memory of a call
+@pytest.mark.parametrize("dtype,act,shift", [("bf16", "softsign", 0), ("bf16", None, 0), ("f32", None, 0), ("f32", "gelu", 0), ("bf16", "gelu", 1)])
+def test_memory_of_a_dense_pass(layers, dtype, act, shift):
+    """What a pass allocates: its results, act'(z) in fp32, dz in two parts (bf16) or one, 8 MB for maps and partial sums
+    of the bias, at most 64 partial results of dW -- and copies of x, W and dy only where they are off 16 bytes."""
+    M, K, n, T = 131072, 512, 512, TYPES[dtype]
+    e = T.itemsize
+    def put(shape, seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        return torch.randn(shape[:-1] + (shape[-1] + 8,), generator=g, device="cuda").to(T)[..., shift:shift + shape[-1]].detach()
+    x, w, dy = put((M, K), 1).requires_grad_(True), put((n, K), 2).requires_grad_(True), put((M, n), 3)
+    layers.dense(x[:100], w[:], activation=act).sum().backward()
+    x.grad = w.grad = None
+    copies = M * K * e + n * K * e if shift else 0
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    start = torch.cuda.memory_allocated()
+    y = layers.dense(x, w, activation=act)
+    kept = M * n * e + (M * n * 4 if act else 0)
+    assert torch.cuda.memory_allocated() - start <= kept + (1 << 20)
+    assert torch.cuda.max_memory_allocated() - start <= kept + copies + (8 << 20)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    dz = M * n * (4 if e == 2 else e) if act else M * n * e if shift else 0
+    most = kept + M * K * e + n * K * e + dz + 64 * n * K * 4 + copies + (8 << 20)
+    assert torch.cuda.max_memory_allocated() - start <= most

@@ -168,3 +168,38 @@ def test_recorders_of_torch_calls_are_refused():
             torch.jit.trace(call, (t,))
         with pytest.raises(_lib.BnpviError, match="traced"):
             make_fx(call)(t)
+
+
+X_OFF, W_OFF, DY_OFF, DACT, DX, DW, DB, DRES = (1 << i for i in range(1, 9))
+
+
+def _need(dtype, M, K, n, G, *bits):
+    return _lib.lib.bnpvi_dense_workspace_for(dtype, M, K, n, G, sum(bits))
+
+
+def test_a_dense_call_needs_no_copy_of_what_lies():
+    """65536 x 4096 -> 256 in bf16 whose operands lie on 16 bytes: no copy of x, no dz where it is dy.  Split sums take at
+    most 64 partial results of dW; every part is rounded up to 256 bytes."""
+    M, K, n, e = 65536, 4096, 256, 2
+    dw_parts, db_parts = 64 * n * K * 4, 2 * (M // 128) * n * 4
+    asked = (1, DX, DW, DB)
+    assert _need(1, M, K, n, 0) == 0
+    assert _need(1, M, K, n, 0, *asked) <= dw_parts + db_parts + 4096
+    assert _need(1, M, K, n, 0, DACT, *asked) <= dw_parts + db_parts + 2 * M * n * e + 4096
+    assert M * K * e > dw_parts + db_parts + 2 * M * n * e                    # the copy of x alone is more
+    assert _need(1, M, K, n, 0, X_OFF, *asked) >= M * K * e                   # where x is off 16 bytes its copy pays
+    assert _need(0, 16385, 64, 4096, 0, *asked) < 16385 * 4096 * 4            # dz is dy
+    assert _need(1, 32768, 1024, 1024, 0) == 0 and _need(1, 32768, 1024, 1024, 0, X_OFF) == 32768 * 1024 * e
+    assert _need(1, M, K, n, 0, 1, DACT, DB) <= db_parts + 4096               # the bias alone: no dz either
+    assert _need(5, 1, 1, 1, 0) == -1 and _need(0, 1, 0, 1, 0, 1) == -1
+
+
+def test_the_workspace_of_all_calls_is_enough_for_each():
+    import random
+    rng = random.Random(3)
+    for _ in range(300):
+        dtype, G = rng.randrange(3), rng.choice([0, 0, 1, 5, 64])
+        M, K, n = (int(2 ** rng.uniform(0, t)) for t in (16, 12, 12))
+        most = [_lib.lib.bnpvi_dense_workspace(dtype, M, K, n, G, b) for b in (0, 1)]
+        for call in range(512):
+            assert _need(dtype, M, K, n, G, call) <= most[call & 1], (dtype, M, K, n, G, call)
