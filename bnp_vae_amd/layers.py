@@ -117,26 +117,48 @@ class LeafPlan(object):
     offsets (L + 1,) int32  first place of each leaf; from offsets[L] on lie the slots without a leaf
 
     sort_by_leaf makes it.  One put together by hand has to be such a sort: rows whose place lies outside are left out, and
-    places that repeat leave other rows unwritten."""
+    places that repeat leave other rows unwritten.  Its tensors are checked here, once, and stay the plan's: another sort is
+    another plan."""
 
-    __slots__ = ("place", "order", "offsets", "num_leaves")
+    __slots__ = ("_place", "_order", "_offsets", "_num_leaves")
 
     def __init__(self, place, order, offsets, num_leaves):
+        for name, t in (("place", place), ("order", order), ("offsets", offsets)):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError("LeafPlan: %s must be a torch tensor, not %s" % (name, type(t).__name__))
         if place.dim() != 2 or place.dtype != torch.int32 or not place.is_contiguous():
             raise ValueError("LeafPlan: place must be a contiguous (N, k) int32 tensor")
+        if tuple(order.shape) != (place.numel(),) or order.dtype != torch.int32 or not order.is_contiguous():
+            raise ValueError("LeafPlan: order must be a contiguous (%d,) int32 tensor" % place.numel())
         if tuple(offsets.shape) != (num_leaves + 1,) or offsets.dtype != torch.int32 or not offsets.is_contiguous():
             raise ValueError("LeafPlan: offsets must be a contiguous (%d,) int32 tensor" % (num_leaves + 1))
-        if place.device != offsets.device:
-            raise ValueError("LeafPlan: place is on %s, offsets on %s" % (place.device, offsets.device))
-        self.place, self.order, self.offsets, self.num_leaves = place, order, offsets, num_leaves
+        if not place.device == order.device == offsets.device:
+            raise ValueError("LeafPlan: place is on %s, order on %s, offsets on %s" % (place.device, order.device, offsets.device))
+        self._place, self._order, self._offsets, self._num_leaves = place, order, offsets, num_leaves
+
+    @property
+    def place(self):
+        return self._place
+
+    @property
+    def order(self):
+        return self._order
+
+    @property
+    def offsets(self):
+        return self._offsets
+
+    @property
+    def num_leaves(self):
+        return self._num_leaves
 
     @property
     def num_frames(self):
-        return self.place.shape[0]
+        return self._place.shape[0]
 
     @property
     def choices(self):
-        return self.place.shape[1]
+        return self._place.shape[1]
 
 
 def sort_by_leaf(leaf, num_leaves):

@@ -203,3 +203,26 @@ def test_the_workspace_of_all_calls_is_enough_for_each():
         most = [_lib.lib.bnpvi_dense_workspace(dtype, M, K, n, G, b) for b in (0, 1)]
         for call in range(512):
             assert _need(dtype, M, K, n, G, call) <= most[call & 1], (dtype, M, K, n, G, call)
+
+
+def test_a_plan_keeps_the_tensors_it_was_checked_with():
+    import copy
+    i = dict(dtype=torch.int32)
+    plan = layers.LeafPlan(torch.zeros((4, 2), **i), torch.arange(8, **i), torch.tensor([0, 8, 8, 8], **i), 3)
+    for name, value in (("place", torch.zeros((4, 2), **i)), ("order", torch.zeros(8, **i)), ("offsets", torch.zeros(1, **i)),
+                        ("num_leaves", 9)):
+        with pytest.raises(AttributeError):
+            setattr(plan, name, value)
+    again = copy.deepcopy(plan)
+    assert torch.equal(again.order, plan.order) and again.order is not plan.order and again.num_leaves == 3
+
+
+def test_orders_of_other_shapes_types_and_devices_are_refused():
+    i = dict(dtype=torch.int32)
+    place, order, offsets = torch.zeros((4, 2), **i), torch.zeros(8, **i), torch.zeros(4, **i)
+    for o in (order[:7], order.long(), order[None], torch.zeros(16, **i)[::2], order.to("meta")):
+        with pytest.raises(ValueError, match="LeafPlan"):
+            layers.LeafPlan(place, o, offsets, 3)
+    for o in (None, [0] * 8):
+        with pytest.raises(TypeError, match="order"):
+            layers.LeafPlan(place, o, offsets, 3)
