@@ -154,6 +154,7 @@ def class_vote(nodes_list, z_train, train_labels, z_test, decay_factor=0.0, devi
     leaves are numbered depth-first.  encoder: as in `closest_frames`, for both sets.  The O(N) parts (both nearest-leaf passes, the vote
     histogram) run on the device, the O(L*C) tree arithmetic on the host."""
     import torch
+    encoder = None if encoder is None else list(encoder)                 # used twice
     order, parent, is_leaf, alpha = _flatten(nodes_list)
     leaves = [k for k in range(len(order)) if is_leaf[k]]
     L = len(leaves)

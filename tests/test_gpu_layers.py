@@ -989,3 +989,15 @@ def test_memory_of_a_dense_pass(layers, dtype, act, shift):
     dz = M * n * (4 if e == 2 else e) if act else M * n * e if shift else 0
     most = kept + M * K * e + n * K * e + dz + 64 * n * K * 4 + copies + (8 << 20)
     assert torch.cuda.max_memory_allocated() - start <= most
+
+
+def test_class_vote_with_an_encoder_that_is_an_iterator(layers):
+    """The layers are needed for the training and for the test frames."""
+    from bnp_vae_amd import hierarchy
+    vi = fitted()
+    nodes = vi.get_nodes_list(vi.root, [])
+    x, labels = rand((300, 40), torch.float32, 1), np.arange(300) % 3
+    enc = [(gpu(rand((16, 40), torch.float32, 2, 0.3)), gpu(rand((16,), torch.float32, 3)), "softsign")]
+    want = hierarchy.class_vote(nodes, x, labels, x[:50], 0.5, encoder=enc)
+    got = hierarchy.class_vote(nodes, x, labels, x[:50], 0.5, encoder=iter(enc))
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
