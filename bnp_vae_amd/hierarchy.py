@@ -66,8 +66,9 @@ def _by_leaf(assign, L, *tables):
     import torch
     from . import layers
     from ._lib import lib
-    if L <= lib.bnpvi_leaf_sort_max_leaves() and assign.shape[0] < 1 << 31:
-        plan = layers.sort_by_leaf(assign, L)              # every row has a leaf
+    if L + 2 <= lib.bnpvi_leaf_sort_max_leaves() and assign.shape[0] < 1 << 31:
+        # a row whose distances are no numbers has an index behind the last leaf, and its place there; none is left out
+        plan = layers.sort_by_leaf(assign.clamp(-1, L) + 1, L + 2)
         moved = [layers.dispatch(t.view(torch.float32), plan).view(t.dtype) for t in tables]      # bytes, whatever they mean
         return [plan.order.to(torch.int64)] + moved
     rows = torch.sort(assign.to(torch.int64), stable=True).indices

@@ -1001,3 +1001,26 @@ def test_class_vote_with_an_encoder_that_is_an_iterator(layers):
     want = hierarchy.class_vote(nodes, x, labels, x[:50], 0.5, encoder=enc)
     got = hierarchy.class_vote(nodes, x, labels, x[:50], 0.5, encoder=iter(enc))
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+def test_frames_without_a_nearest_leaf_keep_their_place(layers, monkeypatch):
+    """A frame whose latents are NaN has no nearest leaf (its index is 2^31 - 1): its rows move with it, behind all leaves, as
+    torch.sort puts them."""
+    from bnp_vae_amd import hierarchy
+    assign = torch.randint(0, 40, (500,), device="cuda", generator=torch.Generator("cuda").manual_seed(3), dtype=torch.int32)
+    assign[[7, 90, 300]] = 2 ** 31 - 1
+    node = torch.randint(0, 60, (500, 3), device="cuda", generator=torch.Generator("cuda").manual_seed(4), dtype=torch.int32)
+    dist = torch.rand((500, 3), device="cuda", dtype=torch.float64)
+    got, want = hierarchy._by_leaf(assign, 40, node, dist), torch.sort(assign.long(), stable=True).indices
+    assert torch.equal(got[0], want) and torch.equal(got[1], node[want]) and torch.equal(got[2], dist[want])
+    vi = fitted()
+    nodes = vi.get_nodes_list(vi.root, [])
+    z = rand((400, 16), torch.float32, 9, 4.0)
+    z[[11, 200, 399]] = float("nan")
+    path, top = hierarchy.closest_frames(nodes, z, 4)
+    def by_torch(assign, L, *tables):
+        rows = torch.sort(assign.to(torch.int64), stable=True).indices
+        return [rows] + [t[rows] for t in tables]
+    monkeypatch.setattr(hierarchy, "_by_leaf", by_torch)
+    want_path, want_top = hierarchy.closest_frames(nodes, z, 4)
+    assert np.array_equal(path, want_path) and top == want_top
