@@ -66,7 +66,8 @@ SHAPES = [
     (300, 8192, 512), (31, 4096, 2048), (513, 70000, 40),                                 # few rows, long sums in parts
     (70000, 64, 32), (90000, 24, 64), (50000, 1024, 32),                                  # narrow on either side
     (5, 4096, 3000), (8, 1031, 77), (1, 4096, 32),                                        # products with vectors
-    (7000, 2001, 601), (32768, 1023, 1021), (600, 37, 41)]                                # rows off 16 bytes, copied and not
+    (7000, 2001, 601), (32768, 1023, 1021), (600, 37, 41), (70000, 63, 31), (70000, 31, 63),     # rows off 16 bytes, copied and not
+    (68278, 367, 254), (6141, 1067, 536), (20919, 1916, 5)]
 
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
@@ -103,7 +104,9 @@ def some_sizes(count, total, seed, least=0):
 @pytest.mark.parametrize("sizes,K,n", [
     ([40000, 0, 9000, 1, 10990], 512, 512), (some_sizes(64, 60000, 1), 512, 512), (some_sizes(12, 60000, 2), 1024, 256),
     ([200] * 256, 512, 512), (some_sizes(500, 20000, 3), 200, 136), (some_sizes(3000, 15000, 4), 64, 96), ([6] * 512, 250, 130),
-    (some_sizes(5, 20000, 5), 301, 203), (some_sizes(8, 50000, 6), 32, 520), (some_sizes(8, 50000, 7), 520, 24), ([1] * 700, 40, 33)])
+    (some_sizes(5, 20000, 5), 301, 203), (some_sizes(8, 50000, 6), 32, 520), (some_sizes(8, 50000, 7), 520, 24), ([1] * 700, 40, 33),
+    (some_sizes(200, 6000, 8), 257, 259), (some_sizes(3, 30000, 9), 31, 63),
+    (some_sizes(26, 5052, 10), 1574, 89), (some_sizes(108, 200, 11), 472, 237), (some_sizes(162, 300, 12), 939, 1114), (some_sizes(10, 84653, 13), 86, 41)])
 def test_dense_per_leaf_is_exact(layers, dtype, act, sizes, K, n):
     check_exact(layers, sum(sizes) + 77 + 5, K, n, TYPES[dtype], act, sizes=sizes, head=5)
 
