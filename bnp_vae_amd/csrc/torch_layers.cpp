@@ -89,6 +89,9 @@ int type_of(const Tensor& t) {
   }
 }
 
+// A gradient whose memory holds its values (views of complex conjugates hold the negated ones).
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // A 2-D tensor with contiguous rows at a pitch the kernels take: itself where it is so already.
 constexpr int64_t kMaxPitchBytes = int64_t(1) << 22;
 Tensor rows(const Tensor& t) {
@@ -158,7 +161,7 @@ struct TopLeaves : Function<TopLeaves> {
     const Tensor &leaf = saved[0], &weight = saved[1], &total = saved[2];
     Tensor dphi;
     if (given[1].defined()) {
-      const Tensor d = given[1].contiguous();
+      const Tensor d = plain(given[1]).contiguous();
       dphi = at::empty({s[0], s[1]}, weight.options());
       check(lib.top_leaves_backward(ctx_of(s[5]), ptr<int32_t>(leaf), ptr<float>(weight), ptr<float>(total), ptr<float>(d), s[0], s[2], s[3],
                                     s[4], ptr<float>(dphi), s[1], s[1], stream_of(leaf)),
@@ -223,7 +226,7 @@ struct Dispatch : Function<Dispatch> {
   }
   static variable_list backward(AutogradContext* c, variable_list given) {
     const auto saved = c->get_saved_variables();
-    return once({from_leaves(given[0], saved[0], saved[1], Tensor(), c->saved_data["ctx"].toInt()), Tensor(), Tensor(), Tensor()}, given, saved);
+    return once({from_leaves(plain(given[0]), saved[0], saved[1], Tensor(), c->saved_data["ctx"].toInt()), Tensor(), Tensor(), Tensor()}, given, saved);
   }
 };
 
@@ -241,9 +244,9 @@ struct Combine : Function<Combine> {
     const int64_t ctx = c->saved_data["ctx"].toInt();
     Tensor dys, dweight;
     if (!weight.defined()) {
-      dys = to_leaves(given[0], place, offsets, ctx);
+      dys = to_leaves(plain(given[0]), place, offsets, ctx);
     } else {
-      const Tensor dy = rows(given[0]), ys = rows(saved[0]);
+      const Tensor dy = rows(plain(given[0])), ys = rows(saved[0]);
       const int64_t N = place.size(0), k = place.size(1), D = ys.size(1);
       if (c->needs_input_grad(0)) dys = at::empty({N * k, D}, ys.options());
       if (c->needs_input_grad(1)) dweight = D ? at::empty({N, k}, weight.options()) : at::zeros({N, k}, weight.options());
@@ -348,7 +351,7 @@ struct Dense : Function<Dense> {
     const int64_t ctx = c->saved_data["ctx"].toInt(), M = x0.size(0), K = x0.size(1), n = w0.size(-2), G = w0.dim() == 3 ? w0.size(0) : 0;
     const int type = type_of(x0);
     Tensor dx, dw, db, dres, work;
-    const Tensor dy = rows(given[0]), x = rows(x0);
+    const Tensor dy = rows(plain(given[0])), x = rows(x0);
     const Weights w = weights(w0);
     if (c->needs_input_grad(0)) dx = at::empty({M, K}, x.options());
     if (c->needs_input_grad(1)) dw = at::empty(w0.sizes(), x.options());

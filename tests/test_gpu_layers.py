@@ -1024,3 +1024,24 @@ def test_frames_without_a_nearest_leaf_keep_their_place(layers, monkeypatch):
     monkeypatch.setattr(hierarchy, "_by_leaf", by_torch)
     want_path, want_top = hierarchy.closest_frames(nodes, z, 4)
     assert np.array_equal(path, want_path) and top == want_top
+
+
+def test_gradients_that_arrive_as_negated_views(layers):
+    """Re(conj(i t) k) = t Im(k): the gradient of t is the imaginary part of a conjugate, whose memory has the other sign.
+    Where it has a row's layout already, no copy makes it plain."""
+    x, w = gpu(rand((7, 8), torch.float32, 1)).requires_grad_(True), gpu(rand((1, 8), torch.float32, 2)).requires_grad_(True)
+    phi, rows = torch.rand((1, 4), device="cuda").requires_grad_(True), gpu(rand((7, 1), torch.float32, 3)).requires_grad_(True)
+    plan, c = layers.sort_by_leaf(torch.arange(7, dtype=torch.int32, device="cuda"), 7), torch.complex(*(gpu(rand((7, 1), torch.float32, s)) for s in (4, 5)))
+    one = torch.rand((7, 1), device="cuda")
+    seen = []
+    def conjugate(t):
+        t.register_hook(lambda g: seen.append(g.is_neg()))
+        return torch.complex(torch.zeros_like(t), t).conj()
+    for call, leaves, k in ((lambda: layers.dense(x, w, activation="tanh"), [x, w], c), (lambda: layers.dense(x, w), [x, w], c),
+                            (lambda: layers.top_leaves(phi, 1, renormalize=False)[1], [phi], c[:1]),
+                            (lambda: layers.dispatch(rows, plan), [rows], c), (lambda: layers.combine(rows, plan), [rows], c),
+                            (lambda: layers.combine(rows, plan, one), [rows], c)):
+        got = torch.autograd.grad((conjugate(call()) * k).real.sum(), leaves)
+        want = torch.autograd.grad((call() * k.imag).sum(), leaves)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(seen)
