@@ -155,7 +155,9 @@ def test_infinities_in_a_gradient(layers, dtype):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("M,K,n,sizes", [(5000, 1032, 520, None), (3001, 600, 777, None), (20000, 512, 264, [3000, 0, 9000, 1, 7900]),
-                                         (2000, 130, 300, [7] * 200)])
+                                         (2000, 130, 300, [7] * 200), (40000, 1024, 1024, None), (3000, 2048, 4096, None),
+                                         (60000, 512, 768, [30000, 0, 17, 9000, 20950]), (84650, 86, 41, [8465] * 10),
+                                         (5122, 1574, 89, [197] * 26)])
 def test_large_gradients_are_as_near_as_one_rounding(layers, dtype, M, K, n, sizes):
     """Every element is off by what rounding the exact value would cost plus at most twice the error in front of the
     rounding, and that is below 2^-15 of a value's size (z and the sums in fp32, dz in two parts), a fortieth of bf16's
