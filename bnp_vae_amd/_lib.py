@@ -88,6 +88,8 @@ EXPORTS = {
     "bnpvi_dense_workspace_for": (_i64, [_i, _i64, _i64, _i64, _i, _i]),
     "bnpvi_dense": (_i, [_p, _i, _p, _i64, _p, _i64, _i64, _p, _i64, _i, _p, _i64, _p, _i, _i64, _i64, _i64, _p, _i64,
                          _p, _i64, _p, _i64, _p]),
+    "bnpvi_dense_backward_act": (_i, [_p, _i, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i, _i64, _i64, _i64, _p,
+                                      _i64, _p, _p, _p, _i64, _p, _i64, _p]),
     "bnpvi_dense_backward": (_i, [_p, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i, _i64, _i64, _i64, _p,
                                   _i64, _p, _p, _p, _i64, _p, _i64, _p]),
 }

@@ -173,7 +173,7 @@ __global__ __launch_bounds__(1024) void maps_kernel(const MapArgs a) {
 }
 
 // ---- dz, residual gradient, partial sums of the bias gradient --------------------------------------------------------
-// One workgroup: a row tile (of one group) x 256 columns.  dz = dy * d, in fp32 rounded once, in 16 bits in two parts
+// One workgroup: a row tile (of one group) x 256 columns.  dz = dy * d, rounded once, or PAIR: in 16 bits in two parts
 // hi + lo (dense_kernels.h): |dz - hi - lo| is at most 2^-16 of |dz| in bf16, 2^-22 in fp16 (where lo's smallest step adds
 // 2^-25, half of dy's own).  hi stays finite where dz is -- a dz behind fp16's largest value, which is up to 1.13 dy, is 65504
 // and the rest of it.  The bias gradient adds the unrounded products: per thread over its rows, then the eight row threads
@@ -189,7 +189,7 @@ __device__ __forceinline__ void two_parts(float v, T& hi, T& lo) {
 
 constexpr int kDzRows = 128;
 
-template <typename T>
+template <typename T, bool PAIR>
 __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64_t lddy, const float* __restrict__ d, int64_t ldd,
                                                  const int4* __restrict__ map, int64_t M, int n, T* __restrict__ dz, int64_t lddz,
                                                  T* __restrict__ dres, int64_t lddres, float* __restrict__ part,
@@ -209,7 +209,6 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, int64
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  constexpr bool PAIR = sizeof(T) == 2;
   if (inside > 0 || (PAIR && dz != nullptr && 2 * c < lddz)) {
 #pragma unroll 2
     for (int64_t r = r0 + ty; r < r1; r += 8) {
@@ -618,6 +617,7 @@ struct Call {
   int G;
   bool x_lies, w_lies, dy_lies;
   bool dact, dx, dw, db, dres;
+  bool step;                   // dact holds 0 and 1 only
 };
 
 struct ForwardPlan {
@@ -675,7 +675,7 @@ static BackwardPlan backward_plan(const Call& c) {
   const int e = dtype_bytes(c.dtype);
   const int64_t weights = c.n * (c.G > 0 ? c.G : 1);
   const bool grouped = c.G > 0, products = c.dx || c.dw;
-  p.pair = c.dact && e == 2;
+  p.pair = c.dact && e == 2 && !c.step;          // dy times 0 or 1 is its 16 bits
   p.write_dz = c.dact && products;
   // dz is dy, or lies in the workspace
   const bool dz_lies = p.write_dz || c.dy_lies, w_lies = !c.dx || c.w_lies, x_lies = !c.dw || c.x_lies;
@@ -753,10 +753,16 @@ static int launch_maps(const MapArgs& a, int device, hipStream_t s) {
 static unsigned flat_grid(int64_t elems) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(elems, 256), 4096)); }
 
 template <typename T>
-static void launch_dz(const T* dy, int64_t lddy, const void* d, int64_t ldd, const int4* map, int64_t M, int n, int64_t tiles, T* dz,
-                      int64_t lddz, T* dres, int64_t lddres, float* part, void* db, hipStream_t s) {
-  dz_kernel<T><<<dim3((unsigned)tiles, (unsigned)ceil_div(n, 256)), 256, 0, s>>>(dy, lddy, (const float*)d, ldd, map, M, n,
-                                                                                 dz, lddz, dres, lddres, part, (T*)db);
+static void launch_dz(bool pair, const void* dy, int64_t lddy, const void* d, int64_t ldd, const int4* map, int64_t M, int n, int64_t tiles,
+                      void* dz, int64_t lddz, void* dres, int64_t lddres, float* part, void* db, hipStream_t s) {
+  const dim3 grid((unsigned)tiles, (unsigned)ceil_div(n, 256));
+  if constexpr (sizeof(T) == 2) {
+    if (pair) {
+      dz_kernel<T, true><<<grid, 256, 0, s>>>((const T*)dy, lddy, (const float*)d, ldd, map, M, n, (T*)dz, lddz, (T*)dres, lddres, part, (T*)db);
+      return;
+    }
+  }
+  dz_kernel<T, false><<<grid, 256, 0, s>>>((const T*)dy, lddy, (const float*)d, ldd, map, M, n, (T*)dz, lddz, (T*)dres, lddres, part, (T*)db);
 }
 
 template <typename T>
@@ -805,7 +811,7 @@ int64_t bnpvi_dense_workspace_for(int dtype, int64_t M, int64_t K, int64_t n, in
   if (!sizes_fit(dtype, M, K, n, G)) return -1;
   auto has = [call](int bit) { return (call & bit) != 0; };
   const Call c = {dtype, M, K, n, G, !has(BNPVI_DENSE_X_OFF), !has(BNPVI_DENSE_W_OFF), !has(BNPVI_DENSE_DY_OFF), has(BNPVI_DENSE_DACT),
-                  has(BNPVI_DENSE_DX), has(BNPVI_DENSE_DW), has(BNPVI_DENSE_DB), has(BNPVI_DENSE_DRES)};
+                  has(BNPVI_DENSE_DX), has(BNPVI_DENSE_DW), has(BNPVI_DENSE_DB), has(BNPVI_DENSE_DRES), has(BNPVI_DENSE_STEP)};
   return (int64_t)(has(BNPVI_DENSE_BACKWARD) ? backward_plan(c).bytes : forward_plan(c).bytes);
 }
 
@@ -815,10 +821,10 @@ int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G,
   // not (a call that asks for less needs no more)
   int64_t most = 0;
   for (int off = 0; off < 8; ++off)
-    for (int given = 0; given < (backward ? 4 : 1); ++given) {
+    for (int given = 0; given < (backward ? 8 : 1); ++given) {
       const int call = (off & 1 ? BNPVI_DENSE_X_OFF : 0) | (off & 2 ? BNPVI_DENSE_W_OFF : 0) | (off & 4 ? BNPVI_DENSE_DY_OFF : 0);
       const int asked = BNPVI_DENSE_BACKWARD | BNPVI_DENSE_DX | BNPVI_DENSE_DB | BNPVI_DENSE_DRES | (given & 1 ? BNPVI_DENSE_DACT : 0) |
-                        (given & 2 ? 0 : BNPVI_DENSE_DW);
+                        (given & 2 ? 0 : BNPVI_DENSE_DW) | (given & 4 ? BNPVI_DENSE_STEP : 0);
       most = std::max(most, bnpvi_dense_workspace_for(dtype, M, K, n, G, backward ? call | asked : call));
     }
   return most;
@@ -919,12 +925,13 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
   return BNPVI_OK;
 }
 
-int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy, const void* dact, int64_t lddact, const void* x,
-                         int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const int32_t* offsets, int G, int64_t M, int64_t K,
+int bnpvi_dense_backward_act(bnpvi_ctx* ctx, int dtype, int activation, const void* dy, int64_t lddy, const void* dact, int64_t lddact,
+                             const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const int32_t* offsets, int G, int64_t M, int64_t K,
                          int64_t n, void* dx, int64_t lddx, void* dw, void* db, void* dres, int64_t lddres, void* work,
                          int64_t work_bytes, void* stream) {
   const int rc = check_dense("bnpvi_dense_backward", ctx, dtype, M, K, n, G, offsets);
   if (rc) return rc;
+  BNPVI_REQUIRE(activation >= -1 && activation <= BNPVI_ACT_GELU, "bnpvi_dense_backward: activation %d unknown", activation);
   BNPVI_REQUIRE(pitch_fits(lddy, n, dtype) && (!dact || lddact >= n) && (!dx || (pitch_fits(ldw, K, dtype) && lddx >= K)) &&
                     (!dw || pitch_fits(ldx, K, dtype)) && (!dres || lddres >= n),
                 "bnpvi_dense_backward: a row pitch is below its width, or above 4 MiB");
@@ -938,6 +945,7 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   c.dw = dw != nullptr;
   c.db = db != nullptr;
   c.dres = dres != nullptr;
+  c.step = dact && activation == BNPVI_ACT_RELU;
   const BackwardPlan p = backward_plan(c);
   BNPVI_REQUIRE(work_bytes >= (int64_t)p.bytes && (p.bytes == 0 || (work && (uintptr_t)work % 256 == 0)),
                 "bnpvi_dense_backward: workspace of %lld bytes (aligned to 256), %lld needed", (long long)work_bytes, (long long)p.bytes);
@@ -987,14 +995,8 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
   float* part = db && !p.db_in_dw && !p.db_in_dz ? (float*)(wk + p.part) : nullptr;
   if (p.dz_pass && !none) {
     void* out = p.write_dz ? (void*)(wk + p.dz) : nullptr;
-    if (dtype == BNPVI_F32)
-      launch_dz<float>((const float*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (float*)out, p.dz_pitch, (float*)dres, lddres, part, db_in_dz, s);
-    else if (dtype == BNPVI_BF16)
-      launch_dz<bf16_t>((const bf16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (bf16_t*)out, p.dz_pitch, (bf16_t*)dres, lddres, part,
-                        db_in_dz, s);
-    else
-      launch_dz<f16_t>((const f16_t*)dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, (f16_t*)out, p.dz_pitch, (f16_t*)dres, lddres, part, db_in_dz,
-                       s);
+    const auto launch = dtype == BNPVI_F32 ? launch_dz<float> : dtype == BNPVI_BF16 ? launch_dz<bf16_t> : launch_dz<f16_t>;
+    launch(p.pair, dy, lddy, dact, lddact, dz_map, M, (int)n, p.dz_tiles, out, p.dz_pitch, dres, lddres, part, db_in_dz, s);
     BNPVI_LAUNCH_CHECK();
     if (p.write_dz) {
       dz = out;
@@ -1101,6 +1103,14 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy
     }
   }
   return BNPVI_OK;
+}
+
+int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy, int64_t lddy, const void* dact, int64_t lddact, const void* x,
+                         int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const int32_t* offsets, int G, int64_t M, int64_t K,
+                         int64_t n, void* dx, int64_t lddx, void* dw, void* db, void* dres, int64_t lddres, void* work,
+                         int64_t work_bytes, void* stream) {
+  return bnpvi_dense_backward_act(ctx, dtype, -1, dy, lddy, dact, lddact, x, ldx, w, ldw, w_group, offsets, G, M, K, n, dx, lddx, dw, db, dres,
+                                  lddres, work, work_bytes, stream);
 }
 
 }  // extern "C"

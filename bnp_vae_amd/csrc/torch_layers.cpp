@@ -38,7 +38,7 @@ struct Library {
   decltype(&bnpvi_rows_from_leaves_backward) rows_from_leaves_backward;
   decltype(&bnpvi_dense_workspace_for) dense_workspace;
   decltype(&bnpvi_dense) dense;
-  decltype(&bnpvi_dense_backward) dense_backward;
+  decltype(&bnpvi_dense_backward_act) dense_backward;
 } lib;
 
 template <typename F>
@@ -60,7 +60,7 @@ void bind(const std::string& path) {
   find(h, "bnpvi_rows_from_leaves_backward", lib.rows_from_leaves_backward);
   find(h, "bnpvi_dense_workspace_for", lib.dense_workspace);
   find(h, "bnpvi_dense", lib.dense);
-  find(h, "bnpvi_dense_backward", lib.dense_backward);
+  find(h, "bnpvi_dense_backward_act", lib.dense_backward);
 }
 
 void check(int rc, const char* what) {
@@ -342,6 +342,7 @@ struct Dense : Function<Dense> {
     auto [y, dact] = dense_forward(x, w, bias.value_or(Tensor()), res.value_or(Tensor()), offsets, act, ctx, want_dact);
     c->save_for_backward({x, w, offsets, dact});
     c->saved_data["ctx"] = ctx;
+    c->saved_data["act"] = act;
     c->saved_data["given"] = (bias ? 1 : 0) + (res ? 2 : 0);          // only tensors that are there count as inputs
     return y;
   }
@@ -355,17 +356,18 @@ struct Dense : Function<Dense> {
     const Weights w = weights(w0);
     if (c->needs_input_grad(0)) dx = at::empty({M, K}, x.options());
     if (c->needs_input_grad(1)) dw = at::empty(w0.sizes(), x.options());
-    const int64_t has = c->saved_data["given"].toInt();
+    const int64_t has = c->saved_data["given"].toInt(), act = c->saved_data["act"].toInt();
     if ((has & 1) && c->needs_input_grad(2)) db = at::empty(w0.sizes().slice(0, w0.dim() - 1), x.options());
     const bool need_res = (has & 2) && c->needs_input_grad(2 + (has & 1));
     if (need_res && G) dres = at::empty({M, n}, x.options());
     if (dx.defined() || dw.defined() || db.defined() || dres.defined()) {
       const int call = BNPVI_DENSE_BACKWARD | off16(x, pitch(x), 0, K, BNPVI_DENSE_X_OFF) | off16(w.t, w.row, w.group, K, BNPVI_DENSE_W_OFF) |
-                       off16(dy, pitch(dy), 0, n, BNPVI_DENSE_DY_OFF) | (ptr(dact) ? BNPVI_DENSE_DACT : 0) | (ptr(dx) ? BNPVI_DENSE_DX : 0) |
+                       off16(dy, pitch(dy), 0, n, BNPVI_DENSE_DY_OFF) | (ptr(dact) ? BNPVI_DENSE_DACT : 0) |
+                       (ptr(dact) && act == BNPVI_ACT_RELU ? BNPVI_DENSE_STEP : 0) | (ptr(dx) ? BNPVI_DENSE_DX : 0) |
                        (dw.defined() ? BNPVI_DENSE_DW : 0) | (db.defined() ? BNPVI_DENSE_DB : 0) | (ptr(dres) ? BNPVI_DENSE_DRES : 0);
       const int64_t need = dense_workspace(type, M, K, n, G, call);
       if (need > 0) work = at::empty({need}, x.options().dtype(at::kByte));
-      check(lib.dense_backward(ctx_of(ctx), type, ptr(dy), pitch(dy), ptr(dact), n, ptr(x), pitch(x), ptr(w.t), w.row, w.group,
+      check(lib.dense_backward(ctx_of(ctx), type, static_cast<int>(act), ptr(dy), pitch(dy), ptr(dact), n, ptr(x), pitch(x), ptr(w.t), w.row, w.group,
                                ptr<int32_t>(offsets), G, M, K, n, ptr(dx), K, ptr(dw), ptr(db), ptr(dres), n, ptr(work), need, stream_of(x)),
             "bnpvi_dense_backward");
     }

@@ -380,7 +380,8 @@ enum {
   BNPVI_DENSE_DX = 32,      /* dx, dw, db, dres are asked for */
   BNPVI_DENSE_DW = 64,
   BNPVI_DENSE_DB = 128,
-  BNPVI_DENSE_DRES = 256
+  BNPVI_DENSE_DRES = 256,
+  BNPVI_DENSE_STEP = 512    /* dact is relu's: 0 and 1 only (bnpvi_dense_backward_act) */
 };
 int64_t bnpvi_dense_workspace(int dtype, int64_t M, int64_t K, int64_t n, int G, int backward);
 int64_t bnpvi_dense_workspace_for(int dtype, int64_t M, int64_t K, int64_t n, int G, int call);
@@ -393,6 +394,13 @@ int bnpvi_dense_backward(bnpvi_ctx* ctx, int dtype, const void* dy_dev, int64_t 
                          const int32_t* offsets_dev, int G, int64_t M, int64_t K, int64_t n, void* dx_dev, int64_t lddx,
                          void* dw_dev, void* db_dev, void* dres_dev, int64_t lddres, void* work_dev, int64_t work_bytes,
                          void* stream);
+/* The same where dact's activation is known (BNPVI_ACT_*, or -1): relu's holds 0 and 1 only, so that dz has the 16 bits of
+ * dy and needs no second part, which halves the products of dx and dw. */
+int bnpvi_dense_backward_act(bnpvi_ctx* ctx, int dtype, int activation, const void* dy_dev, int64_t lddy, const void* dact_dev,
+                             int64_t lddact, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int64_t w_group,
+                             const int32_t* offsets_dev, int G, int64_t M, int64_t K, int64_t n, void* dx_dev, int64_t lddx,
+                             void* dw_dev, void* db_dev, void* dres_dev, int64_t lddres, void* work_dev, int64_t work_bytes,
+                             void* stream);
 
 #ifdef __cplusplus
 }

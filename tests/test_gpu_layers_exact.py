@@ -181,3 +181,66 @@ def test_dense_gradients_against_differences(layers, act):
             # act' to 16 half steps beside 1 and 2 |act''| <= 4 times z's own error, sums of at most 6 terms
             kernel = float((row * reach).sum()) * (16 * 2.0 ** -24 + 4 * 22 * 2.0 ** -23 * 8 + 22 * 2.0 ** -23)
             assert abs(slope - float(g.view(-1)[j].cpu())) <= float((row * reach ** 3).sum()) * h * h + kernel
+
+
+# ------------------------------------------------------------------------------------------------ the C entry points
+def backward(layers, activation, dtype, dy, dact, x, w, offsets, G):
+    """bnpvi_dense_backward, or with an activation bnpvi_dense_backward_act: dx, dw, db."""
+    import ctypes as C
+    lib, p = layers.lib, lambda t: None if t is None else C.c_void_p(t.data_ptr())
+    (M, K), n = x.shape, w.shape[-2]
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty(w.shape[:-1], dtype=x.dtype, device="cuda")
+    need = lib.bnpvi_dense_workspace(dtype, M, K, n, G, 1)
+    work = torch.full((need,), 0x7f, dtype=torch.uint8, device="cuda")
+    args = [p(dy), n, p(dact), n, p(x), K, p(w), K, n * K, p(offsets), G, M, K, n, p(dx), K, p(dw), p(db), None, 0, p(work), need,
+            C.c_void_p(torch.cuda.current_stream().cuda_stream)]
+    ctx = C.c_void_p(layers._ctx(x.device))
+    if activation is None:
+        rc = lib.bnpvi_dense_backward(ctx, dtype, *args)
+    else:
+        rc = lib.bnpvi_dense_backward_act(ctx, dtype, activation, *args)
+    assert rc == 0, lib.bnpvi_last_error()
+    return dx, dw, db
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("M,K,n,sizes", [
+    (40000, 1024, 1024, None), (20000, 4096, 256, None), (16384, 512, 512, None), (5000, 264, 520, None), (300, 2048, 512, None),
+    (40, 24, 33, None), (70000, 64, 32, None), (7000, 1001, 601, None), (600, 37, 41, None), (31, 1024, 70, None),
+    (60000, 512, 512, [40000, 0, 9000, 1, 10990]), (60000, 512, 512, some_sizes(64, 60000, 1)), (51200, 512, 512, [200] * 256),
+    (15000, 64, 96, some_sizes(3000, 15000, 4)), (20000, 301, 203, some_sizes(5, 20000, 5)), (5052, 1574, 89, some_sizes(26, 5052, 10)),
+    (20000, 86, 41, some_sizes(10, 20000, 13))])
+def test_both_parts_of_dz_are_exact(layers, dtype, M, K, n, sizes):
+    """act'(z) given as multiples of 2^-8 up to 16, so that dz needs 12 bits: two parts hold it, one does not; all sums are
+    below 2^24 of these steps.  What a forward pass would give is no matter here."""
+    T, code = TYPES[dtype], {"bf16": 1, "f16": 2}[dtype]
+    lead = (len(sizes),) if sizes else ()
+    x, w, dy = whole((M, K), 1, T, 1), whole(lead + (n, K), 1, T, 2), whole((M, n), 2, T, 3)
+    x, w = x * (whole((M, K), 3, T, 4) == 0), w * (whole(lead + (n, K), 3, T, 5) == 0)          # mostly zeros: shorter sums
+    dact = whole((M, n), 4095, torch.float32, 6) / 256
+    bounds = [0, M] if sizes is None else [int(v) for v in np.concatenate([[0], np.cumsum(sizes)])]
+    off = torch.tensor(bounds, dtype=torch.int32, device="cuda") if sizes else None
+    dx, dw, db = backward(layers, None, code, dy, dact, x, w, off, len(sizes or ()))
+    dz = dy.double() * dact.double()
+    assert float((dz.to(T).double() != dz).double().mean()) > 0.01
+    for g in range(len(bounds) - 1):
+        rows, at = slice(bounds[g], bounds[g + 1]), g if sizes else slice(None)
+        for name, got, want in (("dx", dx[rows], dz[rows] @ w[at].double()), ("dw", dw[at], dz[rows].t().contiguous() @ x[rows].double()),
+                                ("db", db[at], dz[rows].sum(0))):
+            assert float(want.abs().max() if want.numel() else 0) < 2 ** 16, name
+            assert torch.equal(got, want.to(T)), (name, g, int((got != want.to(T)).sum()))
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("sizes", [None, [70, 0, 400, 29]])
+def test_a_named_activation_changes_no_bit(layers, dtype, sizes):
+    """relu's dz has the bits of dy, with and without a second part; other activations go the same way named or not."""
+    T = (torch.float32, torch.bfloat16, torch.float16)[dtype]
+    M, K, n, G = 500, 72, 136, len(sizes or ())
+    lead = (G,) if G else ()
+    x, w, dy = whole((M, K), 2, T, 1), whole(lead + (n, K), 2, T, 2), whole((M, n), 2, T, 3)
+    off = None if sizes is None else torch.tensor([0] + [int(v) for v in np.cumsum(sizes)], dtype=torch.int32, device="cuda")
+    for activation, dact in ((1, whole((M, n), 1, torch.float32, 4).abs()), (5, torch.rand((M, n), device="cuda")), (-1, None)):
+        for a, b in zip(backward(layers, None, dtype, dy, dact, x, w, off, G), backward(layers, activation, dtype, dy, dact, x, w, off, G)):
+            rows = slice(0, sum(sizes)) if sizes and a.shape[0] == M else slice(None)
+            assert torch.equal(a[rows], b[rows])

@@ -170,7 +170,7 @@ def test_recorders_of_torch_calls_are_refused():
             make_fx(call)(t)
 
 
-X_OFF, W_OFF, DY_OFF, DACT, DX, DW, DB, DRES = (1 << i for i in range(1, 9))
+X_OFF, W_OFF, DY_OFF, DACT, DX, DW, DB, DRES, STEP = (1 << i for i in range(1, 10))
 
 
 def _need(dtype, M, K, n, G, *bits):
@@ -190,6 +190,7 @@ def test_a_dense_call_needs_no_copy_of_what_lies():
     assert _need(1, M, K, n, 0, X_OFF, *asked) >= M * K * e                   # where x is off 16 bytes its copy pays
     assert _need(0, 16385, 64, 4096, 0, *asked) < 16385 * 4096 * 4            # dz is dy
     assert _need(1, 32768, 1024, 1024, 0) == 0 and _need(1, 32768, 1024, 1024, 0, X_OFF) == 32768 * 1024 * e
+    assert _need(1, M, K, n, 0, DACT, STEP, *asked) <= dw_parts + db_parts + M * n * e + 4096      # relu: dz in one part
     assert _need(1, M, K, n, 0, 1, DACT, DB) <= db_parts + 4096               # the bias alone: no dz either
     assert _need(5, 1, 1, 1, 0) == -1 and _need(0, 1, 0, 1, 0, 1) == -1
 
@@ -197,11 +198,11 @@ def test_a_dense_call_needs_no_copy_of_what_lies():
 def test_the_workspace_of_all_calls_is_enough_for_each():
     import random
     rng = random.Random(3)
-    for _ in range(300):
+    for _ in range(150):
         dtype, G = rng.randrange(3), rng.choice([0, 0, 1, 5, 64])
         M, K, n = (int(2 ** rng.uniform(0, t)) for t in (16, 12, 12))
         most = [_lib.lib.bnpvi_dense_workspace(dtype, M, K, n, G, b) for b in (0, 1)]
-        for call in range(512):
+        for call in range(1024):
             assert _need(dtype, M, K, n, G, call) <= most[call & 1], (dtype, M, K, n, G, call)
 
 
