@@ -509,7 +509,7 @@ static void tile_size(int tile, int& br, int& bc) {
 // rate), and a tile its first load and its epilogue.  65536 x 4096 -> 256: 207 us in tiles of 128, 173 in tiles of 256;
 // 16384 x 512 -> 512: 15 us in tiles of 128, 22 in tiles of 256; 256 leaves of 200 rows, 512 -> 512: 80 and 102.
 // Splitting the sum costs a launch and two passes over the parts.  Transposing reads cost the large tile's stages a tenth
-// more (8192^3: 938 / 1035 / 1100 us forward, dx, dW).
+// more (8192^3: 922 / 1044 / 1002 us forward, dx, dW).
 //
 // Narrow results take the tall tile (50000 x 1024 -> 32: 19 us in bf16 and 55 in fp32, tiles of 64: 22 and 81), few rows the
 // flat one, and so do small leaves, whose last tile is half empty on average (256 leaves of 40 / 96 / 128 rows, 512 -> 512 in

@@ -18,7 +18,7 @@
 //
 // What bounds it.  A wave tile of 128 x 64 needs 6 KB of fragments for 8 instructions: of the LDS's 128 bytes a cycle the
 // fragments take three quarters and the arriving stages the rest, so that matrix pipe and LDS are full at the same time,
-// and 8192^3 in bf16 runs at 1170 / 1065 / 1050 TFLOP/s (forward, dx, dW; the library 1430; without the loads 1460).  Where
+// and 8192^3 in bf16 runs at 1190 / 1050 / 1100 TFLOP/s (forward, dx, dW; the library's forward 1640, on another card 1430).  Where
 // the sum is short the epilogue counts: dx of 65536 x 256 -> 4096 takes 200 us, 95 of them its 537 MB of stores alone, 60
 // the products, and a tile's stores and the next one's products share the time only as far as its loads reach ahead.
 // 65536 x 4096 -> 256 forward reads 537 MB in 150 us (3.6 TB/s, a copy 4.7).  fp32 is bound by its matrix rate: 135 of 157
@@ -362,8 +362,8 @@ __device__ __forceinline__ void wait_loads() {
 // a single rounding of the results (0.0024 against 0.0017 relative in bf16).  A row of it holds 32 columns of hi, 32 of lo,
 // and so on, so that a stage is as many bytes as ever, of half as many k's (dx) or of both parts of its columns (dW); S's
 // stages are half as long, and each of its fragments is multiplied with both parts.  That is twice the
-// instructions: 65536 x 4096 -> 256 in bf16 takes 282 / 300 us for dx / dW, from one part 200 / 175; 32768 x 1024 -> 1024 takes
-// 135 / 148, from one part 82 / 92 (920 to 1020 TFLOP/s of the doubled products).
+// instructions: 65536 x 4096 -> 256 in bf16 takes 287 / 303 us for dx / dW, from one part 203 / 175; 32768 x 1024 -> 1024 takes
+// 136 / 151, from one part 84 / 92 (910 to 1010 TFLOP/s of the doubled products).
 template <int KIND, bool PAIR, int BR, int BC, int KB>
 struct Stages {
   static constexpr bool kRKM = KIND != kDw, kSKM = KIND == kFwd;

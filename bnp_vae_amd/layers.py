@@ -225,7 +225,8 @@ def dense(x, weight, bias=None, activation=None, residual=None, offsets=None):
     of x (M, K) use weight[g] and bias[g]; rows of no group give 0, take no part in any gradient, and what x and residual
     hold there is not looked at.
     activation: None, "relu", "softsign", "tanh", "silu", "gelu" (with the normal distribution function).
-    Sums in fp32, one rounding of y; for the backward pass act'(z) is kept beside y where there is an activation."""
+    Sums in fp32, one rounding of y and of each gradient; for the backward pass act'(z) is kept in fp32 beside y where there
+    is an activation."""
     device = _on_gpu("dense", x=x, weight=weight, bias=bias, residual=residual, offsets=offsets)
     if activation not in ACTIVATIONS:
         raise ValueError("dense: activation %r unknown (%s)" % (activation, ", ".join(str(a) for a in ACTIVATIONS)))
