@@ -926,9 +926,9 @@ int bnpvi_dense(bnpvi_ctx* ctx, int dtype, const void* x, int64_t ldx, const voi
 }
 
 int bnpvi_dense_backward_act(bnpvi_ctx* ctx, int dtype, int activation, const void* dy, int64_t lddy, const void* dact, int64_t lddact,
-                             const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const int32_t* offsets, int G, int64_t M, int64_t K,
-                         int64_t n, void* dx, int64_t lddx, void* dw, void* db, void* dres, int64_t lddres, void* work,
-                         int64_t work_bytes, void* stream) {
+                             const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t w_group, const int32_t* offsets, int G,
+                             int64_t M, int64_t K, int64_t n, void* dx, int64_t lddx, void* dw, void* db, void* dres, int64_t lddres,
+                             void* work, int64_t work_bytes, void* stream) {
   const int rc = check_dense("bnpvi_dense_backward", ctx, dtype, M, K, n, G, offsets);
   if (rc) return rc;
   BNPVI_REQUIRE(activation >= -1 && activation <= BNPVI_ACT_GELU, "bnpvi_dense_backward: activation %d unknown", activation);

@@ -1045,3 +1045,16 @@ def test_gradients_that_arrive_as_negated_views(layers):
         want = torch.autograd.grad((call() * k.imag).sum(), leaves)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(seen)
+
+
+def test_tensors_without_memory_are_errors(layers):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x, w = gpu(rand((6, 8), torch.float32, 1)), gpu(rand((5, 8), torch.float32, 2))
+    leaf = torch.zeros(6, dtype=torch.int32, device="cuda")
+    plan = layers.sort_by_leaf(leaf, 1)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fx, fw, fleaf = (mode.from_tensor(t) for t in (x, w, leaf))
+        for call in (lambda: layers.dense(fx, fw), lambda: layers.dense(x, w), lambda: layers.dispatch(fx, plan), lambda: layers.combine(fx, plan),
+                     lambda: layers.top_leaves(fx, 2), lambda: layers.sort_by_leaf(fleaf, 1)):
+            with pytest.raises(RuntimeError):
+                call()

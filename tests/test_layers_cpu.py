@@ -227,3 +227,12 @@ def test_orders_of_other_shapes_types_and_devices_are_refused():
     for o in (None, [0] * 8):
         with pytest.raises(TypeError, match="order"):
             layers.LeafPlan(place, o, offsets, 3)
+
+
+def test_a_backward_call_names_a_known_activation():
+    c, one = _Ctx(), C.c_void_p(256)
+    for activation in (-2, 6):
+        _fails(_lib.lib.bnpvi_dense_backward_act(c.p, 0, activation, one, 6, one, 6, one, 8, one, 8, 0, None, 0, 4, 8, 6, one, 8, one, one,
+                                                 None, 0, one, 1 << 40, None), "activation")
+    _fails(_lib.lib.bnpvi_dense_backward_act(c.p, 0, 1, one, 6, one, 6, one, 8, one, 8, 0, None, 0, 4, 8, 6, one, 8, one, one,
+                                             None, 0, one, 0, None), "workspace")
